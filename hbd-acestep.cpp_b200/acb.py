@@ -72,6 +72,13 @@ def lib():
             "acb_gemv": (I, [P, I, I64, I64, I, I, P, I64, P, F, I, P, I64, I, P, I64, I, P, P]),
             "acb_q8_0_to_tiles": (I, [P, P, I64, I64, P]),
             "acb_qkv_post": (I, [P, I64, I64, I, I, I, P, P, F, P, P, I, P, I64, P, P, I, I, I, I, P, P]),
+            "acb_rope_table_scaled_host": (I, [P, I, I, F, I, F, I, F, F]),
+            "acb_rope": (I, [P, I64, I64, P, I64, I64, I, I64, I, I, I, I, P, P, I, P, P]),
+            "acb_kv_q4_append": (I, [P, P, I, I64, I64, I, P, P, F, P, I, I, I, P, P, P, I, I64, P, P]),
+            "acb_kv_q4_read": (I, [P, P, P, I64, P, P, I, I64, P, P]),
+            "acb_attn_kv_q4_work_bytes": (C.c_size_t, [P, I64, I, I, I]),
+            "acb_attn_kv_q4": (I, [P, P, I, I64, I64, I, P, P, I, I, I, F, P, I64, P, C.c_size_t, P, P]),
+            "acb_logits_rules": (I, [P, I, I64, P, I, I64, I, I64, P, P, P]),
             "acb_attn_decode_splits": (I, [I, I]),
             "acb_attn_decode": (I, [P, I64, I, I, I, I, P, P, P, I, I, I, F, I, P, P, P, P, I64, P, I, P]),
             "acb_argmax_scratch_bytes": (C.c_size_t, [I, I64]),
@@ -371,6 +378,235 @@ def argmax(logits, ids, margin=None, pos_advance=None, scratch=None, flags=0, st
                                            _ptr(pos_advance), None, None, 0, None, _ptr(scratch), flags,
                                            _stream(stream)))
     return scratch
+
+
+# ---- serving: rotary layouts, the paged 4-bit KV cache, rules on logits -------------------------
+
+ROPE_HALF, ROPE_INTERLEAVED, ROPE_INVERSE = 0, 1, 2
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_NTK, ROPE_SCALE_YARN = 0, 1, 2, 3
+_ROPE_LAYOUT = {"half": ROPE_HALF, "interleaved": ROPE_INTERLEAVED}
+
+
+def _run_on(name, t, stream, *args):
+    """The entry point `name` on the device that holds t, on its current stream unless one is given."""
+    import torch
+    dev = t.device
+    if dev.type != "cuda":
+        raise ValueError(f"{name}: tensors on the GPU are wanted, got {dev}")
+    fn = getattr(lib(), name)
+    if dev.index == torch.cuda.current_device():
+        st = fn(*args, _stream(stream))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, _stream(stream))
+    if st != 0:
+        raise AcbError(name, st)
+
+
+def _want(name, t, dtype, dev, contiguous=True, numel=None):
+    """Refuses a tensor that the kernels would misread: another type, another device, gaps, too few elements."""
+    if t is None:
+        return
+    if t.dtype is not dtype or t.device != dev or (contiguous and not t.is_contiguous()) or \
+            (numel is not None and t.numel() < numel):
+        raise ValueError(f"{name}: a {'contiguous ' if contiguous else ''}{dtype} tensor on {dev}"
+                         f"{'' if numel is None else f' of {numel} elements or more'} is wanted, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+
+
+def rope_table_scaled(max_pos, rope_dim, base, kind=ROPE_SCALE_NONE, factor=1.0, orig_max_pos=0, beta_fast=32.0,
+                      beta_slow=1.0):
+    """Host table [max_pos, rope_dim] for a context longer than the trained one (angles in double)."""
+    import torch
+    t = torch.empty((max_pos, rope_dim), dtype=torch.float32)
+    _check("acb_rope_table_scaled_host", lib().acb_rope_table_scaled_host(
+        t.data_ptr(), max_pos, rope_dim, base, kind, factor, orig_max_pos, beta_fast, beta_slow))
+    return t
+
+
+def rope(x, pos, table, layout="half", inverse=False, out=None, err=None, stream=None):
+    """x [T, H, D] (any token and head strides) rotated by pos [T] int32 over the table's width; out may be x."""
+    import torch
+    T, H, D = x.shape
+    if out is None:
+        out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
+    if out.dtype is not x.dtype or out.shape != x.shape or x.stride(2) != 1 or out.stride(2) != 1:
+        raise ValueError("rope: x and out have one type and shape, their last dimension contiguous")
+    _want("rope: pos", pos, torch.int32, x.device, numel=T)
+    _want("rope: table", table, torch.float32, x.device)
+    if x.numel() == 0:
+        return out
+    _run_on("acb_rope", x, stream, x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+            dtype_id(x), T, H, D, table.shape[1], _ROPE_LAYOUT[layout] | (ROPE_INVERSE if inverse else 0), pos.data_ptr(),
+            table.data_ptr(), table.shape[0], _ptr(err))
+    return out
+
+
+class _KvQ4(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_codes", C.c_void_p), ("v_scales", C.c_void_p),
+                ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("n_seq", C.c_int32), ("max_pages", C.c_int32)]
+
+
+class KVCacheQ4:
+    """A paged KV cache in 4 bits (acb_kv_q4) over the caller's tensors: codes uint8 [n_pages, n_kv_heads, page_size, D/2],
+    scales float16 [n_pages, n_kv_heads, page_size, D/32] of keys and values, page_table int32 [n_seq, max_pages]."""
+
+    def __init__(self, k_codes, k_scales, v_codes, v_scales, page_table):
+        import torch
+        n_pages, n_kv, page, half = k_codes.shape
+        dev = k_codes.device
+        for n, t in (("k_codes", k_codes), ("v_codes", v_codes)):
+            _want("KVCacheQ4: " + n, t, torch.uint8, dev)
+        for n, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+            _want("KVCacheQ4: " + n, t, torch.float16, dev)
+        _want("KVCacheQ4: page_table", page_table, torch.int32, dev, contiguous=False)
+        if v_codes.shape != k_codes.shape or page_table.dim() != 2 or (page_table.shape[1] > 1 and page_table.stride(1) != 1) \
+                or any(s.shape != (n_pages, n_kv, page, half // 16) for s in (k_scales, v_scales)):
+            raise ValueError("KVCacheQ4: codes [n_pages, n_kv_heads, page_size, D/2], scales [.., D/32], table [n_seq, max_pages]")
+        self.tensors = (k_codes, k_scales, v_codes, v_scales, page_table)
+        self.n_kv_heads, self.head_dim, self.n_seq = n_kv, 2 * half, page_table.shape[0]
+        self.c = _KvQ4(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+                       page_table.data_ptr(), max(page_table.stride(0), page_table.shape[1]), n_pages, page, n_kv, 2 * half,
+                       self.n_seq, page_table.shape[1])
+        self.device = dev
+        self.ref = C.addressof(self.c)
+
+    @classmethod
+    def empty(cls, n_pages, page_size, n_kv_heads, head_dim, page_table):
+        """A pool of n_pages zeroed pages on the table's device."""
+        import torch
+        mk = lambda n, t: torch.zeros((n_pages, n_kv_heads, page_size, n), dtype=t, device=page_table.device)  # noqa: E731
+        return cls(mk(head_dim // 2, torch.uint8), mk(head_dim // 32, torch.float16), mk(head_dim // 2, torch.uint8),
+                   mk(head_dim // 32, torch.float16), page_table)
+
+    def append(self, qkv, n_heads, seq, pos, table=None, layout="half", q_norm=None, k_norm=None, eps=1e-6, q_out=None,
+               q_dtype=None, err=None, stream=None):
+        """qkv [T, (n_heads + 2 n_kv_heads) D] (rows may be strided): norm and rotation of q and k, q returned [T, n_heads, D],
+        k and v quantised into positions pos [T] of sequences seq [T] (int32; seq < 0: padding)."""
+        import torch
+        T, D, dev = qkv.shape[0], self.head_dim, qkv.device
+        if dev != self.device or qkv.stride(1) != 1 or qkv.shape[1] < (n_heads + 2 * self.n_kv_heads) * D:
+            raise ValueError("KVCacheQ4.append: qkv [T, (n_heads + 2 n_kv_heads) * head_dim] on the cache's device is wanted")
+        _want("KVCacheQ4.append: seq", seq, torch.int32, dev, numel=T)
+        _want("KVCacheQ4.append: pos", pos, torch.int32, dev, numel=T)
+        _want("KVCacheQ4.append: table", table, torch.float32, dev)
+        _want("KVCacheQ4.append: q_norm", q_norm, torch.float32, dev, numel=D)
+        _want("KVCacheQ4.append: k_norm", k_norm, torch.float32, dev, numel=D)
+        if n_heads > 0 and q_out is None:
+            q_out = torch.empty((T, n_heads, D), dtype=q_dtype or qkv.dtype, device=dev)
+        if n_heads > 0 and (q_out.shape != (T, n_heads, D) or q_out.stride(2) != 1 or q_out.stride(1) != D or q_out.device != dev):
+            raise ValueError("KVCacheQ4.append: q_out [T, n_heads, head_dim] with contiguous rows is wanted")
+        if T == 0:
+            return q_out
+        mp, rd = table.shape if table is not None else (0, 0)
+        _run_on("acb_kv_q4_append", qkv, stream, self.ref, qkv.data_ptr(), dtype_id(qkv), max(qkv.stride(0), qkv.shape[1]), T,
+                n_heads, _ptr(q_norm), _ptr(k_norm), eps, _ptr(table), mp, rd, _ROPE_LAYOUT[layout], seq.data_ptr(),
+                pos.data_ptr(), _ptr(q_out), dtype_id(q_out if q_out is not None else qkv),
+                max(q_out.stride(0), n_heads * D) if q_out is not None else 0, _ptr(err))
+        return q_out
+
+    def read(self, seq, pos, k_out=None, v_out=None, dtype=None, err=None, stream=None):
+        """The cached keys and values at (seq, pos) as [T, n_kv_heads, D]: both when neither output is given."""
+        import torch
+        T, shape = seq.numel(), (seq.numel(), self.n_kv_heads, self.head_dim)
+        _want("KVCacheQ4.read: seq", seq, torch.int32, self.device)
+        _want("KVCacheQ4.read: pos", pos, torch.int32, self.device, numel=T)
+        if k_out is None and v_out is None:
+            k_out = torch.empty(shape, dtype=dtype or torch.float16, device=self.device)
+            v_out = torch.empty_like(k_out)
+        first = k_out if k_out is not None else v_out
+        for t in (k_out, v_out):
+            if t is not None and (t.shape != shape or t.dtype is not first.dtype or t.stride() != first.stride()
+                                  or t.stride(2) != 1 or t.stride(1) != self.head_dim or t.device != self.device):
+                raise ValueError("KVCacheQ4.read: outputs [T, n_kv_heads, head_dim] of one type with contiguous rows are wanted")
+        if T == 0:
+            return k_out, v_out
+        _run_on("acb_kv_q4_read", seq, stream, self.ref, seq.data_ptr(), pos.data_ptr(), T, _ptr(k_out), _ptr(v_out),
+                dtype_id(first), max(first.stride(0), shape[1] * shape[2]), _ptr(err))
+        return k_out, v_out
+
+    def attn_workspace(self, n_tok, n_heads, max_q_len, max_kv_len):
+        """A workspace for attention() calls of at most these sizes (None where they need none)."""
+        import torch
+        n = lib().acb_attn_kv_q4_work_bytes(self.ref, n_tok, n_heads, max_q_len, max_kv_len)
+        return torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+
+    def attention(self, q, kv_len, q_start=None, max_q_len=1, max_kv_len=None, window=0, scale=None, out=None, work=None,
+                  err=None, stream=None):
+        """q [T, n_heads, D]: causal attention of every sequence's new rows (q_start [n_seq + 1], None: one row each) over its
+        kv_len [n_seq] cached tokens. max_kv_len None: as many as the page table can hold. work: attn_workspace()'s (made
+        here when None)."""
+        import torch
+        T, H, D = q.shape
+        dev, c = q.device, self.c
+        if max_kv_len is None:
+            max_kv_len = c.max_pages * c.page_size
+        if dev != self.device or D != self.head_dim or q.stride(2) != 1 or q.stride(1) != D:
+            raise ValueError("KVCacheQ4.attention: q [T, n_heads, head_dim] with contiguous rows on the cache's device is wanted")
+        _want("KVCacheQ4.attention: kv_len", kv_len, torch.int32, dev, numel=self.n_seq)
+        _want("KVCacheQ4.attention: q_start", q_start, torch.int32, dev, numel=self.n_seq + 1)
+        if out is None:
+            out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+        if out.dtype is not q.dtype or out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != D or out.device != dev:
+            raise ValueError("KVCacheQ4.attention: out of q's type and shape with contiguous rows is wanted")
+        if T == 0:
+            return out
+        if work is None:
+            work = self.attn_workspace(T, H, max_q_len, max_kv_len)
+        _run_on("acb_attn_kv_q4", q, stream, self.ref, q.data_ptr(), dtype_id(q), max(q.stride(0), H * D), T, H, _ptr(q_start),
+                kv_len.data_ptr(), max_q_len, max_kv_len, window, D ** -0.5 if scale is None else scale, out.data_ptr(),
+                max(out.stride(0), H * D), _ptr(work), work.numel() * work.element_size() if work is not None else 0, _ptr(err))
+        return out
+
+
+class _LogitRules(C.Structure):
+    _fields_ = [("hist", C.c_void_p), ("hist_stride", C.c_int64), ("hist_len", C.c_void_p), ("prompt_len", C.c_void_p),
+                ("rep", C.c_void_p), ("freq", C.c_void_p), ("pres", C.c_void_p), ("bias_ids", C.c_void_p),
+                ("bias_val", C.c_void_p), ("bias_stride", C.c_int64), ("n_bias", C.c_int32), ("n_masks", C.c_int32),
+                ("mask", C.c_void_p), ("mask_stride", C.c_int64), ("mask_row", C.c_void_p)]
+
+
+def logits_rules(logits, hist=None, hist_len=None, prompt_len=None, rep=None, freq=None, pres=None, bias_ids=None,
+                 bias_val=None, mask=None, mask_row=None, out=None, out_dtype=None, err=None, stream=None):
+    """logits [R, V] after the rules of acb_logits_rules: hist int32 [R, L] with hist_len / prompt_len int32 [R], rep / freq /
+    pres float32 [R], bias_ids int32 and bias_val float32 [R, n] (or [n]: the same for every row), mask int32 words
+    [n_masks, >= V/32] with mask_row int32 [R]. out may be logits."""
+    import torch
+    R, V = logits.shape
+    dev, i32, f32 = logits.device, torch.int32, torch.float32
+    if out is None:
+        out = torch.empty((R, V), dtype=out_dtype or logits.dtype, device=dev)
+    if out.shape != logits.shape or out.device != dev or logits.stride(1) != 1 or out.stride(1) != 1:
+        raise ValueError("logits_rules: logits and out [R, V] with contiguous rows are wanted")
+    for n, t, d in (("hist_len", hist_len, i32), ("prompt_len", prompt_len, i32), ("rep", rep, f32), ("freq", freq, f32),
+                    ("pres", pres, f32), ("mask_row", mask_row, i32)):
+        _want("logits_rules: " + n, t, d, dev, numel=R)
+    if R == 0:
+        return out
+    r = _LogitRules(mask_row=_ptr(mask_row))
+    if hist is not None:
+        _want("logits_rules: hist", hist, i32, dev)
+        if hist.dim() != 2 or hist.shape[0] < R:
+            raise ValueError("logits_rules: hist [R, L] is wanted")
+    elif rep is not None or freq is not None or pres is not None:
+        raise ValueError("logits_rules: penalties go by a history")
+    if hist is not None and hist.shape[1] > 0:
+        r.hist, r.hist_stride, r.hist_len, r.prompt_len = hist.data_ptr(), hist.shape[1], _ptr(hist_len), _ptr(prompt_len)
+        r.rep, r.freq, r.pres = _ptr(rep), _ptr(freq), _ptr(pres)
+    if bias_ids is not None and bias_ids.numel() > 0:
+        _want("logits_rules: bias_ids", bias_ids, i32, dev)
+        _want("logits_rules: bias_val", bias_val, f32, dev, numel=bias_ids.numel())
+        r.bias_ids, r.bias_val, r.n_bias = bias_ids.data_ptr(), _ptr(bias_val), bias_ids.shape[-1]
+        r.bias_stride = r.n_bias if bias_ids.dim() == 2 else 0
+        if bias_ids.dim() == 2 and bias_ids.shape[0] < R:
+            raise ValueError("logits_rules: a bias list for every row, or one for all, is wanted")
+    if mask is not None:
+        _want("logits_rules: mask", mask, i32, dev)
+        r.mask, r.n_masks, r.mask_stride = mask.data_ptr(), mask.shape[0], mask.shape[1]
+    _run_on("acb_logits_rules", logits, stream, logits.data_ptr(), dtype_id(logits), max(logits.stride(0), V), out.data_ptr(),
+            dtype_id(out), max(out.stride(0), V), R, V, C.addressof(r), _ptr(err))
+    return out
 
 
 # ---- model level ----------------------------------------------------------------------------------

@@ -1,0 +1,159 @@
+// k_rope.cu -- rotary positions in every layout (acb_rope) and the table of angles for contexts longer than
+// the trained one (acb_rope_table_scaled_host).
+//
+// With z = a + i b for a pair and w = c + i s its table entry, the rotation is z' = z w (w's conjugate for the
+// inverse): 6 flops on 2 elements against a read and a write of both, so the memory bounds it.
+#include <math.h>
+
+#include "common.cuh"
+
+namespace acb {
+namespace {
+
+struct RopeArgs {
+    const void *    src;
+    int64_t         sts, shs;
+    void *          dst;
+    int64_t         dts, dhs;
+    int64_t         n_tok;
+    int             n_heads, D, R;
+    const int32_t * pos;
+    const float *   table;
+    int             max_pos;
+    int *           err;
+    bool            half, inverse, in_place;
+};
+
+// one warp per (token, head), a lane per pair
+template <int T> __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
+    using E            = typename io<T>::t;
+    const int     lane = threadIdx.x & 31;
+    const int64_t item = (int64_t) blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    if (item >= a.n_tok * a.n_heads) {
+        return;
+    }
+    const int64_t t = item / a.n_heads;
+    const int     h = (int) (item - t * a.n_heads);
+    const E *     x = reinterpret_cast<const E *>(a.src) + t * a.sts + h * a.shs;
+    E *           y = reinterpret_cast<E *>(a.dst) + t * a.dts + h * a.dhs;
+    const int     p = __ldg(a.pos + t);
+    if (p < 0 || p >= a.max_pos) {
+        if (lane == 0 && a.err) {
+            atomicOr(a.err, ACB_DEVERR_POS_RANGE);
+        }
+        for (int i = lane; i < a.D; i += 32) {
+            y[i] = io<T>::from_f(0.0f);
+        }
+        return;
+    }
+    const float * w = a.table + (int64_t) p * a.R;
+    for (int i = lane; i < a.R / 2; i += 32) {
+        const float c  = __ldg(w + 2 * i);
+        const float s  = a.inverse ? -__ldg(w + 2 * i + 1) : __ldg(w + 2 * i + 1);
+        const int   ia = a.half ? i : 2 * i, ib = a.half ? i + a.R / 2 : 2 * i + 1;
+        const float u = io<T>::to_f(x[ia]), v = io<T>::to_f(x[ib]);
+        y[ia] = io<T>::from_f(__fsub_rn(__fmul_rn(u, c), __fmul_rn(v, s)));
+        y[ib] = io<T>::from_f(__fadd_rn(__fmul_rn(u, s), __fmul_rn(v, c)));
+    }
+    if (!a.in_place) {
+        for (int i = a.R + lane; i < a.D; i += 32) {
+            y[i] = x[i];
+        }
+    }
+}
+
+}  // namespace
+}  // namespace acb
+
+using namespace acb;
+
+extern "C" acb_status acb_rope(const void * src, int64_t src_tok_stride, int64_t src_head_stride, void * dst,
+                               int64_t dst_tok_stride, int64_t dst_head_stride, int type, int64_t n_tok, int n_heads,
+                               int head_dim, int rope_dim, int layout, const int32_t * pos, const float * rope_table,
+                               int max_pos, int * err_flag, acb_stream_t stream) {
+    if (!src || !dst || !pos || !rope_table || n_tok < 0 || n_heads <= 0 || max_pos <= 0 || src_tok_stride < 0 ||
+        dst_tok_stride < 0 || src_head_stride < 0 || dst_head_stride < 0 || head_dim <= 0 || head_dim % 2 != 0 ||
+        rope_dim < 2 || rope_dim > head_dim || rope_dim % 2 != 0 || layout < 0 || layout > 3) {
+        return ACB_ERR_INVALID_ARG;
+    }
+    // one buffer in two layouts would be written before it is read
+    const bool in_place = src == dst;
+    if (in_place && (src_tok_stride != dst_tok_stride || src_head_stride != dst_head_stride)) {
+        return ACB_ERR_INVALID_ARG;
+    }
+    // the destination's rows lie apart: tokens of heads or heads of tokens
+    const bool    toks  = dst_tok_stride >= dst_head_stride;
+    const int64_t inner = toks ? dst_head_stride : dst_tok_stride, outer = toks ? dst_tok_stride : dst_head_stride;
+    const int64_t n_in = toks ? n_heads : n_tok, n_out = toks ? n_tok : n_heads;
+    if ((n_in > 1 && inner < head_dim) || (n_out > 1 && outer < (n_in > 1 ? (n_in - 1) * inner : 0) + head_dim)) {
+        return ACB_ERR_INVALID_ARG;
+    }
+    if (!is_io_type(type) || head_dim > 1024 || n_tok > (int64_t) INT32_MAX * 8 / n_heads) {
+        return ACB_ERR_UNSUPPORTED;
+    }
+    if (n_tok == 0) {
+        return ACB_OK;
+    }
+    const RopeArgs a = { src,      src_tok_stride, src_head_stride, dst,        dst_tok_stride, dst_head_stride,
+                         n_tok,    n_heads,        head_dim,        rope_dim,   pos,            rope_table,
+                         max_pos,  err_flag,       (layout & ACB_ROPE_INTERLEAVED) == 0,
+                         (layout & ACB_ROPE_INVERSE) != 0,          in_place };
+    const unsigned grid = (unsigned) ((n_tok * n_heads + 7) / 8);
+    cudaStream_t   st   = (cudaStream_t) stream;
+    switch (type) {
+        case ACB_TYPE_F32:
+            rope_kernel<ACB_TYPE_F32><<<grid, 256, 0, st>>>(a);
+            break;
+        case ACB_TYPE_F16:
+            rope_kernel<ACB_TYPE_F16><<<grid, 256, 0, st>>>(a);
+            break;
+        default:
+            rope_kernel<ACB_TYPE_BF16><<<grid, 256, 0, st>>>(a);
+    }
+    return launch_status();
+}
+
+// Angles a_i = f_i p with f_i = base^(-2i/rope_dim) changed by the kind of scaling, all in double: a float angle of
+// position 10^5 is off by up to 2^-7, a double one by 2^-36.
+extern "C" acb_status acb_rope_table_scaled_host(float * table, int max_pos, int rope_dim, float base, int kind,
+                                                 float factor, int orig_max_pos, float beta_fast, float beta_slow) {
+    if (!table || max_pos <= 0 || rope_dim < 2 || rope_dim % 2 != 0 || !(base > 1.0f) || !isfinite(base) ||
+        kind < ACB_ROPE_SCALE_NONE || kind > ACB_ROPE_SCALE_YARN || !(factor >= 1.0f) || !isfinite(factor)) {
+        return ACB_ERR_INVALID_ARG;
+    }
+    if (kind == ACB_ROPE_SCALE_YARN &&
+        (orig_max_pos <= 0 || !(beta_slow > 0.0f) || !(beta_fast > beta_slow) || !isfinite(beta_fast))) {
+        return ACB_ERR_INVALID_ARG;
+    }
+    if (kind == ACB_ROPE_SCALE_NTK && rope_dim < 4) {
+        return ACB_ERR_UNSUPPORTED;  // the exponent rope_dim / (rope_dim - 2) needs a second pair
+    }
+    const double pi2 = 6.283185307179586476925286766559;
+    const int    n   = rope_dim / 2;
+    double       b = base, mscale = 1.0;
+    if (kind == ACB_ROPE_SCALE_NTK) {
+        b *= pow((double) factor, (double) rope_dim / (rope_dim - 2));
+    }
+    double lo = 0.0, hi = 0.0;  // pair indices between which YaRN goes from unchanged to divided
+    if (kind == ACB_ROPE_SCALE_YARN) {
+        // the pair that turns r times over orig_max_pos: base^(-2i/rope_dim) orig_max_pos = 2 pi r
+        auto pair_of = [&](double r) { return rope_dim * log(orig_max_pos / (r * pi2)) / (2.0 * log((double) base)); };
+        lo           = fmax(0.0, floor(pair_of(beta_fast)));
+        hi           = fmin((double) (rope_dim - 1), ceil(pair_of(beta_slow)));
+        mscale       = 0.1 * log((double) factor) + 1.0;
+    }
+    for (int i = 0; i < n; i++) {
+        double f = pow(b, -2.0 * i / rope_dim);
+        if (kind == ACB_ROPE_SCALE_LINEAR) {
+            f /= factor;
+        } else if (kind == ACB_ROPE_SCALE_YARN) {
+            const double t = fmin(1.0, fmax(0.0, (i - lo) / fmax(hi - lo, 1e-3)));
+            f              = f * (1.0 - t) + f / factor * t;
+        }
+        for (int p = 0; p < max_pos; p++) {
+            table[(int64_t) p * rope_dim + 2 * i]     = (float) (mscale * cos(f * p));
+            table[(int64_t) p * rope_dim + 2 * i + 1] = (float) (mscale * sin(f * p));
+        }
+    }
+    return ACB_OK;
+}

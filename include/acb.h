@@ -69,6 +69,8 @@ enum {
     ACB_DEVERR_POS_RANGE = 2, /* rope / kv position outside [0, max_pos) */
     ACB_DEVERR_TIMEOUT   = 4, /* a bounded device-side wait gave up */
     ACB_DEVERR_CODE_RANGE = 8, /* a negative FSQ code (acb_fsq_project_out) */
+    ACB_DEVERR_PAGE_RANGE = 16, /* a page id outside [0, n_pages) (acb_kv_q4_*, acb_attn_kv_q4) */
+    ACB_DEVERR_LEN_RANGE = 32, /* a query or key length beyond the call's bounds (acb_attn_kv_q4) */
 };
 
 /* ---- library ------------------------------------------------------------------------------ */
@@ -680,6 +682,132 @@ ACB_API size_t acb_lm_decode_scratch_bytes(const acb_decode_step * step);
  * or a device that cannot hold one CTA per SM; the caller keeps its per-op path for those.
  * After a step that raised a device error the scratch must be zeroed again. */
 ACB_API acb_status acb_lm_decode_step(const acb_decode_step * step, acb_stream_t stream);
+
+/* ---- rotary positions in every layout --------------------------------------------------------- */
+
+enum {
+    ACB_ROPE_HALF        = 0, /* pair i is elements (i, i + rope_dim/2) of the head (NeoX) */
+    ACB_ROPE_INTERLEAVED = 1, /* pair i is elements (2i, 2i + 1) */
+    ACB_ROPE_INVERSE     = 2, /* OR-ed in: rotate by -theta (takes a rotation back; the rotation's gradient) */
+};
+enum {
+    ACB_ROPE_SCALE_NONE   = 0, /* angle p * base^(-2i/rope_dim) */
+    ACB_ROPE_SCALE_LINEAR = 1, /* positions divided by factor */
+    ACB_ROPE_SCALE_NTK    = 2, /* base * factor^(rope_dim / (rope_dim - 2)): the slowest pair turns factor times slower */
+    ACB_ROPE_SCALE_YARN   = 3, /* per pair between both: pairs that turn more than beta_fast times over orig_max_pos keep
+                                  their angle, pairs below beta_slow turns divide it by factor, linear in the pair index
+                                  in between; cos and sin times 0.1 ln(factor) + 1 */
+};
+
+/* acb_rope_table_host for a context longer than the trained one, host memory: table[p][2i] = m cos(a_i p),
+ * table[p][2i+1] = m sin(a_i p), i < rope_dim/2, angles and their reduction in double, one rounding to float. kind one of
+ * ACB_ROPE_SCALE_*; factor >= 1; orig_max_pos, beta_fast > beta_slow > 0 (32 and 1 are usual) are read for YARN only. */
+ACB_API acb_status acb_rope_table_scaled_host(float * table, int max_pos, int rope_dim, float base, int kind,
+                                              float factor, int orig_max_pos, float beta_fast, float beta_slow);
+
+/* Rotates the first rope_dim elements of every head by its token's position and copies the rest: with a pair (a, b) of
+ * the layout and (c, s) = rope_table[pos[t]][2i..2i+1], a' = a c - b s, b' = a s + b c in f32, each product and sum
+ * rounded, then rounded to the type of src and dst (F32, F16 or BF16, the same for both). Element (t, h, d) is
+ * src[t*src_tok_stride + h*src_head_stride + d], dst likewise; dst is src itself (the same pointer and strides) or apart
+ * from it. head_dim even, at most 1024; rope_dim even, in [2, head_dim]. rope_table [max_pos][rope_dim] on the device. A
+ * position outside [0, max_pos) flags ACB_DEVERR_POS_RANGE and its rows are written as zeros. acb_qk_norm_rope is the
+ * whole-head NeoX form with the norm in front. */
+ACB_API acb_status acb_rope(const void * src, int64_t src_tok_stride, int64_t src_head_stride, void * dst,
+                            int64_t dst_tok_stride, int64_t dst_head_stride, int type, int64_t n_tok, int n_heads,
+                            int head_dim, int rope_dim, int layout, const int32_t * pos, const float * rope_table,
+                            int max_pos, int * err_flag, acb_stream_t stream);
+
+/* ---- paged KV cache in 4 bits ------------------------------------------------------------------ */
+
+/* A cache of many sequences in pages of page_size tokens. A head's row of one token is head_dim/32 blocks; a block is 16
+ * bytes of codes, element j in the low half of byte j and element j + 16 in the high half (the order of a GGUF Q4_0 block),
+ * and one f16 scale d; element = (code - 8) * d. d has at most 8 significant bits and |d| <= 2720, so every element is
+ * itself an f16 number: what the tensor cores multiply is what the cache holds. Bytes per element: 0.5625, against 2 of
+ * the f16 cache of acb_qkv_post. The arrays are on the device, 16-byte aligned. */
+typedef struct acb_kv_q4 {
+    uint8_t *       k_codes;    /* [n_pages][n_kv_heads][page_size][head_dim/2] */
+    uint16_t *      k_scales;   /* f16 [n_pages][n_kv_heads][page_size][head_dim/32] */
+    uint8_t *       v_codes;
+    uint16_t *      v_scales;
+    const int32_t * page_table; /* [n_seq][table_stride]: page_table[s][p / page_size] holds position p of sequence s */
+    int64_t         table_stride;
+    int32_t         n_pages, page_size; /* page_size a power of two, 16..4096 */
+    int32_t         n_kv_heads, head_dim; /* head_dim 64, 128 or 256 */
+    int32_t         n_seq, max_pages;   /* rows of the table, and its columns in use */
+} acb_kv_q4;
+
+/* Token t's row of qkv (type F32, F16 or BF16, stride elements apart) is [q(n_heads) | k(n_kv_heads) | v(n_kv_heads)]
+ * heads of head_dim. q and k heads: RMSNorm times q_norm / k_norm (NULL: none), then the rotation of acb_rope by pos[t]
+ * (rope_table NULL: none; layout without ACB_ROPE_INVERSE); q goes to q_out (q_type F32, F16 or BF16; n_heads 0: no q), k
+ * and v into the cache at position pos[t] of sequence seq[t], each block of 32 quantised from its f32 values x as
+ *   mx = the x of largest magnitude (positive where both signs have it),
+ *   d  = f16(bf16(-mx / 8)) limited to +-2720,  code = min(15, max(0, floor(x / d + 8.5)))  (d 0: code 8).
+ * A block with a NaN gets a NaN scale. A negative seq[t] is padding: nothing of token t is written. A position outside
+ * [0, max_pages*page_size), or outside the rope table, a sequence >= n_seq or a page outside the pool raise
+ * ACB_DEVERR_POS_RANGE, ID_RANGE or PAGE_RANGE; that token's q row is then zeros and the cache untouched. Two tokens of a
+ * call must not name the same place. The arithmetic before the quantisation is acb_qkv_post's, whose paged, 4-bit form this is. */
+ACB_API acb_status acb_kv_q4_append(const acb_kv_q4 * kv, const void * qkv, int type, int64_t stride, int64_t n_tok,
+                                    int n_heads, const float * q_norm, const float * k_norm, float eps,
+                                    const float * rope_table, int max_pos, int rope_dim, int layout,
+                                    const int32_t * seq, const int32_t * pos, void * q_out, int q_type,
+                                    int64_t q_stride, int * err_flag, acb_stream_t stream);
+
+/* Rows of the cache as the values they stand for: k_out / v_out [n_tok][out_stride] (either may be NULL), n_kv_heads heads
+ * of head_dim each, out_type F32, F16 (both exact) or BF16. Padding and range errors as acb_kv_q4_append (padded rows are
+ * left alone, rows in error are zeros). */
+ACB_API acb_status acb_kv_q4_read(const acb_kv_q4 * kv, const int32_t * seq, const int32_t * pos, int64_t n_tok,
+                                  void * k_out, void * v_out, int out_type, int64_t out_stride, int * err_flag,
+                                  acb_stream_t stream);
+
+/* Causal attention over the cache for one or more new tokens of every sequence (already appended):
+ *   o[t,h] = sum_j softmax_j(scale * q[t,h] . k_j) v_j over positions j <= p of the sequence (j > p - window when
+ *            window > 0), head h reading kv head h / (n_heads / n_kv_heads).
+ * Sequence s has the rows q_start[s] .. q_start[s+1] - 1 of q and o (q_start NULL: row s alone, n_tok = n_seq), the last of
+ * them at position kv_len[s] - 1. q_start [n_seq + 1] ascending and kv_len [n_seq] are read on the device when the kernels
+ * run, so a captured graph follows them; max_q_len and max_kv_len bound them on the host and size the launch. Rows that see
+ * no key (kv_len 0, or fewer keys than rows) are zeros; rows outside every sequence are left alone. A sequence with
+ * more rows than max_q_len, rows outside [0, n_tok) or kv_len outside [0, min(max_kv_len, max_pages*page_size)] raises
+ * ACB_DEVERR_LEN_RANGE and its rows (the first max_q_len of them inside [0, n_tok)) are zeros; keys on a page outside the pool
+ * raise ACB_DEVERR_PAGE_RANGE and take no part. q and o F32, F16 or BF16, the same type, *_stride elements between tokens,
+ * heads contiguous. Scores, softmax and sums in f32. The keys of a long sequence are split over blocks and joined by a second
+ * kernel, through `work` (acb_attn_kv_q4_work_bytes, device, 16-byte aligned; smaller or NULL: not split). Calls that share a
+ * workspace must not overlap. The result does not depend on what the workspace held. */
+ACB_API size_t     acb_attn_kv_q4_work_bytes(const acb_kv_q4 * kv, int64_t n_tok, int n_heads, int max_q_len,
+                                             int max_kv_len);
+ACB_API acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int type, int64_t q_stride, int64_t n_tok,
+                                  int n_heads, const int32_t * q_start, const int32_t * kv_len, int max_q_len,
+                                  int max_kv_len, int window, float scale, void * o, int64_t o_stride, void * work,
+                                  size_t work_bytes, int * err_flag, acb_stream_t stream);
+
+/* ---- rules on logits --------------------------------------------------------------------------- */
+
+/* What acb_logits_rules applies to each row; every part may be left out (NULL). All arrays are on the device. */
+typedef struct acb_logit_rules {
+    const int32_t *  hist;        /* [rows][hist_stride] tokens of the prompt, then of the answer */
+    int64_t          hist_stride;
+    const int32_t *  hist_len;    /* [rows] tokens of each history (NULL: hist_stride); limited to [0, hist_stride] */
+    const int32_t *  prompt_len;  /* [rows] how many of them are the prompt's (NULL: none) */
+    const float *    rep;         /* [rows] repetition: x > 0 ? x / rep : x * rep, tokens anywhere in the history */
+    const float *    freq;        /* [rows] x -= freq * (times in the answer) */
+    const float *    pres;        /* [rows] x -= pres, tokens in the answer */
+    const int32_t *  bias_ids;    /* [rows][n_bias] tokens (negative: unused entry) */
+    const float *    bias_val;    /* [rows][n_bias] x += the value; of entries with one token the last holds */
+    int64_t          bias_stride; /* elements between rows of both; 0: one list for every row */
+    int32_t          n_bias;
+    int32_t          n_masks;
+    const uint32_t * mask;        /* [n_masks][mask_stride] grammar masks: bit v % 32 of word v / 32 set: token v is open */
+    int64_t          mask_stride; /* words, at least (V + 31) / 32 */
+    const int32_t *  mask_row;    /* [rows] mask of each row, negative: none (NULL: row r has mask r) */
+} acb_logit_rules;
+
+/* out[r][v] = the logits after, in this order and in f32: repetition, frequency, presence, bias, mask (a closed token
+ * is -inf, whatever it was; a mask may close every token). type / out_type F32, F16 or BF16, rows ld / ld_out apart; out is
+ * logits itself (same type and stride) or apart from it. Negative history tokens are padding; a token >= V or a mask row
+ * >= n_masks raises ACB_DEVERR_ID_RANGE and is passed over. In front of acb_sample_top_k_p / acb_argmax. The same result
+ * in every run (counts are whole numbers). */
+ACB_API acb_status acb_logits_rules(const void * logits, int type, int64_t ld, void * out, int out_type, int64_t ld_out,
+                                    int rows, int64_t V, const acb_logit_rules * rules, int * err_flag,
+                                    acb_stream_t stream);
 
 /* ---- bounded device-side wait ---------------------------------------------------------------
  * Holds `stream` on the device until the 32-bit word at `flag` is >= `value` (unsigned compare,

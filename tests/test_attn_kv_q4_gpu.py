@@ -1,0 +1,314 @@
+"""GPU: attention over the paged 4-bit KV cache (acb_attn_kv_q4) against the 64-bit softmax over the values it holds.
+
+Bar, per element, with A = sum_j p_j |v_j| and S = max_j |scale| * sum_d |q_d k_jd|: a score is a sum of D products in f32, so it
+is off by at most (D + 4) 2^-24 S (D roundings, the scale, the exponent's argument twice, its power), a weight by e^that, the
+output by twice that times A (weight and sum); the sums of P and PV over n keys in f32 add (n + D) 2^-24 A in the worst case,
+taken as 2^-15 A (n <= 400 here; longer ones are checked at sqrt(n)). For 16-bit types P may be an f16 number (half a step
+2^-11 of each weight: 2^-11 A) and q may be scaled into f16 (2^-11 of an f16 step below the row's largest: 2^-22 S). Then half
+a step of the output."""
+import numpy as np
+import pytest
+
+import acb
+import serving_ref as S
+
+pytestmark = pytest.mark.gpu
+
+
+def _cache(rng, n_seq, max_len, page, Nkv, D, spare=2, big=1.0):
+    import torch
+    mp = -(-max_len // page)
+    n_pages = n_seq * mp + spare
+    table = torch.from_numpy(rng.permutation(n_pages)[:n_seq * mp].reshape(n_seq, mp).astype(np.int32)).cuda()
+    t = []
+    for _ in "kv":
+        t.append(torch.from_numpy(rng.integers(0, 256, (n_pages, Nkv, page, D // 2), dtype=np.uint8)).cuda())
+        d = S.bf16((big * rng.uniform(0.02, 0.2, (n_pages, Nkv, page, D // 32)) * rng.choice([-1, 1], (n_pages, Nkv, page, D // 32)))
+                   .astype(np.float32)).astype(np.float16)
+        t.append(torch.from_numpy(d).cuda())
+    return acb.KVCacheQ4(*t, table)
+
+
+def _held(cache, s, n):
+    kc, ks, vc, vs, table = (t.cpu().numpy() for t in cache.tensors)
+    P = kc.shape[2]
+    pg = table[s, np.arange(n) // P]
+    at = np.arange(n) % P
+    return S.values(kc[pg, :, at], ks[pg, :, at]), S.values(vc[pg, :, at], vs[pg, :, at])
+
+
+def _check(cache, q, o, q_lens, kv_lens, window, scale, kind, starts=None):
+    q, o = q.float().cpu().numpy().astype(np.float64), o.float().cpu().numpy().astype(np.float64)
+    T, H, D = q.shape
+    G = H // cache.n_kv_heads
+    at = 0
+    for s, (n, m) in enumerate(zip(q_lens, kv_lens)):
+        r0 = starts[s] if starts else at
+        at += n
+        if n == 0:
+            continue
+        k, v = _held(cache, s, m)
+        for h in range(H):
+            ref, A, s1 = S.attention(q[r0:r0 + n, h], k[:, h // G], v[:, h // G], m - n, window, scale)
+            ds = (D + 4) * 2.0 ** -24 * s1 + (2.0 ** -21 * s1 if kind != "f32" else 0)
+            tol = A * (2 * ds + 2.0 ** -15 + (2.0 ** -11 if kind != "f32" else 0))
+            tol = tol + S.HALF_STEP[kind] * (np.abs(ref) + tol) + (2.0 ** -25 if kind == "f16" else 0)
+            d = np.abs(o[r0:r0 + n, h] - ref)
+            assert (d <= tol).all(), (s, h, float(d.max()), float((d / (tol + 1e-30)).max()))
+
+
+def _run(rng, q_lens, kv_lens, page, Nkv, G, D, kind, window=0, scale=None, max_len=None, **kw):
+    import torch
+    n_seq, T, H = len(q_lens), sum(q_lens), Nkv * G
+    cache = _cache(rng, n_seq, max_len or max(max(kv_lens), 1), page, Nkv, D)
+    q = torch.from_numpy(rng.standard_normal((T, H, D)).astype(np.float32)).to(S.torch_type(kind)).cuda()
+    start = torch.tensor(np.concatenate([[0], np.cumsum(q_lens)]), dtype=torch.int32).cuda()
+    ln = torch.tensor(kv_lens, dtype=torch.int32).cuda()
+    err = torch.zeros(1, dtype=torch.int32).cuda()
+    o = cache.attention(q, ln, start, max(max(q_lens), 1), window=window, scale=scale, err=err, **kw)
+    assert int(err) == 0
+    _check(cache, q, o, q_lens, kv_lens, window, D ** -0.5 if scale is None else scale, kind)
+    return cache, q, ln, start, o
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,Nkv,G,page", [(128, 2, 2, 64), (64, 1, 7, 16), (256, 2, 4, 32), (128, 1, 1, 16), (128, 1, 9, 128),
+                                          (64, 3, 16, 16), (256, 1, 17, 16)])
+def test_single_tokens(cuda, kind, D, Nkv, G, page):
+    """One new token each, lengths around every boundary of a page and a tile, zero and one among them."""
+    rng = np.random.default_rng(D + G)
+    kv = [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 100, 129, 255, 256, 257, 400]
+    _run(rng, [1] * len(kv), kv, page, Nkv, G, D, kind)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("window", [1, 5, 16, 100, 10000])
+def test_windows(cuda, kind, window):
+    rng = np.random.default_rng(window)
+    _run(rng, [1, 4, 1, 40, 150], [77, 77, 300, 301, 150], 16, 2, 4, 64, kind, window=window)
+    _run(rng, [1, 3, 1, 140], [77, 77, 300, 301], 32, 1, 2, 128, kind, window=window)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,Nkv,G,page", [(128, 2, 2, 64), (64, 2, 7, 16), (256, 1, 3, 32), (128, 1, 8, 16), (128, 1, 5, 256)])
+def test_chunks_and_drafts(cuda, kind, D, Nkv, G, page):
+    """Rows of many counts over pasts of many lengths, none and whole prompts among them."""
+    rng = np.random.default_rng(D * G)
+    _run(rng, [3, 1, 0, 17, 64, 130, 8], [3, 1, 50, 170, 65, 130, 333], page, Nkv, G, D, kind)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_rows_that_see_nothing(cuda, kind):
+    """No keys, fewer keys than rows: zeros; rows outside every sequence stay as they were."""
+    import torch
+    rng = np.random.default_rng(2)
+    for q_len, big in ((4, 4), (100, 100)):
+        cache = _cache(rng, 3, 200, 16, 2, 128)
+        T = 3 * q_len + 9
+        q = torch.randn(T, 4, 128).to(S.torch_type(kind)).cuda()
+        o = torch.full_like(q, 7.0)
+        start = torch.tensor([5, 5 + q_len, 5 + 2 * q_len, 5 + 3 * q_len], dtype=torch.int32).cuda()
+        kv = [0, 2, q_len + 9]
+        err = torch.zeros(1, dtype=torch.int32).cuda()
+        cache.attention(q, torch.tensor(kv, dtype=torch.int32).cuda(), start, big, out=o, err=err)
+        assert int(err) == 0
+        assert bool((o[:5] == 7).all()) and bool((o[5 + 3 * q_len:] == 7).all())
+        assert bool((o[5:5 + q_len] == 0).all()) and bool((o[5 + q_len:5 + 2 * q_len - 2] == 0).all())
+        _check(cache, q, o, [q_len] * 3, kv, 0, 128 ** -0.5, kind, [5, 5 + q_len, 5 + 2 * q_len])
+
+
+@pytest.mark.parametrize("kind,D,G", [("f32", 128, 2), ("bf16", 128, 4), ("f16", 64, 7), ("bf16", 256, 2)])
+def test_long_sequences_with_and_without_splits(cuda, kind, D, G):
+    """The split over the keys gives what the unsplit pass gives; the answer is the same twice."""
+    import torch
+    rng = np.random.default_rng(11)
+    cache, q, ln, start, o = _run(rng, [1, 1, 2], [9000, 37, 5001], 64, 1, G, D, kind)
+    again = cache.attention(q, ln, start, 2)
+    assert torch.equal(o, again)
+    one = torch.empty(1, dtype=torch.uint8).cuda()
+    plain = cache.attention(q, ln, start, 2, work=one)
+    _check(cache, q, plain, [1, 1, 2], [9000, 37, 5001], 0, D ** -0.5, kind)
+
+
+def test_workspace_contents_do_not_matter(cuda):
+    import torch
+    rng = np.random.default_rng(12)
+    cache = _cache(rng, 2, 6000, 64, 2, 128)
+    q = torch.randn(2, 4, 128).cuda()
+    ln = torch.tensor([6000, 100], dtype=torch.int32).cuda()
+    w = cache.attn_workspace(2, 4, 1, 6000)
+    ref = cache.attention(q, ln)
+    for fill in (0, 255):
+        if w is not None:
+            w.fill_(fill)
+        assert torch.equal(cache.attention(q, ln, work=w, max_kv_len=6000), cache.attention(q, ln, max_kv_len=6000))
+    _check(cache, q, ref, [1, 1], [6000, 100], 0, 128 ** -0.5, "f32")
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1, 130])
+def test_garbage_behind_the_keys(cuda, kind, n):
+    """NaN and infinite scales behind the last key, before the window and on other pages do not show."""
+    import torch
+    rng = np.random.default_rng(13)
+    L = 200
+    cache = _cache(rng, 1, 256, 32, 1, 128)
+    q = torch.randn(n, 2, 128).to(S.torch_type(kind)).cuda()
+    start, ln = torch.tensor([0, n], dtype=torch.int32).cuda(), torch.tensor([L], dtype=torch.int32).cuda()
+    ref = cache.attention(q, ln, start, n, window=40)
+    kc, ks, vc, vs, table = cache.tensors
+    t = table.cpu().numpy()[0]
+    mine = set(t[:-(-L // 32)].tolist())
+    for sc in (ks, vs):
+        for pg in range(sc.shape[0]):
+            if pg not in mine:
+                sc[pg] = float("nan")
+        sc[t[L // 32], :, L % 32:] = float("inf")
+        first = max(0, L - n - 40 + 1)
+        for j in range(first):
+            sc[t[j // 32], :, j % 32] = float("nan")
+    got = cache.attention(q, ln, start, n, window=40)
+    assert torch.equal(got, ref) and bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("n", [1, 130])
+def test_nan_of_a_seen_key_shows(cuda, n):
+    import torch
+    rng = np.random.default_rng(14)
+    cache = _cache(rng, 1, 256, 32, 1, 128)
+    cache.tensors[1][int(cache.tensors[4][0, 1]), :, 3, 0] = float("nan")
+    q = torch.randn(n, 1, 128).bfloat16().cuda()
+    o = cache.attention(q, torch.tensor([200], dtype=torch.int32).cuda(), torch.tensor([0, n], dtype=torch.int32).cuda(), n)
+    assert bool(o.isnan().all())
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 140])
+def test_peaked_and_flat_scores(cuda, kind, n):
+    """Scores of hundreds (one key holds nearly all), of zero, and increasing or decreasing along the keys."""
+    import torch
+    rng = np.random.default_rng(15)
+    D = 128
+    for scale in (0.0, 3.0, -2.0):
+        _run(rng, [n], [300], 16, 1, 2, D, kind, scale=scale)
+    for step in (1, -1):
+        cache = _cache(rng, 1, 512, 16, 1, D)
+        kc, ks = cache.tensors[0], cache.tensors[1]
+        kc.fill_(0xFF)  # code 15: +7
+        j = torch.arange(512).cuda()
+        d = ((j if step > 0 else 511 - j).float() / 512).bfloat16().half()
+        t = cache.tensors[4].long()[0]
+        ks[t[j // 16], 0, j % 16] = d[:, None].expand(512, D // 32).contiguous()
+        q = torch.full((n, 1, D), 0.5).to(S.torch_type(kind)).cuda()
+        ln = torch.tensor([500], dtype=torch.int32).cuda()
+        o = cache.attention(q, ln, torch.tensor([0, n], dtype=torch.int32).cuda(), n, scale=0.3)
+        _check(cache, q, o, [n], [500], 0, 0.3, kind)
+
+
+@pytest.mark.parametrize("kind,size", [("f16", 60000.0), ("f16", 1e-6), ("bf16", 1e30), ("bf16", 1e-30), ("f32", 1e30), ("f32", 1e-30)])
+@pytest.mark.parametrize("n", [1, 130])
+def test_queries_of_any_size(cuda, kind, size, n):
+    """Queries near the ends of their type, the scale taking them back to scores of a few units."""
+    import torch
+    rng = np.random.default_rng(16)
+    cache = _cache(rng, 1, 256, 16, 1, 64)
+    q = torch.from_numpy((rng.uniform(-1, 1, (n, 2, 64)) * size).astype(np.float32)).to(S.torch_type(kind)).cuda()
+    o = cache.attention(q, torch.tensor([250], dtype=torch.int32).cuda(), torch.tensor([0, n], dtype=torch.int32).cuda(), n,
+                        scale=0.125 / size)
+    scale = float(np.float32(0.125 / size))
+    if (kind, size) == ("f16", 1e-6):  # subnormal queries hold few bits: the reference uses the ones given
+        assert bool((q != 0).any())
+    _check(cache, q, o, [n], [250], 0, scale, kind)
+
+
+def test_bounds_errors(cuda):
+    import torch
+    rng = np.random.default_rng(17)
+    for n in (1, 130):
+        cache = _cache(rng, 3, 256, 16, 1, 64)
+        ref_q = torch.randn(3 * n, 2, 64).bfloat16().cuda()
+        start = torch.arange(4, dtype=torch.int32).cuda() * n
+        good = cache.attention(ref_q, torch.tensor([200, 201, 202], dtype=torch.int32).cuda(), start, n)
+        for bad in (-1, 257, 2 ** 31 - 1):
+            err = torch.zeros(1, dtype=torch.int32).cuda()
+            o = cache.attention(ref_q, torch.tensor([200, bad, 202], dtype=torch.int32).cuda(), start, n, err=err)
+            assert int(err) == 32 and bool((o[n:2 * n] == 0).all())
+            assert torch.equal(o[:n], good[:n]) and torch.equal(o[2 * n:], good[2 * n:])
+        err = torch.zeros(1, dtype=torch.int32).cuda()
+        o = torch.full_like(ref_q, 7.0)
+        far = torch.tensor([0, n, 2 * n, 2 * n + 5 * n], dtype=torch.int32).cuda()
+        cache.attention(ref_q, torch.tensor([200, 201, 202], dtype=torch.int32).cuda(), far, n, out=o, err=err)
+        assert int(err) == 32 and torch.equal(o[:2 * n], good[:2 * n]) and bool((o[2 * n:] == 0).all())
+        back = torch.tensor([0, n, n - 1, 2 * n - 1], dtype=torch.int32).cuda()
+        o = torch.full_like(ref_q, 7.0)
+        err.zero_()
+        cache.attention(ref_q, torch.tensor([200, 201, 202], dtype=torch.int32).cuda(), back, n, out=o, err=err)
+        assert int(err) == 32 and torch.equal(o[:n - 1], good[:n - 1]) and bool((o[2 * n:] == 7).all())
+        # a page outside the pool: its keys take no part
+        cache.tensors[4][1, 2] = 10 ** 6
+        cache.tensors[4][2, 0] = -1
+        err.zero_()
+        o = cache.attention(ref_q, torch.tensor([200, 201, 202], dtype=torch.int32).cuda(), start, n, err=err)
+        assert int(err) == 16 and torch.equal(o[:n], good[:n]) and bool(o.isfinite().all())
+        assert not torch.equal(o[n:2 * n], good[n:2 * n])
+
+
+def test_strided_rows(cuda):
+    import torch
+    rng = np.random.default_rng(18)
+    for n in (1, 130):
+        cache = _cache(rng, 2, 256, 16, 2, 64)
+        wide = torch.randn(2 * n, 700).half().cuda()
+        out = torch.full((2 * n, 300), 7.0).half().cuda()
+        start, ln = torch.arange(3, dtype=torch.int32).cuda() * n, torch.tensor([150, 256], dtype=torch.int32).cuda()
+        for off in (0, 1, 4, 9):
+            q = wide[:, off:off + 256].unflatten(1, (4, 64))
+            ref = cache.attention(q.contiguous(), ln, start, n)
+            cache.attention(q, ln, start, n, out=out[:, off:off + 256].unflatten(1, (4, 64)))
+            assert torch.equal(out[:, off:off + 256].unflatten(1, (4, 64)), ref)
+            assert bool((out[:, :off] == 7).all()) and bool((out[:, off + 256:] == 7).all())
+            out.fill_(7.0)
+
+
+def test_captured_graph_follows_the_lengths(cuda):
+    """Two graphs that share a workspace, replayed in turn while lengths and queries change."""
+    import torch
+    rng = np.random.default_rng(19)
+    cache = _cache(rng, 4, 4000, 64, 2, 128)
+    ln = torch.tensor([4000, 3, 700, 0], dtype=torch.int32).cuda()
+    work = cache.attn_workspace(4, 4, 1, 4000)
+    qs = [torch.randn(4, 4, 128).cuda() for _ in range(2)]
+    outs, graphs = [torch.zeros_like(qs[0]) for _ in qs], []
+    cache.attention(qs[0], ln, max_kv_len=4000, work=work)
+    for q, o in zip(qs, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            cache.attention(q, ln, max_kv_len=4000, out=o, work=work)
+        graphs.append(g)
+    for lens in ([4000, 3, 700, 0], [1, 2000, 64, 65], [0, 0, 0, 4000]):
+        ln.copy_(torch.tensor(lens, dtype=torch.int32))
+        for q in qs:
+            q.normal_()
+        for g in graphs + graphs[::-1]:
+            g.replay()
+        for q, o in zip(qs, outs):
+            assert torch.equal(o, cache.attention(q, ln, max_kv_len=4000))
+            _check(cache, q, o, [1] * 4, lens, 0, 128 ** -0.5, "f32")
+
+
+def test_two_streams_at_once(cuda):
+    import torch
+    rng = np.random.default_rng(20)
+    cache = _cache(rng, 2, 5000, 64, 2, 128)
+    q = [torch.randn(2, 8, 128).bfloat16().cuda() for _ in range(4)]
+    ln = torch.tensor([5000, 4999], dtype=torch.int32).cuda()
+    ref = [cache.attention(x, ln) for x in q]
+    work = [cache.attn_workspace(2, 8, 1, 5120) for _ in q]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in q], [None] * 4
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = cache.attention(q[i], ln, work=work[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))
