@@ -1,16 +1,32 @@
 // k_attn_q4.cu -- causal attention over the paged 4-bit KV cache (acb_attn_kv_q4).
 //
-// One pass over the keys with the running maximum m and sum l of the softmax: for a new score s, m' = max(m, s),
-// l' = l e^(m - m') + e^(s - m'), o' = o e^(m - m') + e^(s - m') v; the output is o / l.
+// One pass over the keys with the running reference m and sum l of the softmax. For the rows that share a kv head (its query
+// heads times the sequence's new tokens) both products are matrix products on small tensor-core tiles:
+//   S[key][row] = K[key][:] . Q[row][:]        A = keys as they are unpacked, B = queries
+//   O[dim][row] += V^T[dim][key] P[key][row]   A = values, two keys to a register, B = P
+// Every cached element is an f16 number (kv_q4.cuh), so A is exact; Q is scaled by a power of two per row into f16's range
+// (an f32 query is the sum of two f16 numbers), P goes in as the sum of two f16 numbers: both products then carry 21 bits and
+// more, the sums are f32.
+//
+// Few rows: the bytes of the cache bound it (1.125 bytes per key and dimension against 4 flops a row), so a warp takes 16 keys
+// at a time straight from global memory into the registers that the tensor cores read -- the k index of a product may be any
+// order of the dimensions as long as both operands agree, so a thread's share of a key is 16 consecutive bytes -- with the next
+// 16 keys already in flight. Long sequences are cut into chunks of keys, one block each; a second kernel joins the parts.
 #include "kv_q4.cuh"
+#include "ptx.cuh"
 
 namespace acb {
 namespace {
 
+constexpr int   kSplitWarps = 4;
+constexpr int   kNoChunk    = 1 << 30;  // as many keys as a cache can have for one sequence
+constexpr float kLag        = 8.0f;  // m follows a row's maximum when that has grown by more than 2^kLag
+constexpr float kLift       = 6.0f;  // P is held times 2^kLift: at most 2^14, and whole f16 numbers down to 2^-20 of the maximum
+
 struct AttnQ4Args {
     const void *    q;
     int64_t         q_stride, n_tok;
-    int             Nh;
+    int             Nh, G;
     const int32_t * q_start;
     const int32_t * kv_len;
     int             max_q, max_kv, window;
@@ -19,10 +35,13 @@ struct AttnQ4Args {
     int64_t         o_stride;
     int *           err;
     KvQ4            kv;
+    int             chunk;    // keys of a block, a multiple of 64
+    int             n_split;  // chunks that the rows of one block can touch
+    float *         part_o;   // [n_tok*Nh][n_split][D]: sums of P V
+    float2 *        part_ml;  // [n_tok*Nh][n_split]: m (log2), l
 };
 
-// rows and keys of sequence s as the device arrays give them; false (and the error recorded by one thread of one block) when
-// they are outside the call's bounds
+// rows and keys of sequence s as the device arrays give them; false when they are outside the call's bounds
 __device__ __forceinline__ bool seq_bounds(const AttnQ4Args & a, int s, int64_t * row0, int * n, int * len) {
     const int64_t q0 = a.q_start ? __ldg(a.q_start + s) : s;
     const int64_t q1 = a.q_start ? __ldg(a.q_start + s + 1) : s + 1;
@@ -32,86 +51,536 @@ __device__ __forceinline__ bool seq_bounds(const AttnQ4Args & a, int s, int64_t 
     return q0 >= 0 && q1 >= q0 && q1 <= a.n_tok && q1 - q0 <= a.max_q && *len >= 0 && *len <= a.max_kv;
 }
 
-// one block per (row of a sequence, head), four warps, each taking every fourth key; a lane holds D/32 elements
-template <int T, int D> __global__ void __launch_bounds__(128) attn_q4_kernel(const AttnQ4Args a) {
-    constexpr int E = D / 32;
-    const int     lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int     i = blockIdx.x, h = blockIdx.y, s = blockIdx.z;
-    int64_t       row0;
-    int           n, len;
-    const bool    ok = seq_bounds(a, s, &row0, &n, &len);
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void mma16816(float * c, const uint32_t * a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t u32_of(__half2 h) {
+    return *reinterpret_cast<uint32_t *>(&h);
+}
+
+__device__ __forceinline__ __half2 half2_of(uint32_t u) {
+    return *reinterpret_cast<__half2 *>(&u);
+}
+
+// The four pairs of codes of a word (low and high nibbles of bytes 0 and 2, then of bytes 1 and 3) times the pair of
+// scales. 0x6400 | c is the f16 number 1024 + c and 0x6400 | 16 c is 1024 + 16 c, so that c - 8 comes from one exact f16
+// operation; times d is exact by the scales' 8 bits.
+__device__ __forceinline__ void unpack4(uint32_t w, __half2 d, uint32_t * r) {
+    const __half2  b0 = half2_of(0xE408E408u);  // -1032
+    const __half2  sx = half2_of(0x2C002C00u);  // 1/16
+    const __half2  b1 = half2_of(0xD480D480u);  // -72
+    const uint32_t u  = w >> 8;
+    r[0] = u32_of(__hmul2(__hadd2(half2_of((w & 0x000F000Fu) | 0x64006400u), b0), d));
+    r[1] = u32_of(__hmul2(__hfma2(half2_of((w & 0x00F000F0u) | 0x64006400u), sx, b1), d));
+    r[2] = u32_of(__hmul2(__hadd2(half2_of((u & 0x000F000Fu) | 0x64006400u), b0), d));
+    r[3] = u32_of(__hmul2(__hfma2(half2_of((u & 0x00F000F0u) | 0x64006400u), sx, b1), d));
+}
+
+template <int N> struct Words {
+    uint32_t w[N];
+    __device__ __forceinline__ void load(const void * p) {
+        if constexpr (N % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < N / 4; i++) {
+                const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+                w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+            }
+        } else if constexpr (N == 2) {
+            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p));
+            w[0] = u.x, w[1] = u.y;
+        } else {
+            w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+        }
+    }
+};
+
+// One thread's share of 16 keys and values. With lane = 4 g + t it holds, of keys g and g + 8, the D/8 bytes from
+// t D/8 on, and of values 2t, 2t+1, 2t+8, 2t+9 the D/16 bytes from g D/16 on: what the A operands of both products take.
+template <int D> struct Tile16 {
+    static constexpr int KW = D / 32, VW = D / 64, KS = D == 256 ? 2 : 1;
+    Words<KW>            k[2];
+    Words<VW>            v[4];
+    uint16_t             ks[2][KS], vs[4];
+
+    __device__ __forceinline__ void load(const KvQ4 & kv, int64_t row, int g, int t) {
+        const uint8_t *  kc = kv.kc + row * (D / 2) + t * (D / 8);
+        const uint16_t * ksp = kv.ks + row * (D / 32) + t * D / 128;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            k[i].load(kc + (g + 8 * i) * (D / 2));
+#pragma unroll
+            for (int b = 0; b < KS; b++) {
+                ks[i][b] = __ldg(ksp + (g + 8 * i) * (D / 32) + b);
+            }
+        }
+        const uint8_t *  vc = kv.vc + row * (D / 2) + g * (D / 16);
+        const uint16_t * vsp = kv.vs + row * (D / 32) + g * D / 256;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int j = 2 * t + (i & 1) + (i & 2) * 4;
+            v[i].load(vc + j * (D / 2));
+            vs[i] = __ldg(vsp + j * (D / 32));
+        }
+    }
+};
+
+// dimension of nibble `hi` of byte b of a row's codes
+__device__ __forceinline__ int dim_of(int b, int hi) {
+    return (b >> 4) * 32 + (b & 15) + 16 * hi;
+}
+
+// One block: up to 8 NT rows (r = new token * G + query head of the group) of one sequence and kv head, over one chunk of keys.
+template <int T, int D, int NT>
+__global__ void __launch_bounds__(32 * kSplitWarps) attn_q4_split_kernel(const AttnQ4Args a) {
+    constexpr int  KT  = D / 16;  // k steps of Q.K
+    constexpr int  MT  = D / 16;  // 16-dimension tiles of the output
+    constexpr int  QP  = T == ACB_TYPE_F32 ? 2 : 1;
+    constexpr int  R   = 8 * NT;
+    using T1           = typename io<T>::t;
+    __shared__ int   s_hi[R], s_lo[R];
+    __shared__ float s_m[kSplitWarps][R], s_l[kSplitWarps][R];
+    __shared__ float s_o[R][D];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int rt = blockIdx.x / a.n_split, split = blockIdx.x - rt * a.n_split, hk = blockIdx.y, s = blockIdx.z;
+    ptx::grid_dep_launch();
+    int64_t    row0;
+    int        n, len;
+    const bool ok = seq_bounds(a, s, &row0, &n, &len);
     if (!ok && a.err && threadIdx.x == 0) {
         atomicOr(a.err, ACB_DEVERR_LEN_RANGE);
     }
-    const int64_t t = row0 + i;
-    if (i >= n || t < 0 || t >= a.n_tok) {
+    const int r0 = rt * R;
+    if (r0 >= n * a.G) {
         return;
     }
-    const int p  = ok ? len - n + i : -1;
-    const int j0 = a.window > 0 ? max(0, p - a.window + 1) : 0;
-    const int hk = h / (a.Nh / a.kv.nkv);
-    using T1     = typename io<T>::t;
-    const T1 * q = reinterpret_cast<const T1 *>(a.q) + t * a.q_stride + (int64_t) h * D;
-    float      qv[E], o[E], m = -INFINITY, l = 0.0f;
-    const int  b = lane & 15;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        qv[e] = io<T>::to_f(q[e * 32 + lane]) * a.scale_log2;
-        o[e]  = 0.0f;
+    // the keys that some row of this block sees
+    const int i0 = r0 / a.G, i1 = min(n - 1, (r0 + R - 1) / a.G);
+    const int p0 = ok ? len - n + i0 : -1, p1 = ok ? len - n + i1 : -1;
+    const int lo0 = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
+    // rows that see no key are written by the first block
+    if (split == 0 && p0 < 0) {
+        for (int e = threadIdx.x; e < R * D; e += 32 * kSplitWarps) {
+            const int r = r0 + e / D, i = r / a.G;
+            if (i < n && (!ok || len - n + i < 0) && row0 + i >= 0 && row0 + i < a.n_tok) {
+                reinterpret_cast<T1 *>(a.o)[(row0 + i) * a.o_stride + (int64_t) (hk * a.G + r % a.G) * D + e % D] =
+                    io<T>::from_f(0.0f);
+            }
+        }
     }
-    for (int j = j0 + warp; j <= p; j += 4) {
-        const int pg = a.kv.page_of(s, j);
-        if (pg < 0) {
+    const int c  = lo0 / a.chunk + split;
+    const int j0 = max(lo0, c * a.chunk), j1 = min(p1 + 1, (c + 1) * a.chunk);
+    if (j0 >= j1) {
+        return;
+    }
+    if (threadIdx.x < R) {
+        const int i = (r0 + threadIdx.x) / a.G, p = i < n ? len - n + i : -1;
+        s_hi[threadIdx.x] = p;
+        s_lo[threadIdx.x] = a.window > 0 ? max(0, p - a.window + 1) : 0;
+    }
+    __syncthreads();
+    // keys before full0 are behind the last row's window
+    const int full0 = a.window > 0 ? max(0, p1 - a.window + 1) : 0;
+
+    // queries: row g of each 8, the dimensions that meet this thread's bytes of a key
+    uint32_t qf[QP][NT][KT][2];
+    float    sc[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int  r = r0 + nt * 8 + g, i = r / a.G;
+        const T1 * q = reinterpret_cast<const T1 *>(a.q) + (row0 + i) * a.q_stride + (int64_t) (hk * a.G + r % a.G) * D;
+        float      f[KT][4], mx = 0.0f;
+#pragma unroll
+        for (int w = 0; w < D / 32; w++) {
+            const int b = t * (D / 8) + 4 * w;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                // order of unpack4: bytes 0 and 2 low, 0 and 2 high, 1 and 3 low, 1 and 3 high
+                const int   d = dim_of(b + (e >> 2) + 2 * (e & 1), (e >> 1) & 1);
+                const float v = i < n ? io<T>::to_f(q[d]) : 0.0f;
+                f[2 * w + (e >> 2)][e & 3] = v;
+                mx                         = fmaxf(mx, fabsf(v));
+            }
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // 2^e with mx / 2^e in [1, 2): exponent field of mx, kept where 2^-e is a number
+        int e = (int) (__float_as_uint(mx) >> 23);
+        e     = mx == 0.0f || e == 255 ? 127 : min(max(e, 1), 253);
+        const float down = __uint_as_float((uint32_t) (254 - e) << 23);
+        const float up   = __uint_as_float((uint32_t) e << 23);
+#pragma unroll
+        for (int k = 0; k < KT; k++) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const float   x = f[k][2 * h] * down, y = f[k][2 * h + 1] * down;
+                const __half2 hi = __floats2half2_rn(x, y);
+                qf[0][nt][k][h]  = u32_of(hi);
+                if (QP == 2) {
+                    const float2 b          = __half22float2(hi);
+                    qf[QP - 1][nt][k][h] = u32_of(__floats2half2_rn(x - b.x, y - b.y));
+                }
+            }
+        }
+        const float fs = a.scale_log2 * up;
+        // scores come out with the row in the column index: rows 2t and 2t + 1, held by the lanes with g = 2t, 2t + 1
+        sc[nt][0] = __shfl_sync(0xffffffffu, fs, 8 * t);
+        sc[nt][1] = __shfl_sync(0xffffffffu, fs, 8 * t + 4);
+    }
+
+    float o[MT][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        m[nt][0] = m[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.0f;
+        }
+    }
+
+    const int hi_min = p0;  // the first row's last key: keys up to it are seen by all rows that exist
+    const int tb0    = (j0 & ~15) + 16 * warp;
+    Tile16<D> tile;
+    int       pg = tb0 < j1 ? a.kv.page_of(s, tb0) : -1;
+    if (tb0 < j1 && pg >= 0) {
+        tile.load(a.kv, a.kv.row(pg, hk, tb0), g, t);
+    }
+    for (int tb = tb0; tb < j1; tb += 16 * kSplitWarps) {
+        const Tile16<D> cur = tile;
+        const int       cpg = pg;
+        const int       nb  = tb + 16 * kSplitWarps;
+        if (nb < j1) {
+            pg = a.kv.page_of(s, nb);
+            if (pg >= 0) {
+                tile.load(a.kv, a.kv.row(pg, hk, nb), g, t);
+            }
+        }
+        if (cpg < 0) {
             if (lane == 0 && a.err) {
                 atomicOr(a.err, ACB_DEVERR_PAGE_RANGE);
             }
             continue;
         }
-        const int64_t row = a.kv.row(pg, hk, j);
-        float         sc = 0.0f, v[E];
+        // scores
+        float S[NT][4];
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            const uint32_t ck = a.kv.kc[row * (D / 2) + e * 16 + b], cv = a.kv.vc[row * (D / 2) + e * 16 + b];
-            const float    kx = (float) (int) (lane < 16 ? ck & 15u : ck >> 4) - 8.0f;
-            const float    vx = (float) (int) (lane < 16 ? cv & 15u : cv >> 4) - 8.0f;
-            sc += qv[e] * kx * f16_bits_to_f(a.kv.ks[row * E + e]);
-            v[e] = vx * f16_bits_to_f(a.kv.vs[row * E + e]);
+        for (int nt = 0; nt < NT; nt++) {
+            S[nt][0] = S[nt][1] = S[nt][2] = S[nt][3] = 0.0f;
         }
-        sc            = warp_sum(sc);
-        const float m1 = fmaxf(m, sc);
-        const float al = m1 == -INFINITY ? 1.0f : exp2f(m - m1), pr = m1 == -INFINITY ? 0.0f : exp2f(sc - m1);
-        m             = m1;
-        l             = l * al + pr;
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            o[e] = o[e] * al + pr * v[e];
+        for (int w = 0; w < D / 32; w++) {
+            uint32_t x[4], y[4];
+            unpack4(cur.k[0].w[w], __half2half2(__ushort_as_half(cur.ks[0][w * Tile16<D>::KS / (D / 32)])), x);
+            unpack4(cur.k[1].w[w], __half2half2(__ushort_as_half(cur.ks[1][w * Tile16<D>::KS / (D / 32)])), y);
+            const uint32_t a0[4] = { x[0], y[0], x[1], y[1] }, a1[4] = { x[2], y[2], x[3], y[3] };
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                for (int p = QP - 1; p >= 0; p--) {
+                    mma16816(S[nt], a0, qf[p][nt][2 * w][0], qf[p][nt][2 * w][1]);
+                    mma16816(S[nt], a1, qf[p][nt][2 * w + 1][0], qf[p][nt][2 * w + 1][1]);
+                }
+            }
+        }
+        // a tile that some row does not see whole: -inf for what it does not see, and the values that no row sees left out
+        const bool edge = tb < full0 || tb < j0 || tb + 15 > hi_min || tb + 15 >= j1;
+        bool       grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                S[nt][e] *= sc[nt][e & 1];
+                if (edge) {
+                    const int j = tb + g + 8 * (e >> 1), r = nt * 8 + 2 * t + (e & 1);
+                    if (j < max(j0, s_lo[r]) || j > min(j1 - 1, s_hi[r])) {
+                        S[nt][e] = -INFINITY;
+                    }
+                }
+                grow = grow || S[nt][e] > m[nt][e & 1] + kLag;
+            }
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float x = fmaxf(m[nt][h], fmaxf(S[nt][h], S[nt][h + 2]));
+                    x       = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x       = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x       = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    const float f = x == -INFINITY ? 1.0f : ex2(m[nt][h] - x);
+                    m[nt][h]      = x;
+                    l[nt][h] *= f;
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        o[mt][nt][h] *= f;
+                        o[mt][nt][h + 2] *= f;
+                    }
+                }
+            }
+        }
+        uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const float m0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0] - kLift;
+            const float m1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1] - kLift;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const float x = ex2(S[nt][2 * h] - m0), y = ex2(S[nt][2 * h + 1] - m1);
+                l[nt][0] += x;
+                l[nt][1] += y;
+                const __half2 hi = __floats2half2_rn(x, y);
+                const float2  b  = __half22float2(hi);
+                ph[nt][h]        = transpose8x8(u32_of(hi));
+                pl[nt][h]        = transpose8x8(u32_of(__floats2half2_rn(x - b.x, y - b.y)));
+            }
+        }
+        uint32_t vs01 = (uint32_t) cur.vs[0] | ((uint32_t) cur.vs[1] << 16);
+        uint32_t vs23 = (uint32_t) cur.vs[2] | ((uint32_t) cur.vs[3] << 16);
+        if (edge) {
+            // a scale that is no number must not reach the rows that do not see its key (0 * NaN): it is taken out here and
+            // put on the rows that do see it one by one
+            uint32_t any = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int j = tb + 2 * t + (i & 1) + (i & 2) * 4;
+                if ((cur.vs[i] & 0x7C00u) == 0x7C00u) {
+                    (i < 2 ? vs01 : vs23) &= (i & 1) ? 0x0000FFFFu : 0xFFFF0000u;
+                    any |= j >= j0 && j < j1;
+                }
+            }
+            if (__any_sync(0xffffffffu, any)) {
+                const int64_t row = a.kv.row(cpg, hk, tb);
+                for (int j = max(tb, j0); j < min(tb + 16, j1); j++) {
+                    const uint16_t d = __ldg(a.kv.vs + (row + j - tb) * (D / 32) + g * D / 256);
+                    if ((d & 0x7C00u) == 0x7C00u) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const int r = nt * 8 + 2 * t + h;
+                                if (j >= s_lo[r] && j <= s_hi[r]) {
+#pragma unroll
+                                    for (int mt = 0; mt < MT; mt++) {
+                                        o[mt][nt][h] = o[mt][nt][h + 2] = NAN;
+                                    }
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < D / 64; w++) {
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const uint32_t sel = half ? 0x7632u : 0x5410u;
+                uint32_t       x[4], y[4];  // bytes 2 half, 2 half + 1: low, high, low, high nibble of two keys each
+                unpack4(__byte_perm(cur.v[0].w[w], cur.v[1].w[w], sel), half2_of(vs01), x);
+                unpack4(__byte_perm(cur.v[2].w[w], cur.v[3].w[w], sel), half2_of(vs23), y);
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const int      mt   = w * 4 + half * 2 + b;
+                    const uint32_t f[4] = { x[2 * b], x[2 * b + 1], y[2 * b], y[2 * b + 1] };
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        mma16816(o[mt][nt], f, pl[nt][0], pl[nt][1]);
+                        mma16816(o[mt][nt], f, ph[nt][0], ph[nt][1]);
+                    }
+                }
+            }
         }
     }
-    __shared__ float so[4][D], sm[4], sl[4];
+
+    // the four warps' parts, joined in the warps' order
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        so[warp][e * 32 + lane] = o[e];
-    }
-    if (lane == 0) {
-        sm[warp] = m;
-        sl[warp] = l;
+    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float x = l[nt][h];
+            x += __shfl_xor_sync(0xffffffffu, x, 4);
+            x += __shfl_xor_sync(0xffffffffu, x, 8);
+            x += __shfl_xor_sync(0xffffffffu, x, 16);
+            if (g == 0) {
+                s_m[warp][nt * 8 + 2 * t + h] = m[nt][h];
+                s_l[warp][nt * 8 + 2 * t + h] = x;
+            }
+        }
     }
     __syncthreads();
-    const float M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    T1 *        y = reinterpret_cast<T1 *>(a.o) + t * a.o_stride + (int64_t) h * D;
-    for (int d = threadIdx.x; d < D; d += 128) {
-        float L = 0.0f, r = 0.0f;
-        for (int w = 0; w < 4; w++) {
-            const float f = M == -INFINITY ? 0.0f : exp2f(sm[w] - M);
-            L += f * sl[w];
-            r += f * so[w][d];
+    for (int w = 0; w < kSplitWarps; w++) {
+        if (warp == w) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int   r = nt * 8 + 2 * t + h;
+                    const float M = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+                    const float f = m[nt][h] == -INFINITY ? 0.0f : ex2(m[nt][h] - M);
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+#pragma unroll
+                        for (int q = 0; q < 2; q++) {
+                            float *     p = &s_o[r][dim_of(g * (D / 16) + mt, q)];
+                            const float v = o[mt][nt][h + 2 * q];
+                            const float x = m[nt][h] == -INFINITY && v == v ? 0.0f : v * f;
+                            *p            = w == 0 ? x : *p + x;
+                        }
+                    }
+                }
+            }
         }
-        y[d] = io<T>::from_f(L > 0.0f ? r / L : (L == L ? 0.0f : L));
+        __syncthreads();
+    }
+    for (int e = threadIdx.x; e < R * D / 4; e += 32 * kSplitWarps) {
+        const int rr = e / (D / 4), d = (e % (D / 4)) * 4;
+        const int r = r0 + rr, i = r / a.G;
+        const int p = i < n ? s_hi[rr] : -1;
+        const int c0 = s_lo[rr] / a.chunk, c1 = p / a.chunk;
+        if (p < 0 || c < c0 || c > c1) {  // no key of this row in this chunk
+            continue;
+        }
+        const float M  = fmaxf(fmaxf(s_m[0][rr], s_m[1][rr]), fmaxf(s_m[2][rr], s_m[3][rr]));
+        float       L  = 0.0f;
+        for (int w = 0; w < kSplitWarps; w++) {
+            const float x = s_l[w][rr];
+            L += s_m[w][rr] == -INFINITY && x == x ? 0.0f : x * ex2(s_m[w][rr] - M);
+        }
+        const float4  v   = *reinterpret_cast<const float4 *>(&s_o[rr][d]);
+        const int64_t tok = row0 + i;
+        const int     h   = hk * a.G + r % a.G;
+        if (c0 == c1) {  // every key of this row was in this chunk
+            const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+            T1 *        y   = reinterpret_cast<T1 *>(a.o) + tok * a.o_stride + (int64_t) h * D + d;
+            y[0]            = io<T>::from_f(v.x * inv);
+            y[1]            = io<T>::from_f(v.y * inv);
+            y[2]            = io<T>::from_f(v.z * inv);
+            y[3]            = io<T>::from_f(v.w * inv);
+        } else {
+            const int64_t slot = (tok * a.Nh + h) * a.n_split + c % a.n_split;
+            *reinterpret_cast<float4 *>(a.part_o + slot * D + d) = v;
+            if (d == 0) {
+                a.part_ml[slot] = make_float2(M, L);
+            }
+        }
     }
 }
 
-template <int T> void (*attn_kernel(int D))(const AttnQ4Args) {
-    return D == 64 ? attn_q4_kernel<T, 64> : D == 128 ? attn_q4_kernel<T, 128> : attn_q4_kernel<T, 256>;
+// joins the chunks of the rows that had more than one, in the chunks' order: a warp per row
+template <int T, int D> __global__ void __launch_bounds__(256) attn_q4_join_kernel(const AttnQ4Args a) {
+    constexpr int E    = D / 32;
+    using T1           = typename io<T>::t;
+    const int     lane = threadIdx.x & 31, hk = blockIdx.y, s = blockIdx.z;
+    const int     r    = blockIdx.x * 8 + (threadIdx.x >> 5);
+    ptx::grid_dep_wait();
+    int64_t    row0;
+    int        n, len;
+    const bool ok = seq_bounds(a, s, &row0, &n, &len);
+    const int  i = r / a.G, p = len - n + i;
+    if (!ok || i >= n || p < 0) {
+        return;
+    }
+    const int c0 = (a.window > 0 ? max(0, p - a.window + 1) : 0) / a.chunk, c1 = p / a.chunk;
+    if (c0 == c1) {
+        return;
+    }
+    const int64_t tok = row0 + i;
+    const int     h   = hk * a.G + r % a.G;
+    const int64_t at  = (tok * a.Nh + h) * a.n_split;
+    float         M   = -INFINITY, L = 0.0f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        o[e] = 0.0f;
+    }
+    for (int c = c0; c <= c1; c++) {
+        M = fmaxf(M, a.part_ml[at + c % a.n_split].x);
+    }
+    for (int c = c0; c <= c1; c++) {
+        const int64_t slot = at + c % a.n_split;
+        const float2  ml   = a.part_ml[slot];
+        const float   f    = M == -INFINITY ? 1.0f : ex2(ml.x - M);
+        L += ml.y * f;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            o[e] += a.part_o[slot * D + e * 32 + lane] * f;
+        }
+    }
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+    T1 *        y   = reinterpret_cast<T1 *>(a.o) + tok * a.o_stride + (int64_t) h * D;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        y[e * 32 + lane] = io<T>::from_f(o[e] * inv);
+    }
+}
+
+using Kernel = void (*)(const AttnQ4Args);
+
+template <int T, int NT> Kernel split_kernel(int D) {
+    return D == 64 ? attn_q4_split_kernel<T, 64, NT> : D == 128 ? attn_q4_split_kernel<T, 128, NT>
+                                                                : attn_q4_split_kernel<T, 256, NT>;
+}
+
+template <int T> Kernel split_kernel(int D, int nt) {
+    return nt == 1 ? split_kernel<T, 1>(D) : D == 64 ? attn_q4_split_kernel<T, 64, 2> : attn_q4_split_kernel<T, 128, 2>;
+}
+
+template <int T> Kernel join_kernel(int D) {
+    return D == 64 ? attn_q4_join_kernel<T, 64> : D == 128 ? attn_q4_join_kernel<T, 128> : attn_q4_join_kernel<T, 256>;
+}
+
+// How the keys are cut. Rows of one kv head in tiles of 8 or 16 (8 for heads of 256, whose sums fill the registers); chunks
+// of a multiple of 64 keys (four warps of 16), as many as it takes to give every SM a few blocks to choose from, but
+// none below 256 keys: a chunk's part costs its rows 4 (D + 2) bytes twice, against 1.125 D bytes a key.
+constexpr int kMinChunk = 256;
+
+struct Plan {
+    int     nt, tiles, chunk, n_split;
+    int64_t most;  // n_split of any window at these sizes is at most this
+};
+
+Plan make_plan(const acb_kv_q4 * kv, int n_heads, int max_q, int max_kv, int window) {
+    Plan          p;
+    const int64_t rows   = (int64_t) max_q * (n_heads / kv->n_kv_heads);
+    p.nt                 = rows <= 8 || kv->head_dim == 256 ? 1 : 2;
+    p.tiles              = (int) ((rows + 8 * p.nt - 1) / (8 * p.nt));
+    const int64_t keys   = window > 0 && (int64_t) window + max_q < max_kv ? (int64_t) window + max_q : max_kv;
+    const int64_t tasks  = (int64_t) p.tiles * kv->n_kv_heads * kv->n_seq;
+    const int64_t splits = (int64_t) num_sms() * 12 / tasks;
+    const int64_t cuts   = (max_kv + kMinChunk - 1) / kMinChunk;
+    if (splits <= 1 || cuts <= 1) {
+        p.n_split = 1;
+        p.most    = 1;
+        p.chunk   = kNoChunk;
+        return p;
+    }
+    int64_t chunk = (keys + splits - 1) / splits;
+    chunk         = ((chunk < kMinChunk ? kMinChunk : chunk) + 63) / 64 * 64;
+    p.chunk       = (int) chunk;
+    // a window's keys can begin anywhere in a chunk
+    p.n_split = (int) ((keys + chunk - 1) / chunk) + (keys < max_kv ? 1 : 0);
+    p.most    = (splits < cuts ? splits : cuts) + 1;
+    return p;
+}
+
+size_t plan_bytes(int64_t n_split, const acb_kv_q4 * kv, int64_t n_tok, int n_heads) {
+    return n_split <= 1 ? 0 : (size_t) n_tok * n_heads * n_split * (kv->head_dim + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -121,7 +590,12 @@ using namespace acb;
 
 extern "C" size_t acb_attn_kv_q4_work_bytes(const acb_kv_q4 * kv, int64_t n_tok, int n_heads, int max_q_len,
                                             int max_kv_len) {
-    return 0;
+    KvQ4 d;
+    if (kv_q4_check(kv, &d) != ACB_OK || n_tok <= 0 || n_heads <= 0 || n_heads % kv->n_kv_heads != 0 || max_q_len <= 0 ||
+        max_kv_len <= 0) {
+        return 0;
+    }
+    return plan_bytes(make_plan(kv, n_heads, max_q_len, max_kv_len, 0).most, kv, n_tok, n_heads);
 }
 
 extern "C" acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int type, int64_t q_stride, int64_t n_tok,
@@ -135,22 +609,30 @@ extern "C" acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int t
     }
     if (!q || !o || !kv_len || n_tok < 0 || n_heads <= 0 || n_heads % kv->n_kv_heads != 0 || max_q_len <= 0 ||
         max_kv_len < 0 || window < 0 || !(scale == scale) || q_stride < (int64_t) n_heads * kv->head_dim ||
-        o_stride < (int64_t) n_heads * kv->head_dim || (!q_start && (n_tok != kv->n_seq || max_q_len != 1))) {
+        o_stride < (int64_t) n_heads * kv->head_dim || (!q_start && (n_tok != kv->n_seq || max_q_len != 1)) ||
+        (work && !kv_q4_aligned(work))) {
         return ACB_ERR_INVALID_ARG;
     }
     if (max_kv_len > (int64_t) kv->max_pages * kv->page_size) {
         return ACB_ERR_OUT_OF_RANGE;
     }
-    if (!is_io_type(type) || n_heads > 65535 || kv->n_seq > 65535) {
+    if (!is_io_type(type) || kv->n_kv_heads > 65535 || kv->n_seq > 65535 ||
+        (int64_t) max_q_len * n_heads > (1 << 24)) {
         return ACB_ERR_UNSUPPORTED;
     }
     if (n_tok == 0) {
         return ACB_OK;
     }
+    Plan p = make_plan(kv, n_heads, max_q_len, max_kv_len, window);
+    if (p.n_split > 1 && (!work || work_bytes < plan_bytes(p.n_split, kv, n_tok, n_heads))) {
+        p.n_split = 1;
+        p.chunk   = kNoChunk;
+    }
     a.q          = q;
     a.q_stride   = q_stride;
     a.n_tok      = n_tok;
     a.Nh         = n_heads;
+    a.G          = n_heads / kv->n_kv_heads;
     a.q_start    = q_start;
     a.kv_len     = kv_len;
     a.max_q      = max_q_len;
@@ -160,9 +642,36 @@ extern "C" acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int t
     a.o          = o;
     a.o_stride   = o_stride;
     a.err        = err_flag;
-    const auto kern = type == ACB_TYPE_F32   ? attn_kernel<ACB_TYPE_F32>(kv->head_dim)
-                      : type == ACB_TYPE_F16 ? attn_kernel<ACB_TYPE_F16>(kv->head_dim)
-                                             : attn_kernel<ACB_TYPE_BF16>(kv->head_dim);
-    kern<<<dim3((unsigned) max_q_len, (unsigned) n_heads, (unsigned) kv->n_seq), 128, 0, (cudaStream_t) stream>>>(a);
-    return launch_status();
+    a.chunk      = p.chunk;
+    a.n_split    = p.n_split;
+    a.part_ml    = reinterpret_cast<float2 *>(work);
+    a.part_o     = reinterpret_cast<float *>(work) + 2 * n_tok * n_heads * p.n_split;
+    const int    D    = kv->head_dim;
+    const Kernel kern = type == ACB_TYPE_F32   ? split_kernel<ACB_TYPE_F32>(D, p.nt)
+                        : type == ACB_TYPE_F16 ? split_kernel<ACB_TYPE_F16>(D, p.nt)
+                                               : split_kernel<ACB_TYPE_BF16>(D, p.nt);
+    kern<<<dim3((unsigned) (p.tiles * p.n_split), (unsigned) kv->n_kv_heads, (unsigned) kv->n_seq), 32 * kSplitWarps, 0,
+           (cudaStream_t) stream>>>(a);
+    const acb_status st = launch_status();
+    if (st != ACB_OK || p.n_split == 1) {
+        return st;
+    }
+    const Kernel join = type == ACB_TYPE_F32   ? join_kernel<ACB_TYPE_F32>(D)
+                        : type == ACB_TYPE_F16 ? join_kernel<ACB_TYPE_F16>(D)
+                                               : join_kernel<ACB_TYPE_BF16>(D);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim  = dim3((unsigned) (((int64_t) max_q_len * a.G + 7) / 8), (unsigned) kv->n_kv_heads, (unsigned) kv->n_seq);
+    cfg.blockDim = dim3(256);
+    cfg.stream   = (cudaStream_t) stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs                                          = attr;
+    cfg.numAttrs                                       = 1;
+    const cudaError_t e                                = cudaLaunchKernelEx(&cfg, join, a);
+    if (e != cudaSuccess) {
+        set_last_cuda_error(e);
+        return ACB_ERR_CUDA;
+    }
+    return ACB_OK;
 }

@@ -42,7 +42,7 @@ inline acb_status kv_q4_check(const acb_kv_q4 * kv, KvQ4 * out) {
     }
     if ((kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256) || kv->page_size < 16 ||
         kv->page_size > 4096 || (kv->page_size & (kv->page_size - 1)) != 0 ||
-        (int64_t) kv->max_pages * kv->page_size > INT32_MAX) {
+        (int64_t) kv->max_pages * kv->page_size > (1 << 30)) {
         return ACB_ERR_UNSUPPORTED;
     }
     int shift = 0;

@@ -733,7 +733,8 @@ typedef struct acb_kv_q4 {
     int64_t         table_stride;
     int32_t         n_pages, page_size; /* page_size a power of two, 16..4096 */
     int32_t         n_kv_heads, head_dim; /* head_dim 64, 128 or 256 */
-    int32_t         n_seq, max_pages;   /* rows of the table, and its columns in use */
+    int32_t         n_seq, max_pages;   /* rows of the table, and its columns in use (at most 2^30
+                                           tokens a sequence) */
 } acb_kv_q4;
 
 /* Token t's row of qkv (type F32, F16 or BF16, stride elements apart) is [q(n_heads) | k(n_kv_heads) | v(n_kv_heads)]

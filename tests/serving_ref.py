@@ -59,10 +59,10 @@ def values(codes, scales):
 
 
 def attention(q, k, v, first, window, scale):
-    """q [n, D] at positions first.., k / v [len, D]: outputs [n, D] and, per element, sum_j p_j |v_j| and the largest
-    |scale| * sum |q k| (what the roundings of the sums and of the scores are relative to)"""
+    """q [n, D] at positions first.., k / v [len, D]: outputs [n, D] and, per element, sum_j p_j |v_j|, the largest
+    |scale| * sum |q k| (what the roundings of the sums and of the scores are relative to) and sum_j |v_j|"""
     n, D = q.shape
-    o, a, s1 = np.zeros((n, D)), np.zeros((n, D)), np.zeros((n, 1))
+    o, a, s1, av = np.zeros((n, D)), np.zeros((n, D)), np.zeros((n, 1)), np.zeros((n, D))
     for i in range(n):
         p = first + i
         lo = max(0, p - window + 1) if window else 0
@@ -73,7 +73,8 @@ def attention(q, k, v, first, window, scale):
         e = np.exp(s - s.max())
         w = e / e.sum()
         o[i], a[i], s1[i] = w @ vv, w @ np.abs(vv), (np.abs(kk) @ np.abs(q[i])).max() * abs(scale)
-    return o, a, s1
+        av[i] = np.abs(vv).sum(0)
+    return o, a, s1, av
 
 
 def rules(x, hist=None, n_prompt=0, rep=None, freq=None, pres=None, bias=(), mask=None):
