@@ -2,7 +2,9 @@
 // the trained one (acb_rope_table_scaled_host).
 //
 // With z = a + i b for a pair and w = c + i s its table entry, the rotation is z' = z w (w's conjugate for the
-// inverse): 6 flops on 2 elements against a read and a write of both, so the memory bounds it.
+// inverse): 6 flops on 2 elements against a read and a write of both, so the memory bounds it. The vector form takes 16
+// bytes at a time (with half pairs, 16 bytes of each half), a block one or more whole tokens, so that the angles of a token come
+// from L1 for all its heads; where alignment or an odd width forbids that, a warp takes a head pair by pair.
 #include <math.h>
 
 #include "common.cuh"
@@ -62,6 +64,116 @@ template <int T> __global__ void __launch_bounds__(256) rope_kernel(const RopeAr
     }
 }
 
+// Units of a head: half pairs, two 16-byte vectors R/2 apart; interleaved, one vector of whole pairs; then the vectors that are
+// copied. threadIdx.x runs over a token's units (head by head), threadIdx.y over the block's tokens.
+template <int T, bool HALF> __global__ void __launch_bounds__(256) rope_vec_kernel(const RopeArgs a, uint32_t rot_units,
+                                                                                   uint32_t units, uint32_t magic) {
+    using E           = typename io<T>::t;
+    constexpr int V   = vec16<T>::N;
+    const int64_t t   = (int64_t) blockIdx.x * blockDim.y + threadIdx.y;
+    if (t >= a.n_tok) {
+        return;
+    }
+    const int  p   = __ldg(a.pos + t);
+    const bool bad = p < 0 || p >= a.max_pos;
+    if (bad && threadIdx.x == 0 && a.err) {
+        atomicOr(a.err, ACB_DEVERR_POS_RANGE);
+    }
+    const float *  w = a.table + (int64_t) (bad ? 0 : p) * a.R;
+    const E *      x = reinterpret_cast<const E *>(a.src) + t * a.sts;
+    E *            y = reinterpret_cast<E *>(a.dst) + t * a.dts;
+    const uint32_t n = (uint32_t) a.n_heads * units;
+    vec16<T>       lo[2], hi[2];
+    auto           head_of = [&](uint32_t i) { return units == 1 ? i : __umulhi(i, magic); };
+    auto           off_of  = [&](uint32_t u) { return u < rot_units ? (int) u * V : (HALF ? a.R : 0) + (int) (HALF ? u - rot_units : u) * V; };
+    for (uint32_t i = threadIdx.x; i < n; i += 2 * blockDim.x) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {  // both units' loads before either's store
+            const uint32_t j = i + k * blockDim.x;
+            if (j < n) {
+                const uint32_t h = head_of(j), u = j - h * units;
+                const E *      q = x + (int64_t) h * a.shs + off_of(u);
+                lo[k].load(q);
+                if (HALF && u < rot_units) {
+                    hi[k].load(q + a.R / 2);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const uint32_t j = i + k * blockDim.x;
+            if (j >= n) {
+                break;
+            }
+            const uint32_t h = head_of(j), u = j - h * units;
+            E *            q = y + (int64_t) h * a.dhs + off_of(u);
+            if (bad) {
+                lo[k].u = make_uint4(0, 0, 0, 0);
+                hi[k].u = lo[k].u;
+            } else if (u < rot_units) {
+                const float4 * cs = reinterpret_cast<const float4 *>(w + (HALF ? 2 : 1) * V * u);
+#pragma unroll
+                for (int e = 0; e < (HALF ? V : V / 2); e += 2) {
+                    const float4 c4 = __ldg(cs + e / 2);
+#pragma unroll
+                    for (int f = 0; f < 2; f++) {
+                        const float c = f ? c4.z : c4.x, s0 = f ? c4.w : c4.y, sn = a.inverse ? -s0 : s0;
+                        const int   ia = HALF ? e + f : 2 * (e + f);
+                        const float g = lo[k].get(ia), z = HALF ? hi[k].get(ia) : lo[k].get(ia + 1);
+                        const float r0 = __fsub_rn(__fmul_rn(g, c), __fmul_rn(z, sn));
+                        const float r1 = __fadd_rn(__fmul_rn(g, sn), __fmul_rn(z, c));
+                        lo[k].set(ia, r0);
+                        if (HALF) {
+                            hi[k].set(ia, r1);
+                        } else {
+                            lo[k].set(ia + 1, r1);
+                        }
+                    }
+                }
+            } else if (a.in_place) {
+                continue;
+            }
+            lo[k].store(q);
+            if (HALF && u < rot_units) {
+                hi[k].store(q + a.R / 2);
+            }
+        }
+    }
+}
+
+// whether every row of the call is made of whole aligned vectors
+bool rope_vector(const RopeArgs & a, int type) {
+    const int64_t v = 16 / type_size(type);
+    const int64_t r = a.half ? a.R / 2 : a.R;
+    return (reinterpret_cast<uintptr_t>(a.src) | reinterpret_cast<uintptr_t>(a.dst) | reinterpret_cast<uintptr_t>(a.table)) % 16 == 0 &&
+           (a.sts | a.shs | a.dts | a.dhs) % v == 0 && a.D % v == 0 && r % v == 0 && a.R % 4 == 0 && a.n_heads <= 4096;
+}
+
+template <int T> void rope_launch(const RopeArgs & a, cudaStream_t st) {
+    if (!rope_vector(a, T)) {
+        rope_kernel<T><<<(unsigned) ((a.n_tok * a.n_heads + 7) / 8), 256, 0, st>>>(a);
+        return;
+    }
+    constexpr int  V     = vec16<T>::N;
+    const uint32_t rot   = (uint32_t) (a.half ? a.R / 2 : a.R) / V;
+    const uint32_t units = rot + (uint32_t) (a.D - a.R) / V;
+    const uint32_t n     = (uint32_t) a.n_heads * units;
+    // i / units as the high word of i * magic: exact while i * units < 2^32 (4096 heads of at most 256 units)
+    const uint32_t magic = units == 1 ? 0 : (uint32_t) ((0x100000000ull + units - 1) / units);
+    // each thread takes two units; the threads that a token does not need take further tokens
+    uint32_t bx = 32;
+    while (bx < 256 && bx * 2 < n) {
+        bx *= 2;
+    }
+    const dim3     block(bx, 256 / bx);
+    const unsigned grid = (unsigned) ((a.n_tok + block.y - 1) / block.y);
+    if (a.half) {
+        rope_vec_kernel<T, true><<<grid, block, 0, st>>>(a, rot, units, magic);
+    } else {
+        rope_vec_kernel<T, false><<<grid, block, 0, st>>>(a, rot, units, magic);
+    }
+}
+
 }  // namespace
 }  // namespace acb
 
@@ -98,17 +210,13 @@ extern "C" acb_status acb_rope(const void * src, int64_t src_tok_stride, int64_t
                          n_tok,    n_heads,        head_dim,        rope_dim,   pos,            rope_table,
                          max_pos,  err_flag,       (layout & ACB_ROPE_INTERLEAVED) == 0,
                          (layout & ACB_ROPE_INVERSE) != 0,          in_place };
-    const unsigned grid = (unsigned) ((n_tok * n_heads + 7) / 8);
-    cudaStream_t   st   = (cudaStream_t) stream;
-    switch (type) {
-        case ACB_TYPE_F32:
-            rope_kernel<ACB_TYPE_F32><<<grid, 256, 0, st>>>(a);
-            break;
-        case ACB_TYPE_F16:
-            rope_kernel<ACB_TYPE_F16><<<grid, 256, 0, st>>>(a);
-            break;
-        default:
-            rope_kernel<ACB_TYPE_BF16><<<grid, 256, 0, st>>>(a);
+    cudaStream_t st = (cudaStream_t) stream;
+    if (type == ACB_TYPE_F32) {
+        rope_launch<ACB_TYPE_F32>(a, st);
+    } else if (type == ACB_TYPE_F16) {
+        rope_launch<ACB_TYPE_F16>(a, st);
+    } else {
+        rope_launch<ACB_TYPE_BF16>(a, st);
     }
     return launch_status();
 }

@@ -784,14 +784,15 @@ ACB_API acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int type
 
 /* What acb_logits_rules applies to each row; every part may be left out (NULL). All arrays are on the device. */
 typedef struct acb_logit_rules {
-    const int32_t *  hist;        /* [rows][hist_stride] tokens of the prompt, then of the answer */
+    const int32_t *  hist;        /* [rows][hist_stride] tokens of the prompt, then of the answer;
+                                     hist_stride below 2^20 */
     int64_t          hist_stride;
     const int32_t *  hist_len;    /* [rows] tokens of each history (NULL: hist_stride); limited to [0, hist_stride] */
     const int32_t *  prompt_len;  /* [rows] how many of them are the prompt's (NULL: none) */
     const float *    rep;         /* [rows] repetition: x > 0 ? x / rep : x * rep, tokens anywhere in the history */
     const float *    freq;        /* [rows] x -= freq * (times in the answer) */
     const float *    pres;        /* [rows] x -= pres, tokens in the answer */
-    const int32_t *  bias_ids;    /* [rows][n_bias] tokens (negative: unused entry) */
+    const int32_t *  bias_ids;    /* [rows][n_bias] tokens (negative: unused entry), n_bias at most 2047 */
     const float *    bias_val;    /* [rows][n_bias] x += the value; of entries with one token the last holds */
     int64_t          bias_stride; /* elements between rows of both; 0: one list for every row */
     int32_t          n_bias;
