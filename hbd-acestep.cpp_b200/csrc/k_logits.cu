@@ -1,20 +1,29 @@
 // k_logits.cu -- rules on logits in front of the sampler (acb_logits_rules): repetition, frequency and presence
 // penalties, a bias per token and a grammar mask, in one pass over the row.
 //
-// A block owns a chunk of columns of one row, each thread kLCols of them, whose logits are under way before anything else is
-// done. A 32-bit word per column in shared memory then takes the last bias entry of the column (its number + 1 above kBiasBit, by
-// a maximum), whether the prompt holds it, and how often the answer does (whole numbers, so the order of the atomics does not
-// show). The row's bytes bound it; the history is short against them, but every block of the row reads it, so the chunks are
-// large, except where a call of few rows would leave SMs idle.
+// A block owns a slice of one row. It notes in shared memory what the history and the bias list say of its columns, streams the
+// slice through (as it is, or -inf where the mask is closed), and then changes the few columns that were noted, a thread each.
+// The row's bytes bound it. The history is read once by every block of its row, so there are only as many slices as fill
+// the GPU: cut into 19 slices a row, the histories of 128 rows of 151936 were over half of the work (49-62 us in four forms against
+// the slices' REPLACE).
+//
+// A column's word holds the last bias entry of the column (its number + 1 above kBiasBit, by a maximum), whether the prompt
+// has it, and how often the answer does: whole numbers, so the order of the atomics does not show. The words are found by
+// hashing where the history is short enough for it (the slice's distinct tokens are then at most 3/4 of the slots);
+// otherwise the slice is gone through in parts of kWords columns with a word for each column.
 #include "common.cuh"
 
 namespace acb {
 namespace {
 
-constexpr int      kLCols     = 16;
+constexpr int      kLThreads  = 512;
+constexpr int      kWords     = 16384;        // 64 KB
+constexpr int      kSlotsMost = kWords / 2;   // of the hash: a column and its word each
+constexpr int      kHashMost  = kSlotsMost / 4 * 3;
 constexpr int      kBiasBit   = 21;
 constexpr uint32_t kInPrompt  = 1u << 20;
 constexpr uint32_t kCountMask = kInPrompt - 1;  // histories and bias lists are limited to what the fields hold
+constexpr uint32_t kNoColumn  = 0xFFFFFFFFu;
 
 struct RulesArgs {
     const void *    x;
@@ -24,198 +33,268 @@ struct RulesArgs {
     int64_t         V;
     acb_logit_rules r;
     int *           err;
+    int             slice;   // columns of a block, a multiple of 256
+    int             noters;  // threads that go through the history and the bias list
+    int             slots, shift;  // of the hash: 2^(32 - shift)
 };
 
-// VEC: rows are 16-byte aligned on both sides and V is a multiple of 8, so a thread's columns are whole vectors of 8
-template <int TI, int TO, int THREADS, bool VEC>
-__global__ void __launch_bounds__(THREADS) logits_rules_kernel(const RulesArgs a) {
-    constexpr int       C = THREADS * kLCols, G = kLCols / 8;
-    using EI              = typename io<TI>::t;
-    using EO              = typename io<TO>::t;
-    __shared__ uint32_t tab[C];
-    const int           row = blockIdx.y, tid = threadIdx.x;
-    const int64_t       c0  = (int64_t) blockIdx.x * C;
-    const int           n   = (int) min((int64_t) C, a.V - c0);
-    const EI *          x   = reinterpret_cast<const EI *>(a.x) + (int64_t) row * a.ld + c0;
-    EO *                y   = reinterpret_cast<EO *>(a.y) + (int64_t) row * a.ldo + c0;
-    // column of element e of group g: vectors of 8 in turn over the threads, or single columns
-    auto     col = [&](int g, int e) { return VEC ? (g * THREADS + tid) * 8 + e : (g * 8 + e) * THREADS + tid; };
-    vec16<TI> in[G][8 / vec16<TI>::N];
-    float     f[VEC ? 1 : G][8];
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-        if constexpr (VEC) {
-            if (col(g, 0) < n) {
-#pragma unroll
-                for (int v = 0; v < 8 / vec16<TI>::N; v++) {
-                    in[g][v].load(x + col(g, v * vec16<TI>::N));
+// VEC: rows are 16-byte aligned on both sides and V is a multiple of 8
+template <int TI, int TO, bool VEC, bool HASH>
+__global__ void __launch_bounds__(kLThreads, 2) logits_rules_kernel(const RulesArgs a) {
+    using EI = typename io<TI>::t;
+    using EO = typename io<TO>::t;
+    extern __shared__ uint32_t words[];
+    __shared__ uint16_t        taken[HASH ? kHashMost : 1];  // slots in use, so that the change runs with full warps
+    __shared__ int             n_taken;
+    const int     row = blockIdx.y, tid = threadIdx.x;
+    const int64_t c0  = (int64_t) blockIdx.x * a.slice;
+    const int     n   = (int) min((int64_t) a.slice, a.V - c0);
+    const EI *    x   = reinterpret_cast<const EI *>(a.x) + (int64_t) row * a.ld + c0;
+    EO *          y   = reinterpret_cast<EO *>(a.y) + (int64_t) row * a.ldo + c0;
+    const int32_t * hist = a.r.hist ? a.r.hist + (int64_t) row * a.r.hist_stride : nullptr;
+    const int32_t * bids = a.r.bias_ids ? a.r.bias_ids + (int64_t) row * a.r.bias_stride : nullptr;
+    const int       n_bias = bids ? a.r.n_bias : 0;
+    int             len    = hist ? (int) a.r.hist_stride : 0;
+    if (hist && a.r.hist_len) {
+        len = min(max(__ldg(a.r.hist_len + row), 0), len);
+    }
+    const int        np   = a.r.prompt_len ? __ldg(a.r.prompt_len + row) : 0;
+    const int        mr   = !a.r.mask ? -1 : a.r.mask_row ? __ldg(a.r.mask_row + row) : row;
+    const uint32_t * mask = mr >= 0 && mr < a.r.n_masks ? a.r.mask + (int64_t) mr * a.r.mask_stride + (c0 >> 5) : nullptr;
+    bool             bad  = a.r.mask && mr >= a.r.n_masks;
+    const float      rep  = a.r.rep ? __ldg(a.r.rep + row) : 1.0f;
+    const float      freq = a.r.freq ? __ldg(a.r.freq + row) : 0.0f;
+    const float      pres = a.r.pres ? __ldg(a.r.pres + row) : 0.0f;
+
+    // the word of column k of the slice while columns [k0, k1) are looked at; nullptr outside
+    auto word_of = [&](int64_t v, int k0, int k1) -> uint32_t * {
+        bad |= v >= a.V;
+        const int64_t k = v - c0;
+        if (k < k0 || k >= k1) {
+            return nullptr;
+        }
+        if constexpr (HASH) {
+            uint32_t s = ((uint32_t) k * 2654435761u) >> a.shift;
+            for (;;) {  // ends: there are fewer columns than slots
+                const uint32_t old = atomicCAS(&words[s], kNoColumn, (uint32_t) k);
+                if (old == kNoColumn) {
+                    taken[atomicAdd(&n_taken, 1)] = (uint16_t) s;
                 }
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                f[g][e] = col(g, e) < n ? io<TI>::to_f(x[col(g, e)]) : 0.0f;
-            }
-        }
-    }
-    const bool use = a.r.hist != nullptr || a.r.bias_ids != nullptr;
-    int        bad = 0;
-    if (use) {
-        for (int i = tid; i < C / 4; i += THREADS) {
-            reinterpret_cast<uint4 *>(tab)[i] = make_uint4(0, 0, 0, 0);
-        }
-        __syncthreads();
-    }
-    if (a.r.bias_ids) {
-        const int32_t * b = a.r.bias_ids + (int64_t) row * a.r.bias_stride;
-        for (int i = tid; i < a.r.n_bias; i += THREADS) {
-            const int64_t v = __ldg(b + i);
-            if (v >= a.V) {
-                bad = 1;
-            } else if (v >= c0 && v < c0 + n) {
-                atomicMax(&tab[v - c0], (uint32_t) (i + 1) << kBiasBit);
+                if (old == kNoColumn || old == (uint32_t) k) {
+                    return &words[a.slots + s];
+                }
+                s = (s + 1) & (a.slots - 1);
             }
         }
-        __syncthreads();
-    }
-    if (a.r.hist) {
-        const int32_t * h   = a.r.hist + (int64_t) row * a.r.hist_stride;
-        int             len = a.r.hist_len ? __ldg(a.r.hist_len + row) : (int) a.r.hist_stride;
-        len                 = min(max(len, 0), (int) a.r.hist_stride);
-        const int np        = a.r.prompt_len ? __ldg(a.r.prompt_len + row) : 0;
-        constexpr int U     = 8;  // tokens in flight per thread
-        for (int i0 = 0; i0 < len; i0 += THREADS * U) {
+        return &words[k - k0];
+    };
+    const int  nt   = a.noters;
+    auto       sync = [&] { asm volatile("bar.sync 1, %0;" ::"r"(nt) : "memory"); };
+    auto       note = [&](int k0, int k1) {  // called by the first nt threads
+        const int m = HASH ? 2 * a.slots : kWords;
+        if (tid == 0) {
+            n_taken = 0;
+        }
+        for (int i = 4 * tid; i < m; i += 4 * nt) {
+            const uint32_t z                       = HASH && i < a.slots ? kNoColumn : 0u;
+            *reinterpret_cast<uint4 *>(words + i) = make_uint4(z, z, z, z);
+        }
+        sync();
+        for (int i = tid; i < n_bias; i += nt) {
+            if (uint32_t * w = word_of(__ldg(bids + i), k0, k1)) {
+                atomicMax(w, (uint32_t) (i + 1) << kBiasBit);
+            }
+        }
+        if (n_bias > 0) {
+            sync();  // a maximum of whole words: before anything is counted in them
+        }
+        constexpr int U = 8;
+        for (int i0 = tid; i0 < len; i0 += U * nt) {
             int v[U];
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int i = i0 + u * THREADS + tid;
-                v[u]        = i < len ? __ldg(h + i) : -1;
+                v[u] = i0 + u * nt < len ? __ldg(hist + i0 + u * nt) : -1;
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                bad |= v[u] >= a.V;
-                const int64_t k = (int64_t) v[u] - c0;
-                if (k >= 0 && k < n) {
-                    if (i0 + u * THREADS + tid < np) {
-                        atomicOr(&tab[k], kInPrompt);
+                if (uint32_t * w = word_of(v[u], k0, k1)) {
+                    if (i0 + u * nt < np) {
+                        atomicOr(w, kInPrompt);
                     } else {
-                        atomicAdd(&tab[k], 1u);
+                        atomicAdd(w, 1u);
                     }
                 }
             }
         }
+    };
+    // (in place, an open column still holds its logit when this comes: it was written as it was)
+    auto changed = [&](float v, uint32_t w) {
+        if (w & (kInPrompt | kCountMask)) {
+            if (a.r.rep) {
+                v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+            }
+            const uint32_t times = w & kCountMask;
+            if (times) {
+                v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float) times)), pres);
+            }
+        }
+        if (w >> kBiasBit) {
+            v = __fadd_rn(v, __ldg(a.r.bias_val + (int64_t) row * a.r.bias_stride + (w >> kBiasBit) - 1));
+        }
+        return v;
+    };
+    // m words found by at(i, &column), i of this thread's share: logits and masks of several at once, since each comes from far
+    auto change = [&](int m, auto at) {
+        constexpr int U = 8;
+        for (int i0 = tid; i0 < m; i0 += U * kLThreads) {
+            int      k[U];
+            uint32_t w[U], open[U];
+            float    v[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                k[u] = 0;
+                w[u] = i0 + u * kLThreads < m ? at(i0 + u * kLThreads, &k[u]) : 0u;
+                if (w[u]) {
+                    v[u]    = io<TI>::to_f(x[k[u]]);
+                    open[u] = mask ? __ldg(mask + (k[u] >> 5)) >> (k[u] & 31) : 1u;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (w[u] && (open[u] & 1u)) {
+                    y[k[u]] = io<TO>::from_f(changed(v[u], w[u]));
+                }
+            }
+        }
+    };
+
+    const bool use = hist || bids;
+    if (HASH && use && tid < nt) {
+        note(0, n);
     }
-    const uint32_t * mask = nullptr;
-    if (a.r.mask) {
-        const int mr = a.r.mask_row ? __ldg(a.r.mask_row + row) : row;
-        if (mr >= a.r.n_masks) {
-            bad = 1;
-        } else if (mr >= 0) {
-            mask = a.r.mask + (int64_t) mr * a.r.mask_stride;
+    // the stream: by the threads that do not note, or by all
+    const int  st    = HASH && use && nt < kLThreads ? tid - nt : tid;
+    const int  sts   = HASH && use && nt < kLThreads ? kLThreads - nt : kLThreads;
+    if (st < 0) {
+    } else if constexpr (VEC) {
+        constexpr int U = 4, NI = 8 / vec16<TI>::N, NO = 8 / vec16<TO>::N;
+        for (int k0 = st * 8; k0 < n; k0 += U * sts * 8) {
+            vec16<TI> in[U][NI];
+            uint32_t  open[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int k = k0 + u * sts * 8;
+                if (k < n) {
+#pragma unroll
+                    for (int q = 0; q < NI; q++) {
+                        in[u][q].load(x + k + q * vec16<TI>::N);
+                    }
+                    open[u] = mask ? __ldg(mask + (k >> 5)) >> (k & 31) : 0xFFu;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int k = k0 + u * sts * 8;
+                if (k < n) {
+#pragma unroll
+                    for (int q = 0; q < NO; q++) {
+                        vec16<TO> out;
+#pragma unroll
+                        for (int e = 0; e < vec16<TO>::N; e++) {
+                            const int   j = q * vec16<TO>::N + e;
+                            const float v = in[u][j / vec16<TI>::N].get(j % vec16<TI>::N);
+                            out.set(e, (open[u] >> j) & 1u ? v : -INFINITY);
+                        }
+                        out.store(y + k + q * vec16<TO>::N);
+                    }
+                }
+            }
+        }
+    } else {
+        constexpr int U = 8;
+        for (int k0 = st; k0 < n; k0 += U * sts) {
+            float v[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int k = k0 + u * sts;
+                if (k < n) {
+                    v[u] = io<TI>::to_f(x[k]);
+                    v[u] = mask && !((__ldg(mask + (k >> 5)) >> (k & 31)) & 1u) ? -INFINITY : v[u];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int k = k0 + u * sts;
+                if (k < n) {
+                    y[k] = io<TO>::from_f(v[u]);
+                }
+            }
+        }
+    }
+    if (use) {
+        if constexpr (HASH) {
+            __syncthreads();
+            change(n_taken, [&](int i, int * k) {
+                *k = (int) words[taken[i]];
+                return words[a.slots + taken[i]];
+            });
+        } else {
+            for (int k0 = 0; k0 < n; k0 += kWords) {
+                const int k1 = min(n, k0 + kWords);
+                __syncthreads();  // the part before has been read, the slice written
+                note(k0, k1);
+                __syncthreads();
+                change(k1 - k0, [&](int i, int * k) {
+                    *k = k0 + i;
+                    return words[i];
+                });
+            }
         }
     }
     if (bad && a.err) {
         atomicOr(a.err, ACB_DEVERR_ID_RANGE);
     }
-    const float rep  = a.r.rep ? __ldg(a.r.rep + row) : 1.0f;
-    const float freq = a.r.freq ? __ldg(a.r.freq + row) : 0.0f;
-    const float pres = a.r.pres ? __ldg(a.r.pres + row) : 0.0f;
-    if (use) {
-        __syncthreads();
-    }
-    auto change = [&](float v, uint32_t w) {
-        if (w) {
-            if (w & (kInPrompt | kCountMask)) {
-                if (a.r.rep) {
-                    v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-                }
-                const uint32_t k = w & kCountMask;
-                if (k) {
-                    v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float) k)), pres);
-                }
-            }
-            if (w >> kBiasBit) {
-                v = __fadd_rn(v, __ldg(a.r.bias_val + (int64_t) row * a.r.bias_stride + (w >> kBiasBit) - 1));
-            }
-        }
-        return v;
-    };
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-        if constexpr (VEC) {
-            const int c = col(g, 0);
-            if (c >= n) {
-                continue;
-            }
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                v[e] = in[g][e / vec16<TI>::N].get(e % vec16<TI>::N);
-            }
-            if (use) {
-                const uint4 w0 = *reinterpret_cast<const uint4 *>(tab + c), w1 = *reinterpret_cast<const uint4 *>(tab + c + 4);
-                if (w0.x | w0.y | w0.z | w0.w | w1.x | w1.y | w1.z | w1.w) {
-                    const uint32_t w[8] = { w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w };
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        v[e] = change(v[e], w[e]);
-                    }
-                }
-            }
-            if (mask) {
-                const uint32_t m = __ldg(mask + ((c0 + c) >> 5)) >> ((c0 + c) & 31);
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    v[e] = (m >> e) & 1u ? v[e] : -INFINITY;
-                }
-            }
-            vec16<TO> out;
-#pragma unroll
-            for (int q = 0; q < 8 / vec16<TO>::N; q++) {
-#pragma unroll
-                for (int e = 0; e < vec16<TO>::N; e++) {
-                    out.set(e, v[q * vec16<TO>::N + e]);
-                }
-                out.store(y + c + q * vec16<TO>::N);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int c = col(g, e);
-                if (c < n) {
-                    float v = use ? change(f[g][e], tab[c]) : f[g][e];
-                    if (mask && !((__ldg(mask + ((c0 + c) >> 5)) >> ((c0 + c) & 31)) & 1u)) {
-                        v = -INFINITY;
-                    }
-                    y[c] = io<TO>::from_f(v);
-                }
-            }
-        }
-    }
 }
 
-template <int TI, int TO> void rules_launch(const RulesArgs & a, int rows, cudaStream_t st) {
-    const bool vec = (reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y)) % 16 == 0 &&
+template <int TI, int TO> acb_status rules_launch(RulesArgs a, int rows, cudaStream_t st) {
+    const bool vec  = (reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.y)) % 16 == 0 &&
                      (a.ld * type_size(TI) | a.ldo * type_size(TO)) % 16 == 0 && a.V % 8 == 0;
-    // 8192 columns a block; 2048 where that leaves SMs without a block
-    const bool    few = (a.V + 8191) / 8192 * rows < num_sms();
-    const int     c   = few ? 128 * kLCols : 512 * kLCols;
-    const dim3    grid((unsigned) ((a.V + c - 1) / c), (unsigned) rows);
-    if (few) {
-        (vec ? logits_rules_kernel<TI, TO, 128, true> : logits_rules_kernel<TI, TO, 128, false>)<<<grid, 128, 0, st>>>(a);
-    } else {
-        (vec ? logits_rules_kernel<TI, TO, 512, true> : logits_rules_kernel<TI, TO, 512, false>)<<<grid, 512, 0, st>>>(a);
+    const bool use  = a.r.hist || a.r.bias_ids;
+    const bool hash = (a.r.hist ? a.r.hist_stride : 0) + (a.r.bias_ids ? a.r.n_bias : 0) <= kHashMost;
+    // two blocks fit on an SM: one slice per block of a full GPU, or of four full GPUs where the rows alone fill it, and
+    // at least 2048 columns each
+    const int64_t full = 2 * (int64_t) num_sms();
+    int64_t       cut  = rows * 2 > full ? (4 * full + rows - 1) / rows : full / rows;
+    cut                = cut < 1 ? 1 : cut;
+    int64_t slice      = ((a.V + cut - 1) / cut + 255) / 256 * 256;
+    a.slice            = (int) (slice < 2048 ? 2048 : slice);
+    // a long slice's stream takes longer than the history: four warps note while the others stream
+    a.noters = a.slice >= 16384 && hash ? 128 : kLThreads;
+    a.slots  = 64;
+    a.shift  = 32 - 6;
+    while (hash && a.slots / 4 * 3 < (a.r.hist ? a.r.hist_stride : 0) + (a.r.bias_ids ? a.r.n_bias : 0)) {
+        a.slots *= 2;
+        a.shift--;
     }
+    const dim3   grid((unsigned) ((a.V + a.slice - 1) / a.slice), (unsigned) rows);
+    const size_t smem = !use ? 0 : (hash ? 2 * a.slots : kWords) * sizeof(uint32_t);
+    const auto   kern = vec ? (hash ? logits_rules_kernel<TI, TO, true, true> : logits_rules_kernel<TI, TO, true, false>)
+                            : (hash ? logits_rules_kernel<TI, TO, false, true> : logits_rules_kernel<TI, TO, false, false>);
+    if (smem) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
+        if (e != cudaSuccess) {
+            set_last_cuda_error(e);
+            return ACB_ERR_CUDA;
+        }
+    }
+    kern<<<grid, kLThreads, smem, st>>>(a);
+    return launch_status();
 }
 
-template <int TI> void rules_launch(const RulesArgs & a, int to, int rows, cudaStream_t st) {
-    if (to == ACB_TYPE_F32) {
-        rules_launch<TI, ACB_TYPE_F32>(a, rows, st);
-    } else if (to == ACB_TYPE_F16) {
-        rules_launch<TI, ACB_TYPE_F16>(a, rows, st);
-    } else {
-        rules_launch<TI, ACB_TYPE_BF16>(a, rows, st);
-    }
+template <int TI> acb_status rules_launch(const RulesArgs & a, int to, int rows, cudaStream_t st) {
+    return to == ACB_TYPE_F32   ? rules_launch<TI, ACB_TYPE_F32>(a, rows, st)
+           : to == ACB_TYPE_F16 ? rules_launch<TI, ACB_TYPE_F16>(a, rows, st)
+                                : rules_launch<TI, ACB_TYPE_BF16>(a, rows, st);
 }
 
 }  // namespace
@@ -246,14 +325,9 @@ extern "C" acb_status acb_logits_rules(const void * logits, int type, int64_t ld
     if (rows == 0) {
         return ACB_OK;
     }
-    const RulesArgs a  = { logits, ld, out, ld_out, V, r, err_flag };
+    const RulesArgs a  = { logits, ld, out, ld_out, V, r, err_flag, 0, 0, 0, 0 };
     cudaStream_t    st = (cudaStream_t) stream;
-    if (type == ACB_TYPE_F32) {
-        rules_launch<ACB_TYPE_F32>(a, out_type, rows, st);
-    } else if (type == ACB_TYPE_F16) {
-        rules_launch<ACB_TYPE_F16>(a, out_type, rows, st);
-    } else {
-        rules_launch<ACB_TYPE_BF16>(a, out_type, rows, st);
-    }
-    return launch_status();
+    return type == ACB_TYPE_F32   ? rules_launch<ACB_TYPE_F32>(a, out_type, rows, st)
+           : type == ACB_TYPE_F16 ? rules_launch<ACB_TYPE_F16>(a, out_type, rows, st)
+                                  : rules_launch<ACB_TYPE_BF16>(a, out_type, rows, st);
 }

@@ -160,11 +160,10 @@ template <int T> void rope_launch(const RopeArgs & a, cudaStream_t st) {
     const uint32_t n     = (uint32_t) a.n_heads * units;
     // i / units as the high word of i * magic: exact while i * units < 2^32 (4096 heads of at most 256 units)
     const uint32_t magic = units == 1 ? 0 : (uint32_t) ((0x100000000ull + units - 1) / units);
-    // each thread takes two units; the threads that a token does not need take further tokens
-    uint32_t bx = 32;
-    while (bx < 256 && bx * 2 < n) {
-        bx *= 2;
-    }
+    // each thread takes two units a time, as few idle as whole warps allow; what a small token leaves of 256 threads takes
+    // further tokens
+    const uint32_t turns = (n + 511) / 512;
+    const uint32_t bx    = ((n + 2 * turns - 1) / (2 * turns) + 31) / 32 * 32;
     const dim3     block(bx, 256 / bx);
     const unsigned grid = (unsigned) ((a.n_tok + block.y - 1) / block.y);
     if (a.half) {

@@ -1,5 +1,7 @@
 """Plain implementations in 64 bits of the serving operators (rotary layouts, the paged 4-bit KV cache, attention over it,
 rules on logits), for the tests: loops and numpy, nothing of the library."""
+import collections
+
 import numpy as np
 
 HALF_STEP = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}  # of a rounding, relative to the value
@@ -89,8 +91,7 @@ def rules(x, hist=None, n_prompt=0, rep=None, freq=None, pres=None, bias=(), mas
             if rep is not None:
                 x[t] = x[t] / rep if x[t] > 0 else x[t] * rep
             m[t] = max(m[t], abs(x[t]))
-        for t in set(out):
-            n = out.count(t)
+        for t, n in collections.Counter(out).items():
             for term in ((freq or 0.0) * n, pres or 0.0):
                 x[t] -= term
                 m[t] += abs(term)

@@ -83,6 +83,22 @@ def test_each_part_alone(cuda, kind):
     _check(y.float().cpu().numpy().astype(np.float64), xs, R, kind, bits=bits)
 
 
+@pytest.mark.parametrize("R,V,L", [(1, 3000, 20000), (300, 9000, 6000), (2, 40, 5000)])
+def test_histories_that_name_nearly_every_column(cuda, R, V, L):
+    import torch
+    rng = np.random.default_rng(V)
+    x = torch.from_numpy(rng.standard_normal((R, V)).astype(np.float32))
+    hist = rng.integers(0, V, (R, L)).astype(np.int32)
+    rep, freq = (rng.uniform(0.1, 1.5, R).astype(np.float32) for _ in "rf")
+    prompt = np.full(R, L // 4, np.int32)
+    bias = [rng.integers(0, V, (R, 2047)).astype(np.int32), rng.standard_normal((R, 2047)).astype(np.float32)]
+    c = lambda a: torch.from_numpy(a).cuda()  # noqa: E731
+    y = acb.logits_rules(x.cuda(), c(hist), None, c(prompt), c(rep), c(freq), None, c(bias[0]), c(bias[1]))
+    rows = [0, R - 1]
+    _check(y.cpu().numpy().astype(np.float64)[rows], x.numpy()[rows], len(rows), "f32", hist[rows], None, prompt[rows], rep[rows],
+           freq[rows], None, [b[rows] for b in bias])
+
+
 def test_in_place_strides_and_rows_around(cuda):
     import torch
     rng = np.random.default_rng(4)
