@@ -74,47 +74,9 @@ template <bool SPLIT> struct TcLayout {
     static constexpr uint32_t TO = 256, TQ = 384;
 };
 
-// 2^x on the special-function unit (relative error ~2^-22; -inf -> +0, denormal results flush to 0)
-__device__ __forceinline__ float ex2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // lazy rescaling: the reference max of a row moves only when a block max exceeds it by more than
 // this many powers of two
 constexpr float kRescaleLog2 = 8.0f;
-
-__device__ __forceinline__ bool tc_wait(uint64_t * bar, uint32_t parity, volatile int * abort_flag, int * err) {
-    if (*abort_flag) {
-        return false;
-    }
-    if (!ptx::mbar_wait(bar, parity)) {
-        *abort_flag = 1;
-        if (err) {
-            atomicOr(err, ACB_DEVERR_TIMEOUT);
-        }
-        return false;
-    }
-    return true;
-}
-
-// D (TMEM) += A (TMEM: lane = row, two f16 of K per 32-bit column) x B (shared-memory descriptor)
-__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(b), "r"(idesc), "r"(acc));
-}
-
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t * r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
-            taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
 
 template <int MASK, bool SPLIT>
 __global__ void __launch_bounds__(kTcThreads, 1)

@@ -193,7 +193,7 @@ template <int TI, int TQ, int D> __global__ void __launch_bounds__(256) kv_q4_ap
 constexpr int kAppendWarps = 4;
 
 template <int TI, int TQ, int D, int ROPE>
-__global__ void __launch_bounds__(32 * kAppendWarps, 8) kv_q4_append_vec_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(32 * kAppendWarps, 7) kv_q4_append_vec_kernel(const AppendArgs a) {
     constexpr int LPR = D / 8, RPW = 32 / LPR, VI = vec16<TI>::N, VQ = vec16<TQ>::N, U = TI == ACB_TYPE_F32 ? 1 : 2;
     constexpr int TURN = kAppendWarps * RPW;  // rows of one row a thread
     using EI           = typename io<TI>::t;
