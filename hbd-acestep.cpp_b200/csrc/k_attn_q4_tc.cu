@@ -1,16 +1,19 @@
 // k_attn_q4_tc.cu -- attention over the paged 4-bit KV cache for chunks of prompts, on the 5th-generation tensor cores.
 //
-// One CTA per 128 rows (new token * G + query head of the group) of a sequence and kv head; key blocks of 128. The layout of
-// TMEM and the softmax are those of k_attn_tc.cu: two S/P buffers, O and Q in TMEM, A of both products from TMEM, two softmax
-// threads a row. What differs is where K and V come from: four warps read the codes from the pages and write f16 tiles
-// into shared memory (every cached value is an f16 number, so nothing is rounded), K^ [key][dim] and V^T [dim][key], both
-// K-major with the 128-byte swizzle:
-//   K: a thread a key; the 8 dimensions of a word of codes make one 16-byte unit in the order that unpack4 gives them, and Q
-//      is put into TMEM in the same order (a product does not depend on the order of its k index);
-//   V: a thread 8 keys by 16 dimensions: the words of two keys are merged by halves, so that unpack4 gives pairs of keys, and
-//      four pairs make the 16-byte unit of a dimension.
-// A block costs the tensor cores 2 x 512 cycles (D = 128), the exponentials 1024 cycles of the special-function units, and the
-// unpacking about 520 issue slots of each scheduler beside the softmax's 700: all three overlap.
+// One CTA per 256 rows (new token * G + query head of the group) of a sequence and kv head, in two tiles of 128; key blocks of
+// 128. Every cached value is an f16 number, so nothing is rounded on the way into the tiles. 17 warps:
+//   0..3, 4..7  softmax of tile 0 and of tile 1, a thread a row (a TMEM lane): 64 scores at a time: the maximum of
+//               the first half, that of the second, the second's exponentials, the first half again for its own; P takes the
+//               second half's columns as f16. (Two threads a row with both halves of one
+//               tile in registers, and the exchange that takes, held the tensor cores at 20%: 462 us where this takes REPLACE.)
+//   8..11       K: a thread a key; the 8 dimensions of a word of codes make one 16-byte unit in the order that unpack4 gives
+//               them, and Q is written in the same order (a product does not depend on the order of its k index);
+//   12..15      V^T: a thread 8 keys by 16 dimensions: the words of two keys are merged by halves, so that unpack4 gives pairs of
+//               keys, and four pairs make the 16-byte unit of a dimension;
+//   16          one thread issues the products: S = Q K^T from shared memory, O += P V with P from TMEM. P.V of a tile is
+//               followed by its next S, which may then take P's place; meanwhile the other tile's softmax runs.
+// Per key block and tile the tensor cores need 1024 cycles (D = 128) and so do the exponentials; shared memory moves 128 bytes a
+// cycle during Q K^T. The unpacking is shared by the tiles.
 //
 // Every wait is bounded, as in k_attn_tc.cu.
 #include "attn_q4.cuh"
@@ -20,42 +23,57 @@
 namespace acb {
 namespace {
 
-constexpr int   kQtRows    = 128;
+constexpr int   kQtRows    = 128;  // of a tile
 constexpr int   kQtKeys    = 128;
-constexpr int   kQtSoft    = 8;   // softmax warps 0..7
-constexpr int   kQtMma     = 8;   // the warp that issues the products
-constexpr int   kQtUnpack  = 4;   // unpacking warps 9..12
-constexpr int   kQtThreads = 32 * (kQtSoft + 1 + kQtUnpack);
+constexpr int   kQtSoft    = 8;   // softmax warps
+constexpr int   kQtUnpack  = 4;   // warps that unpack K, and as many for V
+constexpr int   kQtMma     = kQtSoft + 2 * kQtUnpack;
+constexpr int   kQtThreads = 32 * (kQtMma + 1);
 constexpr float kQtLag     = 8.0f;  // the reference maximum moves when exceeded by more than 2^kQtLag
 constexpr float kQtLift    = 6.0f;  // P is held times 2^kQtLift: at most 2^14
 constexpr int   kQtRing    = 8;     // blocks whose notes are kept
 
 template <int D> struct QtLayout {
-    static constexpr int KB = kQtKeys * D * 2, VB = kQtKeys * D * 2, NK = 2, NV = 2;
-    static constexpr int TOTAL = NK * KB + NV * VB;
-    // TMEM columns: S/P buffers at 0 and 128, O at 256, Q at 384 (two f16 a column)
-    static constexpr uint32_t TO = 256, TQ = 384;
+    static constexpr int QB = kQtRows * D * 2, KB = kQtKeys * D * 2, VB = kQtKeys * D * 2, NK = 2, NV = 2;
+    static constexpr int TOTAL = 2 * QB + NK * KB + NV * VB;
+    // TMEM columns: S/P of the tiles at 0 and 128, O at 256 and 384
 };
+
+// 64 columns of this warp's lanes
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t * r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+          "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+          "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+          "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+          "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        : "r"(taddr)
+        : "memory");
+}
 
 template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThreads, 1) attn_q4_tc_kernel(const AttnQ4Args a) {
     using Lay = QtLayout<D>;
     using T1  = typename io<T>::t;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t *  sK      = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *  sQ      = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *  sK      = sQ + 2 * Lay::QB;
     uint8_t *  sV      = sK + Lay::NK * Lay::KB;
     uint64_t * q_full  = reinterpret_cast<uint64_t *>(sV + Lay::NV * Lay::VB);
     uint64_t * k_full  = q_full + 1;
     uint64_t * k_empty = k_full + Lay::NK;
     uint64_t * v_full  = k_empty + Lay::NK;
     uint64_t * v_empty = v_full + Lay::NV;
-    uint64_t * s_full  = v_empty + Lay::NV;  // [2]
+    uint64_t * s_full  = v_empty + Lay::NV;  // [2], of the tiles: S(i) is there, and P.V(i - 1) done
     uint64_t * p_full  = s_full + 2;         // [2]
-    uint64_t * pv_done = p_full + 2;         // [2]
-    uint64_t * o_done  = pv_done + 2;
-    uint64_t * xbar    = o_done + 1;  // [4]: softmax pairs, one per TMEM lane quarter
-    uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(xbar + 4);
+    uint64_t * o_done  = p_full + 2;         // [2]
+    uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(o_done + 2);
     __shared__ volatile int abort_flag;
-    __shared__ float        xchg[2 * 2 * kQtRows];  // [parity][half][row]
     // notes on a block, for what hardly ever happens: keys whose page is not in the pool, and per 32 dimensions the keys whose
     // value scale is no number (their values are left out of the product, where 0 * NaN would reach the rows that do not see
     // them, and make their dimensions NaN in the rows that do)
@@ -71,11 +89,12 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
         atomicOr(a.err, ACB_DEVERR_LEN_RANGE);
     }
     // the longest rows first: what is left for the end is short
-    const int r0 = (int) (gridDim.x - 1 - blockIdx.x) * kQtRows;
+    const int r0 = (int) (gridDim.x - 1 - blockIdx.x) * 2 * kQtRows;
     if (r0 >= n * a.G) {
         return;
     }
-    const int i0 = r0 / a.G, i1 = min(n - 1, (r0 + kQtRows - 1) / a.G);
+    const int tiles = r0 + kQtRows < n * a.G ? 2 : 1;
+    const int i0 = r0 / a.G, i1 = min(n - 1, (r0 + 2 * kQtRows - 1) / a.G);
     const int p0 = okay ? len - n + i0 : -1, p1 = okay ? len - n + i1 : -1;
     const int key_lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
     const int kb_lo  = key_lo / kQtKeys;
@@ -83,7 +102,7 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
 
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        ptx::mbar_init(q_full, kQtSoft);
+        ptx::mbar_init(q_full, kQtSoft / 2 * tiles);
         for (int i = 0; i < Lay::NK; i++) {
             ptx::mbar_init(&k_full[i], kQtUnpack);
             ptx::mbar_init(&k_empty[i], 1);
@@ -94,12 +113,8 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
         }
         for (int i = 0; i < 2; i++) {
             ptx::mbar_init(&s_full[i], 1);
-            ptx::mbar_init(&p_full[i], kQtSoft);
-            ptx::mbar_init(&pv_done[i], 1);
-        }
-        ptx::mbar_init(o_done, 1);
-        for (int x = 0; x < 4; x++) {
-            ptx::mbar_init(&xbar[x], 2);
+            ptx::mbar_init(&p_full[i], kQtSoft / 2);
+            ptx::mbar_init(&o_done[i], 1);
         }
         ptx::fence_mbar_init();
     }
@@ -121,81 +136,44 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const uint32_t tO = tmem + Lay::TO, tQ = tmem + Lay::TQ;
 
-    if (warp > kQtMma) {
-        // ---- unpacking ----
-        const int tid = threadIdx.x - 32 * (kQtMma + 1);  // 0..127
-        // K: this thread's key of a block
-        Words<D / 8>  kw;
-        Words<D / 64> ksw;
-        int           kpg = 0;
-        auto          key_of = [&](int i) { return min((kb_lo + i) * kQtKeys + tid, p1); };
-        auto          k_page = [&](int i) { kpg = a.kv.page_of(s, key_of(i)); };
-        bool          k_bad  = false;
-        auto          k_load = [&](int i) {
-            const int j = key_of(i);
-            k_bad       = kpg < 0;
-            if (!k_bad) {
-                const int64_t row = a.kv.row(kpg, hk, j);
-                kw.load(a.kv.kc + row * (D / 2));
-                ksw.load(a.kv.ks + row * (D / 32));
-            }
-        };
-        // V: 8 keys from 8 kg on, 16 dimensions: the 8 bytes from 8 wq on; lanes of a store phase differ in kg
-        const int kg = (tid & 7) | ((tid >> 6) << 3), wq = (tid >> 3) & 7;
-        constexpr bool ALL = D == 128;  // heads of 64 have 4 such 8-byte runs: half the threads have none
-        const bool     v_on = ALL || wq < 4;
-        uint2          vw[8];
-        uint16_t       vs[8];
-        int            vpg = 0;
-        uint32_t       v_bad = 0;
-        auto           v_page = [&](int i) { vpg = a.kv.page_of(s, min((kb_lo + i) * kQtKeys + 8 * kg, p1)); };
-        auto           v_load = [&](int i) {
-            const int j = (kb_lo + i) * kQtKeys + 8 * kg;  // 8 keys of one page (pages hold 16 or more)
-            if (v_on) {
-                const int64_t   row = vpg < 0 ? 0 : a.kv.row(vpg, hk, j);
-                const uint8_t * c   = a.kv.vc + row * (D / 2) + wq * 8;
-                const uint16_t * d  = a.kv.vs + row * (D / 32) + (wq >> 1);
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    // a key past the last one: none of its own (the page may hold anything there)
-                    const bool in = vpg >= 0 && j + e <= p1;
-                    vw[e]         = in ? __ldg(reinterpret_cast<const uint2 *>(c + e * (D / 2))) : make_uint2(0, 0);
-                    vs[e]         = in ? __ldg(d + e * (D / 32)) : (uint16_t) 0;
+    if (warp >= kQtSoft && warp < kQtMma) {
+        // ---- unpacking: four warps K, four warps V ----
+        const int tid = threadIdx.x & (32 * kQtUnpack - 1);  // 0..127 of each
+        if (warp < kQtSoft + kQtUnpack) {
+            // K: this thread's key of a block
+            Words<D / 8>  kw;
+            Words<D / 64> ksw;
+            bool          k_bad = false;
+            int           pg    = nblk > 0 ? a.kv.page_of(s, min(kb_lo * kQtKeys + tid, p1)) : 0;
+            auto          load  = [&](int i) {
+                const int j = min((kb_lo + i) * kQtKeys + tid, p1);
+                k_bad       = pg < 0;
+                if (!k_bad) {
+                    const int64_t row = a.kv.row(pg, hk, j);
+                    kw.load(a.kv.kc + row * (D / 2));
+                    ksw.load(a.kv.ks + row * (D / 32));
                 }
+            };
+            if (nblk > 0) {
+                load(0);
             }
-        };
-        if (nblk > 0) {
-            k_page(0);
-            v_page(0);
-            k_load(0);
-        }
-        for (int i = 0; i < nblk; i++) {
-            v_load(i);
-            if (i + 1 < nblk) {
-                k_page(i + 1);
-                v_page(i + 1);
-            }
-            const int sk = i % Lay::NK, sv = i % Lay::NV, note = i % kQtRing;
-            if (!__all_sync(0xffffffffu, i < Lay::NK || tc_wait(&k_empty[sk], (i / Lay::NK - 1) & 1, &abort_flag, a.err))) {
-                break;
-            }
-            // Room for the notes of block i + 2, where those of block i - 6 are: S(i - 2) is done, so the softmax has published
-            // P(i - 4) and looked at block i - 6; and no unpacking warp is at block i + 2 before this one has filled block i.
-            if (tid < 32) {
-                const int next = (i + 2) % kQtRing;
-                if (lane < 4) {
-                    bad_key[next][lane] = 0;
+            for (int i = 0; i < nblk; i++) {
+                if (i + 1 < nblk) {
+                    pg = a.kv.page_of(s, min((kb_lo + i + 1) * kQtKeys + tid, p1));
                 }
-                if (lane < (D / 32) * 4) {
-                    (&bad_val[next][0][0])[lane] = 0;
+                const int sk = i % Lay::NK, note = i % kQtRing, next = (i + 2) % kQtRing;
+                if (!__all_sync(0xffffffffu, i < Lay::NK || tc_wait(&k_empty[sk], (i / Lay::NK - 1) & 1, &abort_flag, a.err))) {
+                    break;
                 }
-                if (lane < 2) {
-                    bad_any[next][lane] = 0;
+                // Room for the notes of block i + 2, where those of block i - 6 are: both tiles' S(i - 2) are done, so both
+                // softmaxes are past block i - 3, and no K warp is at block i + 2 before this one has filled block i. (V: the
+                // same with P.V.)
+                if (tid < 4) {
+                    bad_key[next][tid] = 0;
+                } else if (tid == 4) {
+                    bad_any[next][0] = 0;
                 }
-            }
-            {
                 const bool gone = (kb_lo + i) * kQtKeys + tid > p1;
                 if (k_bad && !gone) {
                     atomicOr(&bad_key[note][tid >> 5], 1u << (tid & 31));
@@ -204,65 +182,111 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
                         atomicOr(a.err, ACB_DEVERR_PAGE_RANGE);
                     }
                 }
+                if (k_bad || gone) {
+#pragma unroll
+                    for (int w = 0; w < D / 64; w++) {
+                        ksw.w[w] = 0;
+                    }
+                }
                 uint8_t * dst = sK + sk * Lay::KB + tid * 128;
 #pragma unroll
                 for (int w = 0; w < D / 8; w++) {
-                    const uint32_t sc = ksw.w[w / 8] >> (16 * ((w / 4) & 1));
-                    uint32_t       r[4];
-                    unpack4(kw.w[w], __half2half2(__ushort_as_half((uint16_t) (k_bad || gone ? 0u : sc))), r);
+                    uint32_t r[4];
+                    unpack4(kw.w[w], half2_of(__byte_perm(ksw.w[w / 8], 0, (w / 4) & 1 ? 0x3232u : 0x1010u)), r);
                     *reinterpret_cast<uint4 *>(dst + (w / 8) * 16384 + (((w & 7) ^ (tid & 7)) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
                 }
+                if (i + 1 < nblk) {
+                    load(i + 1);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::mbar_arrive(&k_full[sk]);
+                }
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                ptx::mbar_arrive(&k_full[sk]);
-            }
-            if (i + 1 < nblk) {
-                k_load(i + 1);
-            }
-            if (!__all_sync(0xffffffffu, i < Lay::NV || tc_wait(&v_empty[sv], (i / Lay::NV - 1) & 1, &abort_flag, a.err))) {
-                break;
-            }
-            if (v_on) {
-                v_bad = 0;
+        } else {
+            // V: 8 keys from 8 kg on (of one page: pages hold 16 or more), 16 dimensions: the 8 bytes from 8 wq on; the lanes of a
+            // store phase differ in kg
+            const int kg = (tid & 7) | ((tid >> 6) << 3), wq = (tid >> 3) & 7;
+            const bool on = D == 128 || wq < 4;  // heads of 64 have 4 such runs
+            uint2      vw[8];
+            uint16_t   vs[8];
+            int        pg   = nblk > 0 ? a.kv.page_of(s, min(kb_lo * kQtKeys + 8 * kg, p1)) : 0;
+            auto       load = [&](int i) {
+                const int j = (kb_lo + i) * kQtKeys + 8 * kg;
+                if (on) {
+                    const int64_t    row = pg < 0 ? 0 : a.kv.row(pg, hk, j);
+                    const uint8_t *  c   = a.kv.vc + row * (D / 2) + wq * 8;
+                    const uint16_t * d   = a.kv.vs + row * (D / 32) + (wq >> 1);
+                    const int        in  = pg < 0 ? 0 : p1 - j + 1;  // keys past the last one: none of their own
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    if ((vs[e] & 0x7C00u) == 0x7C00u) {
-                        vs[e] = 0;
-                        v_bad |= 1u << e;
+                    for (int e = 0; e < 8; e++) {
+                        vw[e] = e < in ? __ldg(reinterpret_cast<const uint2 *>(c + e * (D / 2))) : make_uint2(0, 0);
+                        vs[e] = e < in ? __ldg(d + e * (D / 32)) : (uint16_t) 0;
                     }
                 }
-                if (v_bad) {
-                    atomicOr(&bad_val[note][wq >> 1][kg >> 2], v_bad << (8 * (kg & 3)));
-                    bad_any[note][1] = 1;
+            };
+            if (nblk > 0) {
+                load(0);
+            }
+            for (int i = 0; i < nblk; i++) {
+                if (i + 1 < nblk) {
+                    pg = a.kv.page_of(s, min((kb_lo + i + 1) * kQtKeys + 8 * kg, p1));
                 }
-                uint32_t sc[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    sc[e] = (uint32_t) vs[2 * e] | ((uint32_t) vs[2 * e + 1] << 16);
+                const int sv = i % Lay::NV, note = i % kQtRing, next = (i + 2) % kQtRing;
+                if (!__all_sync(0xffffffffu, i < Lay::NV || tc_wait(&v_empty[sv], (i / Lay::NV - 1) & 1, &abort_flag, a.err))) {
+                    break;
                 }
-                uint8_t * base = sV + sv * Lay::VB + (kg >> 3) * (D * 128);
-#pragma unroll
-                for (int h = 0; h < 4; h++) {  // bytes 2h and 2h + 1 of the 8
-                    uint32_t r[4][4];          // [pair of keys][low, high of byte 2h, low, high of byte 2h + 1]
+                if (tid < (D / 32) * 4) {
+                    (&bad_val[next][0][0])[tid] = 0;
+                } else if (tid == (D / 32) * 4) {
+                    bad_any[next][1] = 0;
+                }
+                if (on) {
+                    uint32_t sc[4], odd = 0;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const uint32_t x = h < 2 ? vw[2 * e].x : vw[2 * e].y, y = h < 2 ? vw[2 * e + 1].x : vw[2 * e + 1].y;
-                        unpack4(__byte_perm(x, y, (h & 1) ? 0x7632u : 0x5410u), half2_of(sc[e]), r[e]);
+                        sc[e] = (uint32_t) vs[2 * e] | ((uint32_t) vs[2 * e + 1] << 16);
+                        // exponent field full: adding one unit carries into the sign's place
+                        odd |= (((sc[e] & 0x7C007C00u) + 0x04000400u) & 0x80008000u);
                     }
+                    if (odd) {
+                        uint32_t bits = 0;
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const int d = (wq >> 1) * 32 + (wq & 1) * 8 + 2 * h + (q >> 1) + 16 * (q & 1);
-                        *reinterpret_cast<uint4 *>(base + d * 128 + (((kg & 7) ^ (d & 7)) << 4)) =
-                            make_uint4(r[0][q], r[1][q], r[2][q], r[3][q]);
+                        for (int e = 0; e < 8; e++) {
+                            if ((vs[e] & 0x7C00u) == 0x7C00u) {
+                                sc[e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                                bits |= 1u << e;
+                            }
+                        }
+                        atomicOr(&bad_val[note][wq >> 1][kg >> 2], bits << (8 * (kg & 3)));
+                        bad_any[note][1] = 1;
+                    }
+                    uint8_t * base = sV + sv * Lay::VB + (kg >> 3) * (D * 128);
+#pragma unroll
+                    for (int h = 0; h < 4; h++) {  // bytes 2h and 2h + 1 of the 8
+                        uint32_t r[4][4];          // [pair of keys][low, high of byte 2h, low, high of byte 2h + 1]
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t x = h < 2 ? vw[2 * e].x : vw[2 * e].y, y = h < 2 ? vw[2 * e + 1].x : vw[2 * e + 1].y;
+                            unpack4(__byte_perm(x, y, (h & 1) ? 0x7632u : 0x5410u), half2_of(sc[e]), r[e]);
+                        }
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const int d = (wq >> 1) * 32 + (wq & 1) * 8 + 2 * h + (q >> 1) + 16 * (q & 1);
+                            *reinterpret_cast<uint4 *>(base + d * 128 + (((kg & 7) ^ (2 * h + (q >> 1))) << 4)) =
+                                make_uint4(r[0][q], r[1][q], r[2][q], r[3][q]);
+                        }
                     }
                 }
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                ptx::mbar_arrive(&v_full[sv]);
+                if (i + 1 < nblk) {
+                    load(i + 1);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::mbar_arrive(&v_full[sv]);
+                }
             }
         }
     } else if (warp == kQtMma) {
@@ -270,97 +294,99 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
             tc_fence_after();
             constexpr uint32_t idesc_s = idesc_kind_f16(128, kQtKeys, true);
             constexpr uint32_t idesc_o = idesc_kind_f16(128, D, true);
-            auto issue_s = [&](int i) -> bool {
-                const int sk = i % Lay::NK;
-                if (!tc_wait(&k_full[sk], (i / Lay::NK) & 1, &abort_flag, a.err)) {
-                    return false;
-                }
-                tc_fence_after();
-                const uint32_t st = ptx::smem_u32(sK + sk * Lay::KB);
-                const uint32_t tS = tmem + (uint32_t) ((i & 1) * 128);
+            auto issue_s = [&](int t, int i) {
+                const uint32_t q = ptx::smem_u32(sQ + t * Lay::QB), k = ptx::smem_u32(sK + (i % Lay::NK) * Lay::KB);
 #pragma unroll
                 for (int kk = 0; kk < D / 16; kk++) {
-                    umma_ts(tS, tQ + (uint32_t) (kk * 8), smem_desc_sw128(st + (kk >> 2) * 16384 + (kk & 3) * 32), idesc_s, kk > 0);
+                    const uint32_t off = (uint32_t) ((kk >> 2) * 16384 + (kk & 3) * 32);
+                    umma_f16kind(tmem + (uint32_t) (t * 128), smem_desc_sw128(q + off), smem_desc_sw128(k + off), idesc_s, kk > 0);
                 }
-                umma_commit(&s_full[i & 1]);
-                umma_commit(&k_empty[sk]);
-                return true;
+                umma_commit(&s_full[t]);
             };
-            bool ok = issue_s(0) && (nblk < 2 || issue_s(1));
-            for (int i = 0; ok && i < nblk; i++) {
-                if (!tc_wait(&p_full[i & 1], (i >> 1) & 1, &abort_flag, a.err)) {
-                    break;
-                }
-                const int sv = i % Lay::NV;
-                if (!tc_wait(&v_full[sv], (i / Lay::NV) & 1, &abort_flag, a.err)) {
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t vt = ptx::smem_u32(sV + sv * Lay::VB);
-                const uint32_t tP = tmem + (uint32_t) ((i & 1) * 128);
+            auto issue_pv = [&](int t, int i) {
+                const uint32_t v = ptx::smem_u32(sV + (i % Lay::NV) * Lay::VB);
 #pragma unroll
                 for (int kk = 0; kk < kQtKeys / 16; kk++) {
-                    umma_ts(tO, tP + (uint32_t) (kk * 8), smem_desc_sw128(vt + (kk >> 2) * (D * 128) + (kk & 3) * 32), idesc_o,
-                            (i > 0 || kk > 0) ? 1u : 0u);
+                    umma_ts(tmem + (uint32_t) (256 + t * 128), tmem + (uint32_t) (t * 128 + 64 + kk * 8),
+                            smem_desc_sw128(v + (kk >> 2) * (D * 128) + (kk & 3) * 32), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
                 }
-                umma_commit(&pv_done[i & 1]);
-                umma_commit(&v_empty[sv]);
-                if (i + 1 == nblk) {
-                    umma_commit(o_done);
+            };
+            bool ok = tc_wait(&k_full[0], 0, &abort_flag, a.err);
+            if (ok) {
+                tc_fence_after();
+                for (int t = 0; t < tiles; t++) {
+                    issue_s(t, 0);
                 }
-                if (i + 2 < nblk) {
-                    ok = issue_s(i + 2);
+                umma_commit(&k_empty[0]);
+            }
+            for (int i = 0; ok && i < nblk; i++) {
+                const bool more = i + 1 < nblk;
+                for (int t = 0; ok && t < tiles; t++) {
+                    ok = tc_wait(&p_full[t], i & 1, &abort_flag, a.err) &&
+                         (t > 0 || tc_wait(&v_full[i % Lay::NV], (i / Lay::NV) & 1, &abort_flag, a.err));
+                    if (!ok) {
+                        break;
+                    }
+                    tc_fence_after();
+                    issue_pv(t, i);
+                    if (!more) {
+                        umma_commit(&o_done[t]);
+                        continue;
+                    }
+                    ok = t > 0 || tc_wait(&k_full[(i + 1) % Lay::NK], ((i + 1) / Lay::NK) & 1, &abort_flag, a.err);
+                    if (ok) {
+                        tc_fence_after();
+                        issue_s(t, i + 1);
+                    }
                 }
-            }
-        }
-    } else {
-        // ---- softmax: warp w and w + 4 share the TMEM lanes of quarter w % 4 (two threads a row) ----
-        constexpr int  HD    = D / 2;  // dimensions of a thread's half of Q and O
-        const int      qq    = warp & 3, hf = warp >> 2;
-        const int      row   = qq * 32 + lane, r = r0 + row, i_tok = r / a.G;
-        const uint32_t lanes = (uint32_t) (qq * 32) << 16;
-        const bool     live  = i_tok < n && row0 + i_tok >= 0 && row0 + i_tok < a.n_tok;
-        const int      p     = okay && i_tok < n ? len - n + i_tok : -1;
-        const int      lo    = a.window > 0 ? max(0, p - a.window + 1) : 0;
-        const int64_t  head  = (int64_t) (hk * a.G + r % a.G) * D + hf * HD;
-        float          m = -INFINITY, l = 0.0f;
-        bool           ok = true;
-        uint32_t       nan_blocks = 0;  // of this thread's half
-        auto pair_xchg = [&](int phase, float v, float * other) -> bool {
-            xchg[((phase & 1) * 2 + hf) * kQtRows + row] = v;
-            __syncwarp();
-            if (lane == 0) {
-                ptx::mbar_arrive(&xbar[qq]);
-            }
-            if (!__all_sync(0xffffffffu, tc_wait(&xbar[qq], phase & 1, &abort_flag, a.err))) {
-                return false;
-            }
-            *other = xchg[((phase & 1) * 2 + (hf ^ 1)) * kQtRows + row];
-            return true;
-        };
-        float sc = 1.0f;  // of the scores, with log2 e: never 0, so that a masked score stays -inf
-        if (nblk > 0) {
-            // Q: a power of two takes the row's largest element into [1, 2), the scale's sign goes into it too
-            T1         q[HD];
-            const T1 * src = reinterpret_cast<const T1 *>(a.q) + (row0 + i_tok) * a.q_stride + head;
-            float      mx  = 0.0f, other = 0.0f;
-#pragma unroll
-            for (int e = 0; e < HD; e += 8) {
-                if constexpr (ALIGNED) {
-                    *reinterpret_cast<uint4 *>(q + e) = live ? __ldg(reinterpret_cast<const uint4 *>(src + e)) : make_uint4(0, 0, 0, 0);
-                } else {
-#pragma unroll
-                    for (int f = 0; f < 8; f++) {
-                        q[e + f] = live ? src[e + f] : io<T>::from_f(0.0f);
+                if (ok) {
+                    umma_commit(&v_empty[i % Lay::NV]);
+                    if (more) {
+                        umma_commit(&k_empty[(i + 1) % Lay::NK]);
                     }
                 }
             }
+        }
+    } else if ((warp >> 2) < tiles) {
+        // ---- softmax: warp w reads TMEM lanes 32 (w % 4).. of tile w / 4 ----
+        const int      t = warp >> 2, qq = warp & 3, row = qq * 32 + lane, r = r0 + t * kQtRows + row, i_tok = r / a.G;
+        const uint32_t lanes = (uint32_t) (qq * 32) << 16;
+        const uint32_t tS = tmem + lanes + (uint32_t) (t * 128), tO = tS + 256;
+        const bool     live = i_tok < n && row0 + i_tok >= 0 && row0 + i_tok < a.n_tok;
+        const int      p    = okay && i_tok < n ? len - n + i_tok : -1;
+        const int      lo   = a.window > 0 ? max(0, p - a.window + 1) : 0;
+        const int64_t  head = (int64_t) (hk * a.G + r % a.G) * D;
+        float          m = -INFINITY, l = 0.0f;
+        float          sc = 1.0f;  // of the scores, with log2 e: never 0, so that a masked score stays -inf
+        bool           ok = true;
+        uint32_t       nan_blocks = 0;  // 32 dimensions each
+        if (nblk > 0) {
+            // Q: a power of two takes the row's largest element into [1, 2), the scale's sign goes into it too
+            const T1 * src = reinterpret_cast<const T1 *>(a.q) + (row0 + i_tok) * a.q_stride + head;
+            float      mx  = 0.0f;
+            T1         q[32];  // 32 dimensions at a time, read again once the row's largest is known
+            auto       take = [&](int b) {
 #pragma unroll
-            for (int e = 0; e < HD; e++) {
-                mx = fmaxf(mx, fabsf(io<T>::to_f(q[e])));
+                for (int e = 0; e < 32; e += 8) {
+                    if constexpr (ALIGNED) {
+                        *reinterpret_cast<uint4 *>(q + e) =
+                            live ? __ldg(reinterpret_cast<const uint4 *>(src + 32 * b + e)) : make_uint4(0, 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int f = 0; f < 8; f++) {
+                            q[e + f] = live ? src[32 * b + e + f] : io<T>::from_f(0.0f);
+                        }
+                    }
+                }
+            };
+#pragma unroll 1
+            for (int b = 0; b < D / 32; b++) {
+                take(b);
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    mx = fmaxf(mx, fabsf(io<T>::to_f(q[e])));
+                }
             }
-            ok = pair_xchg(0, mx, &other);
-            mx = fmaxf(mx, other);
             int ex = (int) (__float_as_uint(mx) >> 23);
             ex     = mx == 0.0f || ex == 255 ? 127 : min(max(ex, 1), 253);
             float down = __uint_as_float((uint32_t) (254 - ex) << 23);
@@ -370,25 +396,22 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
                 sc   = fmaxf(fabsf(a.scale_log2) * __uint_as_float((uint32_t) ex << 23), 1.2e-38f);
                 down = copysignf(down, a.scale_log2);
             }
-            uint32_t v[HD / 2];
+            uint8_t * dst = sQ + t * Lay::QB + row * 128;
+#pragma unroll 1
+            for (int b = 0; b < D / 32; b++) {
+                take(b);
 #pragma unroll
-            for (int b = 0; b < HD / 32; b++) {
-#pragma unroll
-                for (int w = 0; w < 4; w++) {  // unpack4's order of the dimensions of a word
-                    const T1 * z = q + 32 * b + 4 * w;
-                    v[16 * b + 4 * w]     = u32_of(__floats2half2_rn(io<T>::to_f(z[0]) * down, io<T>::to_f(z[2]) * down));
-                    v[16 * b + 4 * w + 1] = u32_of(__floats2half2_rn(io<T>::to_f(z[16]) * down, io<T>::to_f(z[18]) * down));
-                    v[16 * b + 4 * w + 2] = u32_of(__floats2half2_rn(io<T>::to_f(z[1]) * down, io<T>::to_f(z[3]) * down));
-                    v[16 * b + 4 * w + 3] = u32_of(__floats2half2_rn(io<T>::to_f(z[17]) * down, io<T>::to_f(z[19]) * down));
+                for (int v = 0; v < 4; v++) {  // unit u: the dimensions of word u of the codes in unpack4's order
+                    const int      u = 4 * b + v;
+                    const T1 *     z = q + 4 * v;
+                    const uint32_t w0 = u32_of(__floats2half2_rn(io<T>::to_f(z[0]) * down, io<T>::to_f(z[2]) * down));
+                    const uint32_t w1 = u32_of(__floats2half2_rn(io<T>::to_f(z[16]) * down, io<T>::to_f(z[18]) * down));
+                    const uint32_t w2 = u32_of(__floats2half2_rn(io<T>::to_f(z[1]) * down, io<T>::to_f(z[3]) * down));
+                    const uint32_t w3 = u32_of(__floats2half2_rn(io<T>::to_f(z[17]) * down, io<T>::to_f(z[19]) * down));
+                    *reinterpret_cast<uint4 *>(dst + (u >> 3) * 16384 + (((u & 7) ^ (row & 7)) << 4)) = make_uint4(w0, w1, w2, w3);
                 }
             }
-            if constexpr (D == 128) {
-                tmem_st32(tQ + lanes + (uint32_t) (hf * 32), v);
-            } else {
-                tmem_st16(tQ + lanes + (uint32_t) (hf * 16), v);
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            }
-            tc_fence_before();
+            fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
                 ptx::mbar_arrive(q_full);
@@ -398,74 +421,70 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
         auto look_at_values = [&](int i) {
             if (bad_any[i % kQtRing][1]) {
                 const int key0 = (kb_lo + i) * kQtKeys;
-                for (int b = 0; b < HD / 32; b++) {
-                    for (int c = 0; c < kQtKeys; c++) {
-                        if ((bad_val[i % kQtRing][hf * (HD / 32) + b][c >> 5] >> (c & 31)) & 1u) {
-                            nan_blocks |= (uint32_t) (key0 + c >= lo && key0 + c <= p) << b;
-                        }
+#pragma unroll 1
+                for (int e = 0; e < (D / 32) * kQtKeys; e++) {
+                    const int b = e / kQtKeys, c = e % kQtKeys;
+                    if ((bad_val[i % kQtRing][b][c >> 5] >> (c & 31)) & 1u) {
+                        nan_blocks |= (uint32_t) (key0 + c >= lo && key0 + c <= p) << b;
                     }
                 }
             }
         };
-        int  pv_seen0 = 0, pv_seen1 = 0;
-        auto wait_pv  = [&](int k) -> bool {
-            const int bb = k & 1, ph = k >> 1;
-            int &     seen = bb ? pv_seen1 : pv_seen0;
-            if (seen > ph) {
-                return true;
-            }
-            if (!__all_sync(0xffffffffu, tc_wait(&pv_done[bb], ph & 1, &abort_flag, a.err))) {
-                return false;
-            }
-            seen = ph + 1;
-            tc_fence_after();
-            return true;
-        };
-        for (int i = 0; ok && i < nblk; i++) {
-            if (!__all_sync(0xffffffffu, tc_wait(&s_full[i & 1], (i >> 1) & 1, &abort_flag, a.err))) {
-                ok = false;
+        for (int i = 0; i < nblk; i++) {
+            ok = __all_sync(0xffffffffu, tc_wait(&s_full[t], i & 1, &abort_flag, a.err));
+            if (!ok) {
                 break;
             }
             tc_fence_after();
-            const uint32_t tS = tmem + lanes + (uint32_t) ((i & 1) * 128);
-            uint32_t       x[64];
-            tmem_ld32(tS + (uint32_t) (hf * 64), x);
-            tmem_ld32(tS + (uint32_t) (hf * 64 + 32), x + 32);
-            const int key0 = (kb_lo + i) * kQtKeys + hf * 64;
-            if (key0 + 63 > p || key0 < lo) {
+            if (i > 0) {
+                look_at_values(i - 1);
+            }
+            const int key0 = (kb_lo + i) * kQtKeys;
+            // bit c of see[w]: key key0 + 32 w + c is seen; looked at only where one is not
+            uint32_t   see[4];
+            const bool part = __any_sync(0xffffffffu, key0 + kQtKeys - 1 > p || key0 < lo || bad_any[i % kQtRing][0]);
+            if (part) {
 #pragma unroll
-                for (int c = 0; c < 64; c++) {
-                    if (key0 + c > p || key0 + c < lo) {
-                        x[c] = __float_as_uint(-INFINITY);
-                    }
+                for (int w = 0; w < 4; w++) {
+                    const int k = key0 + 32 * w;
+                    see[w]      = p < k ? 0u : p >= k + 31 ? ~0u : (2u << (p - k)) - 1u;
+                    see[w] &= lo <= k ? ~0u : lo > k + 31 ? 0u : ~0u << (lo - k);
+                    see[w] &= ~bad_key[i % kQtRing][w];
                 }
             }
-            if (bad_any[i % kQtRing][0]) {
+            uint32_t x[64];
+            auto     hide = [&](uint32_t b0, uint32_t b1) {
 #pragma unroll
                 for (int c = 0; c < 64; c++) {
-                    if ((bad_key[i % kQtRing][hf * 2 + (c >> 5)] >> (c & 31)) & 1u) {
-                        x[c] = __float_as_uint(-INFINITY);
+                    x[c] = ((c < 32 ? b0 : b1) >> (c & 31)) & 1u ? x[c] : 0xFF800000u;
+                }
+            };
+            auto top = [&]() {
+                float g[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    g[c] = fmaxf(__uint_as_float(x[c]), __uint_as_float(x[c + 4]));
+#pragma unroll
+                    for (int e = 8; e < 64; e += 8) {
+                        g[c] = fmaxf(g[c], fmaxf(__uint_as_float(x[c + e]), __uint_as_float(x[c + e + 4])));
                     }
                 }
+                return fmaxf(fmaxf(g[0], g[1]), fmaxf(g[2], g[3]));
+            };
+            // keys 0..63 for their maximum, keys 64..127 to stay; then keys 0..63 once more
+            tmem_ld64(tS, x);
+            if (part) {
+                hide(see[0], see[1]);
             }
-            float mt[8];
-#pragma unroll
-            for (int c = 0; c < 8; c++) {
-                mt[c] = fmaxf(fmaxf(fmaxf(__uint_as_float(x[c]), __uint_as_float(x[c + 8])),
-                                    fmaxf(__uint_as_float(x[c + 16]), __uint_as_float(x[c + 24]))),
-                              fmaxf(fmaxf(__uint_as_float(x[c + 32]), __uint_as_float(x[c + 40])),
-                                    fmaxf(__uint_as_float(x[c + 48]), __uint_as_float(x[c + 56]))));
+            float mx = top();
+            tmem_ld64(tS + 64, x);
+            if (part) {
+                hide(see[2], see[3]);
             }
-            const float mh = fmaxf(fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3])), fmaxf(fmaxf(mt[4], mt[5]), fmaxf(mt[6], mt[7])));
-            // the exchange also puts both threads' reads of this S buffer before either's P
-            float mo;
-            if (!pair_xchg(i + 1, mh, &mo)) {
-                ok = false;
-                break;
-            }
-            const float mb    = fmaxf(mh, mo) * sc;
+            mx               = fmaxf(mx, top());
+            const float mb   = mx * sc;
+            bool        resc = false;
             float       alpha = 1.0f;
-            bool        resc  = false;
             if (m == -INFINITY) {
                 m = mb;
             } else if (mb > m + kQtLag) {
@@ -475,66 +494,62 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
             }
             const float nm    = m == -INFINITY ? 0.0f : kQtLift - m;
             float       ps[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
-            uint32_t    ph[32];
+            // P of keys k.. into columns 64 + k / 2.., over the scores of keys 64..127
+            auto weigh = [&](int half) {
 #pragma unroll
-            for (int e = 0; e < 32; e++) {
-                const float e0 = ex2_fast(fmaf(__uint_as_float(x[2 * e]), sc, nm));
-                const float e1 = ex2_fast(fmaf(__uint_as_float(x[2 * e + 1]), sc, nm));
-                ps[e & 1] += e0;
-                ps[2 + (e & 1)] += e1;
-                ph[e] = u32_of(__floats2half2_rn(e0, e1));
-            }
-            if (i >= 2) {
-                if (!wait_pv(i - 2)) {
-                    ok = false;
-                    break;
+                for (int c = 0; c < 2; c++) {
+                    uint32_t ph[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float e0 = ex2_fast(fmaf(__uint_as_float(x[32 * c + 2 * e]), sc, nm));
+                        const float e1 = ex2_fast(fmaf(__uint_as_float(x[32 * c + 2 * e + 1]), sc, nm));
+                        ps[e & 1] += e0;
+                        ps[2 + (e & 1)] += e1;
+                        ph[e] = u32_of(__floats2half2_rn(e0, e1));
+                    }
+                    tmem_st16(tS + (uint32_t) (64 + 32 * half + 16 * c), ph);
                 }
-                look_at_values(i - 2);
+            };
+            weigh(1);
+            tmem_ld64(tS, x);
+            if (part) {
+                hide(see[0], see[1]);
             }
-            if (__any_sync(0xffffffffu, resc)) {
-                if (!wait_pv(i - 1)) {
-                    ok = false;
-                    break;
-                }
+            weigh(0);
+            if (__any_sync(0xffffffffu, resc)) {  // P.V(i - 1) is done: O is whole
 #pragma unroll 1
-                for (int c = 0; c < HD / 32; c++) {
-                    uint32_t       o[32];
-                    const uint32_t col = (uint32_t) (hf * HD + c * 32);
-                    tmem_ld32(tO + lanes + col, o);
+                for (int c = 0; c < D / 32; c++) {
+                    uint32_t o[32];
+                    tmem_ld32(tO + (uint32_t) (c * 32), o);
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
                         o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
                     }
-                    tmem_st32(tO + lanes + col, o);
+                    tmem_st32(tO + (uint32_t) (c * 32), o);
                 }
             }
             l = l * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
-            tmem_st32(tS + (uint32_t) (hf * 32), ph);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                ptx::mbar_arrive(&p_full[i & 1]);
+                ptx::mbar_arrive(&p_full[t]);
             }
         }
         if (ok && nblk > 0) {
-            ok = __all_sync(0xffffffffu, tc_wait(o_done, 0, &abort_flag, a.err));
+            ok = __all_sync(0xffffffffu, tc_wait(&o_done[t], 0, &abort_flag, a.err));
             tc_fence_after();
-            for (int i = max(0, nblk - 2); ok && i < nblk; i++) {
-                look_at_values(i);
+            if (ok) {
+                look_at_values(nblk - 1);
             }
         }
-        float lo_sum = 0.0f;
-        if (ok && nblk > 0) {
-            ok = pair_xchg(nblk + 1, l, &lo_sum);
-        }
-        const float lt  = ok ? l + lo_sum : 0.0f;
-        const float inv = lt != 0.0f ? 1.0f / lt : 0.0f;
+        const float inv = ok && l != 0.0f ? 1.0f / l : 0.0f;
         T1 *        y   = reinterpret_cast<T1 *>(a.o) + (row0 + i_tok) * a.o_stride + head;
 #pragma unroll 1
-        for (int c = 0; c < HD / 32; c++) {
+        for (int c = 0; c < D / 32; c++) {
             uint32_t o[32];
             if (nblk > 0 && ok) {
-                tmem_ld32(tO + lanes + (uint32_t) (hf * HD + c * 32), o);
+                tmem_ld32(tO + (uint32_t) (c * 32), o);
             } else {
 #pragma unroll
                 for (int e = 0; e < 32; e++) {
@@ -592,7 +607,7 @@ acb_status attn_q4_tc_launch(const AttnQ4Args & a, int type, int head_dim, cudaS
         return ACB_ERR_CUDA;
     }
     const int64_t rows = (int64_t) a.max_q * a.G;
-    kern<<<dim3((unsigned) ((rows + kQtRows - 1) / kQtRows), (unsigned) a.kv.nkv, (unsigned) a.kv.n_seq), kQtThreads, smem, st>>>(a);
+    kern<<<dim3((unsigned) ((rows + 2 * kQtRows - 1) / (2 * kQtRows)), (unsigned) a.kv.nkv, (unsigned) a.kv.n_seq), kQtThreads, smem, st>>>(a);
     return launch_status();
 }
 
