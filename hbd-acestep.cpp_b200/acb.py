@@ -224,9 +224,15 @@ def _check(fn: str, st: int):
         raise AcbError(fn, st)
 
 
+_dtype_ids = None
+
+
 def dtype_id(t) -> int:
-    import torch
-    return {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.int32: I32}[t.dtype]
+    global _dtype_ids
+    if _dtype_ids is None:
+        import torch
+        _dtype_ids = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.int32: I32}
+    return _dtype_ids[t.dtype]
 
 
 def rope_table(max_pos: int, head_dim: int, base: float):
@@ -387,31 +393,50 @@ ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_NTK, ROPE_SCALE_YARN = 0, 1, 2, 3
 _ROPE_LAYOUT = {"half": ROPE_HALF, "interleaved": ROPE_INTERLEAVED}
 
 
-def _run_on(name, t, stream, *args):
-    """The entry point `name` on the device that holds t, on its current stream unless one is given."""
-    import torch
-    dev = t.device
-    if dev.type != "cuda":
-        raise ValueError(f"{name}: tensors on the GPU are wanted, got {dev}")
-    fn = getattr(lib(), name)
-    if dev.index == torch.cuda.current_device():
-        st = fn(*args, _stream(stream))
+_fast = None
+
+
+def _torch_fast():
+    """(current raw stream of a device, current device) without the Stream object that torch.cuda.current_stream makes, which
+    takes longer than a small kernel; the public calls where a torch lacks the raw ones."""
+    global _fast
+    if _fast is None:
+        import torch
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+        cur = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+        _fast = (raw, cur)
+    return _fast
+
+
+def _run_on(name, dev, stream, *args):
+    """The entry point `name` on device number dev, on its current stream unless one is given."""
+    raw, cur = _fast or _torch_fast()
+    fn = getattr(_lib or lib(), name)
+    s = raw(dev) if stream is None else stream if isinstance(stream, int) else stream.cuda_stream
+    if dev == cur():
+        st = fn(*args, s)
     else:
+        import torch
         with torch.cuda.device(dev):
-            st = fn(*args, _stream(stream))
+            st = fn(*args, s)
     if st != 0:
         raise AcbError(name, st)
 
 
-def _want(name, t, dtype, dev, contiguous=True, numel=None):
+def _device(name, t):
+    """Number of the GPU that holds t."""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError(f"{name}: tensors on the GPU are wanted, got {t.device}")
+    return dev
+
+
+def _want(name, t, dtype, dev, numel=0, contiguous=True):
     """Refuses a tensor that the kernels would misread: another type, another device, gaps, too few elements."""
-    if t is None:
-        return
-    if t.dtype is not dtype or t.device != dev or (contiguous and not t.is_contiguous()) or \
-            (numel is not None and t.numel() < numel):
-        raise ValueError(f"{name}: a {'contiguous ' if contiguous else ''}{dtype} tensor on {dev}"
-                         f"{'' if numel is None else f' of {numel} elements or more'} is wanted, got {t.dtype} "
-                         f"{tuple(t.shape)} on {t.device}")
+    if t is not None and (t.dtype is not dtype or t.get_device() != dev or t.numel() < numel
+                          or (contiguous and not t.is_contiguous())):
+        raise ValueError(f"{name}: a {'contiguous ' if contiguous else ''}{dtype} tensor on GPU {dev} of {numel} elements or more "
+                         f"is wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def rope_table_scaled(max_pos, rope_dim, base, kind=ROPE_SCALE_NONE, factor=1.0, orig_max_pos=0, beta_fast=32.0,
@@ -428,17 +453,19 @@ def rope(x, pos, table, layout="half", inverse=False, out=None, err=None, stream
     """x [T, H, D] (any token and head strides) rotated by pos [T] int32 over the table's width; out may be x."""
     import torch
     T, H, D = x.shape
+    dev = _device("rope", x)
     if out is None:
         out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
-    if out.dtype is not x.dtype or out.shape != x.shape or x.stride(2) != 1 or out.stride(2) != 1:
-        raise ValueError("rope: x and out have one type and shape, their last dimension contiguous")
-    _want("rope: pos", pos, torch.int32, x.device, numel=T)
-    _want("rope: table", table, torch.float32, x.device)
-    if x.numel() == 0:
+    if out.dtype is not x.dtype or out.shape != x.shape or out.get_device() != dev or x.stride(2) != 1 or out.stride(2) != 1:
+        raise ValueError("rope: x and out have one type, shape and device, their last dimension contiguous")
+    _want("rope: pos", pos, torch.int32, dev, T)
+    _want("rope: table", table, torch.float32, dev)
+    if T == 0 or H == 0:
         return out
-    _run_on("acb_rope", x, stream, x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-            dtype_id(x), T, H, D, table.shape[1], _ROPE_LAYOUT[layout] | (ROPE_INVERSE if inverse else 0), pos.data_ptr(),
-            table.data_ptr(), table.shape[0], _ptr(err))
+    max_pos, width = table.shape
+    _run_on("acb_rope", dev, stream, x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+            dtype_id(x), T, H, D, width,
+            _ROPE_LAYOUT[layout] | (ROPE_INVERSE if inverse else 0), pos.data_ptr(), table.data_ptr(), max_pos, _ptr(err))
     return out
 
 
@@ -455,12 +482,12 @@ class KVCacheQ4:
     def __init__(self, k_codes, k_scales, v_codes, v_scales, page_table):
         import torch
         n_pages, n_kv, page, half = k_codes.shape
-        dev = k_codes.device
+        dev = _device("KVCacheQ4", k_codes)
         for n, t in (("k_codes", k_codes), ("v_codes", v_codes)):
             _want("KVCacheQ4: " + n, t, torch.uint8, dev)
         for n, t in (("k_scales", k_scales), ("v_scales", v_scales)):
             _want("KVCacheQ4: " + n, t, torch.float16, dev)
-        _want("KVCacheQ4: page_table", page_table, torch.int32, dev, contiguous=False)
+        _want("KVCacheQ4: page_table", page_table, torch.int32, dev, 0, False)
         if v_codes.shape != k_codes.shape or page_table.dim() != 2 or (page_table.shape[1] > 1 and page_table.stride(1) != 1) \
                 or any(s.shape != (n_pages, n_kv, page, half // 16) for s in (k_scales, v_scales)):
             raise ValueError("KVCacheQ4: codes [n_pages, n_kv_heads, page_size, D/2], scales [.., D/32], table [n_seq, max_pages]")
@@ -469,7 +496,7 @@ class KVCacheQ4:
         self.c = _KvQ4(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
                        page_table.data_ptr(), max(page_table.stride(0), page_table.shape[1]), n_pages, page, n_kv, 2 * half,
                        self.n_seq, page_table.shape[1])
-        self.device = dev
+        self.device, self.dev = k_codes.device, dev
         self.ref = C.addressof(self.c)
 
     @classmethod
@@ -485,22 +512,22 @@ class KVCacheQ4:
         """qkv [T, (n_heads + 2 n_kv_heads) D] (rows may be strided): norm and rotation of q and k, q returned [T, n_heads, D],
         k and v quantised into positions pos [T] of sequences seq [T] (int32; seq < 0: padding)."""
         import torch
-        T, D, dev = qkv.shape[0], self.head_dim, qkv.device
-        if dev != self.device or qkv.stride(1) != 1 or qkv.shape[1] < (n_heads + 2 * self.n_kv_heads) * D:
+        T, D, dev = qkv.shape[0], self.head_dim, self.dev
+        if qkv.get_device() != dev or qkv.stride(1) != 1 or qkv.shape[1] < (n_heads + 2 * self.n_kv_heads) * D:
             raise ValueError("KVCacheQ4.append: qkv [T, (n_heads + 2 n_kv_heads) * head_dim] on the cache's device is wanted")
-        _want("KVCacheQ4.append: seq", seq, torch.int32, dev, numel=T)
-        _want("KVCacheQ4.append: pos", pos, torch.int32, dev, numel=T)
+        _want("KVCacheQ4.append: seq", seq, torch.int32, dev, T)
+        _want("KVCacheQ4.append: pos", pos, torch.int32, dev, T)
         _want("KVCacheQ4.append: table", table, torch.float32, dev)
-        _want("KVCacheQ4.append: q_norm", q_norm, torch.float32, dev, numel=D)
-        _want("KVCacheQ4.append: k_norm", k_norm, torch.float32, dev, numel=D)
+        _want("KVCacheQ4.append: q_norm", q_norm, torch.float32, dev, D)
+        _want("KVCacheQ4.append: k_norm", k_norm, torch.float32, dev, D)
         if n_heads > 0 and q_out is None:
-            q_out = torch.empty((T, n_heads, D), dtype=q_dtype or qkv.dtype, device=dev)
-        if n_heads > 0 and (q_out.shape != (T, n_heads, D) or q_out.stride(2) != 1 or q_out.stride(1) != D or q_out.device != dev):
+            q_out = torch.empty((T, n_heads, D), dtype=q_dtype or qkv.dtype, device=self.device)
+        if n_heads > 0 and (q_out.shape != (T, n_heads, D) or q_out.stride(2) != 1 or q_out.stride(1) != D or q_out.get_device() != dev):
             raise ValueError("KVCacheQ4.append: q_out [T, n_heads, head_dim] with contiguous rows is wanted")
         if T == 0:
             return q_out
         mp, rd = table.shape if table is not None else (0, 0)
-        _run_on("acb_kv_q4_append", qkv, stream, self.ref, qkv.data_ptr(), dtype_id(qkv), max(qkv.stride(0), qkv.shape[1]), T,
+        _run_on("acb_kv_q4_append", dev, stream, self.ref, qkv.data_ptr(), dtype_id(qkv), max(qkv.stride(0), qkv.shape[1]), T,
                 n_heads, _ptr(q_norm), _ptr(k_norm), eps, _ptr(table), mp, rd, _ROPE_LAYOUT[layout], seq.data_ptr(),
                 pos.data_ptr(), _ptr(q_out), dtype_id(q_out if q_out is not None else qkv),
                 max(q_out.stride(0), n_heads * D) if q_out is not None else 0, _ptr(err))
@@ -510,19 +537,19 @@ class KVCacheQ4:
         """The cached keys and values at (seq, pos) as [T, n_kv_heads, D]: both when neither output is given."""
         import torch
         T, shape = seq.numel(), (seq.numel(), self.n_kv_heads, self.head_dim)
-        _want("KVCacheQ4.read: seq", seq, torch.int32, self.device)
-        _want("KVCacheQ4.read: pos", pos, torch.int32, self.device, numel=T)
+        _want("KVCacheQ4.read: seq", seq, torch.int32, self.dev)
+        _want("KVCacheQ4.read: pos", pos, torch.int32, self.dev, T)
         if k_out is None and v_out is None:
             k_out = torch.empty(shape, dtype=dtype or torch.float16, device=self.device)
             v_out = torch.empty_like(k_out)
         first = k_out if k_out is not None else v_out
         for t in (k_out, v_out):
             if t is not None and (t.shape != shape or t.dtype is not first.dtype or t.stride() != first.stride()
-                                  or t.stride(2) != 1 or t.stride(1) != self.head_dim or t.device != self.device):
+                                  or t.stride(2) != 1 or t.stride(1) != self.head_dim or t.get_device() != self.dev):
                 raise ValueError("KVCacheQ4.read: outputs [T, n_kv_heads, head_dim] of one type with contiguous rows are wanted")
         if T == 0:
             return k_out, v_out
-        _run_on("acb_kv_q4_read", seq, stream, self.ref, seq.data_ptr(), pos.data_ptr(), T, _ptr(k_out), _ptr(v_out),
+        _run_on("acb_kv_q4_read", self.dev, stream, self.ref, seq.data_ptr(), pos.data_ptr(), T, _ptr(k_out), _ptr(v_out),
                 dtype_id(first), max(first.stride(0), shape[1] * shape[2]), _ptr(err))
         return k_out, v_out
 
@@ -539,22 +566,24 @@ class KVCacheQ4:
         here when None)."""
         import torch
         T, H, D = q.shape
-        dev, c = q.device, self.c
+        dev, c = self.dev, self.c
         if max_kv_len is None:
             max_kv_len = c.max_pages * c.page_size
-        if dev != self.device or D != self.head_dim or q.stride(2) != 1 or q.stride(1) != D:
+        if q.get_device() != dev or D != self.head_dim or q.stride(2) != 1 or q.stride(1) != D:
             raise ValueError("KVCacheQ4.attention: q [T, n_heads, head_dim] with contiguous rows on the cache's device is wanted")
-        _want("KVCacheQ4.attention: kv_len", kv_len, torch.int32, dev, numel=self.n_seq)
-        _want("KVCacheQ4.attention: q_start", q_start, torch.int32, dev, numel=self.n_seq + 1)
+        _want("KVCacheQ4.attention: kv_len", kv_len, torch.int32, dev, self.n_seq)
+        _want("KVCacheQ4.attention: q_start", q_start, torch.int32, dev, self.n_seq + 1)
         if out is None:
-            out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
-        if out.dtype is not q.dtype or out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != D or out.device != dev:
+            out = torch.empty((T, H, D), dtype=q.dtype, device=self.device)
+        if out.dtype is not q.dtype or out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != D or out.get_device() != dev:
             raise ValueError("KVCacheQ4.attention: out of q's type and shape with contiguous rows is wanted")
         if T == 0:
             return out
         if work is None:
             work = self.attn_workspace(T, H, max_q_len, max_kv_len)
-        _run_on("acb_attn_kv_q4", q, stream, self.ref, q.data_ptr(), dtype_id(q), max(q.stride(0), H * D), T, H, _ptr(q_start),
+        elif work.get_device() != dev or not work.is_contiguous():
+            raise ValueError("KVCacheQ4.attention: the workspace is a contiguous tensor on the cache's device")
+        _run_on("acb_attn_kv_q4", dev, stream, self.ref, q.data_ptr(), dtype_id(q), max(q.stride(0), H * D), T, H, _ptr(q_start),
                 kv_len.data_ptr(), max_q_len, max_kv_len, window, D ** -0.5 if scale is None else scale, out.data_ptr(),
                 max(out.stride(0), H * D), _ptr(work), work.numel() * work.element_size() if work is not None else 0, _ptr(err))
         return out
@@ -574,14 +603,17 @@ def logits_rules(logits, hist=None, hist_len=None, prompt_len=None, rep=None, fr
     [n_masks, >= V/32] with mask_row int32 [R]. out may be logits."""
     import torch
     R, V = logits.shape
-    dev, i32, f32 = logits.device, torch.int32, torch.float32
+    dev, i32, f32 = _device("logits_rules", logits), torch.int32, torch.float32
     if out is None:
-        out = torch.empty((R, V), dtype=out_dtype or logits.dtype, device=dev)
-    if out.shape != logits.shape or out.device != dev or logits.stride(1) != 1 or out.stride(1) != 1:
+        out = torch.empty((R, V), dtype=out_dtype or logits.dtype, device=logits.device)
+    if out.shape != logits.shape or out.get_device() != dev or logits.stride(1) != 1 or out.stride(1) != 1:
         raise ValueError("logits_rules: logits and out [R, V] with contiguous rows are wanted")
-    for n, t, d in (("hist_len", hist_len, i32), ("prompt_len", prompt_len, i32), ("rep", rep, f32), ("freq", freq, f32),
-                    ("pres", pres, f32), ("mask_row", mask_row, i32)):
-        _want("logits_rules: " + n, t, d, dev, numel=R)
+    _want("logits_rules: hist_len", hist_len, i32, dev, R)
+    _want("logits_rules: prompt_len", prompt_len, i32, dev, R)
+    _want("logits_rules: rep", rep, f32, dev, R)
+    _want("logits_rules: freq", freq, f32, dev, R)
+    _want("logits_rules: pres", pres, f32, dev, R)
+    _want("logits_rules: mask_row", mask_row, i32, dev, R)
     if R == 0:
         return out
     r = _LogitRules(mask_row=_ptr(mask_row))
@@ -596,7 +628,7 @@ def logits_rules(logits, hist=None, hist_len=None, prompt_len=None, rep=None, fr
         r.rep, r.freq, r.pres = _ptr(rep), _ptr(freq), _ptr(pres)
     if bias_ids is not None and bias_ids.numel() > 0:
         _want("logits_rules: bias_ids", bias_ids, i32, dev)
-        _want("logits_rules: bias_val", bias_val, f32, dev, numel=bias_ids.numel())
+        _want("logits_rules: bias_val", bias_val, f32, dev, bias_ids.numel())
         r.bias_ids, r.bias_val, r.n_bias = bias_ids.data_ptr(), _ptr(bias_val), bias_ids.shape[-1]
         r.bias_stride = r.n_bias if bias_ids.dim() == 2 else 0
         if bias_ids.dim() == 2 and bias_ids.shape[0] < R:
@@ -604,7 +636,7 @@ def logits_rules(logits, hist=None, hist_len=None, prompt_len=None, rep=None, fr
     if mask is not None:
         _want("logits_rules: mask", mask, i32, dev)
         r.mask, r.n_masks, r.mask_stride = mask.data_ptr(), mask.shape[0], mask.shape[1]
-    _run_on("acb_logits_rules", logits, stream, logits.data_ptr(), dtype_id(logits), max(logits.stride(0), V), out.data_ptr(),
+    _run_on("acb_logits_rules", dev, stream, logits.data_ptr(), dtype_id(logits), max(logits.stride(0), V), out.data_ptr(),
             dtype_id(out), max(out.stride(0), V), R, V, C.addressof(r), _ptr(err))
     return out
 

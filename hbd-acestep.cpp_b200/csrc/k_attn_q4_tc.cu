@@ -81,15 +81,15 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
     __shared__ int      bad_any[kQtRing][2];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int hk = blockIdx.y, s = blockIdx.z;
+    const int hk = blockIdx.x, s = blockIdx.y;
     int64_t    row0;
     int        n, len;
     const bool okay = seq_bounds(a, s, &row0, &n, &len);
     if (!okay && a.err && threadIdx.x == 0) {
         atomicOr(a.err, ACB_DEVERR_LEN_RANGE);
     }
-    // the longest rows first: what is left for the end is short
-    const int r0 = (int) (gridDim.x - 1 - blockIdx.x) * 2 * kQtRows;
+    // the last rows of every sequence first, they see the most keys: what is left for the end is short
+    const int r0 = (int) (gridDim.z - 1 - blockIdx.z) * 2 * kQtRows;
     if (r0 >= n * a.G) {
         return;
     }
@@ -593,7 +593,7 @@ template <int T, int D> void (*tc_kernel(bool aligned))(const AttnQ4Args) {
 
 // From 64 rows on (half a tile) the tiles of 128 win over tiles of 16 that unpack every key again.
 bool attn_q4_tc_wanted(const AttnQ4Args & a, int type, int head_dim) {
-    return type != ACB_TYPE_F32 && head_dim <= 128 && (int64_t) a.max_q * a.G >= 64;
+    return type != ACB_TYPE_F32 && head_dim <= 128 && (int64_t) a.max_q * a.G >= 64 && (int64_t) a.max_q * a.G <= 65535 * 2 * kQtRows;
 }
 
 acb_status attn_q4_tc_launch(const AttnQ4Args & a, int type, int head_dim, cudaStream_t st) {
@@ -607,7 +607,7 @@ acb_status attn_q4_tc_launch(const AttnQ4Args & a, int type, int head_dim, cudaS
         return ACB_ERR_CUDA;
     }
     const int64_t rows = (int64_t) a.max_q * a.G;
-    kern<<<dim3((unsigned) ((rows + 2 * kQtRows - 1) / (2 * kQtRows)), (unsigned) a.kv.nkv, (unsigned) a.kv.n_seq), kQtThreads, smem, st>>>(a);
+    kern<<<dim3((unsigned) a.kv.nkv, (unsigned) a.kv.n_seq, (unsigned) ((rows + 2 * kQtRows - 1) / (2 * kQtRows))), kQtThreads, smem, st>>>(a);
     return launch_status();
 }
 
