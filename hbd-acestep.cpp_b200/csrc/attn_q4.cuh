@@ -18,6 +18,7 @@ struct AttnQ4Args {
     int64_t         o_stride;
     int *           err;
     KvQ4            kv;
+    bool            q_vec;    // rows of q are 16-byte aligned
     int             chunk;    // keys of a block, a multiple of 64
     int             n_split;  // chunks that the rows of one block can touch
     float *         part_o;   // [n_tok*Nh][n_split][D]: sums of P V
@@ -58,19 +59,25 @@ __device__ __forceinline__ void unpack4(uint32_t w, __half2 d, uint32_t * r) {
 
 template <int N> struct Words {
     uint32_t w[N];
-    __device__ __forceinline__ void load(const void * p) {
+    template <class Load> __device__ __forceinline__ void load_with(const void * p, Load ld) {
         if constexpr (N % 4 == 0) {
 #pragma unroll
             for (int i = 0; i < N / 4; i++) {
-                const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+                const uint4 u = ld(reinterpret_cast<const uint4 *>(p) + i);
                 w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
             }
         } else if constexpr (N == 2) {
-            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p));
+            const uint2 u = ld(reinterpret_cast<const uint2 *>(p));
             w[0] = u.x, w[1] = u.y;
         } else {
-            w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
+            w[0] = ld(reinterpret_cast<const uint32_t *>(p));
         }
+    }
+    __device__ __forceinline__ void load(const void * p) {
+        load_with(p, [](auto * q) { return __ldg(q); });
+    }
+    __device__ __forceinline__ void load_shared(const void * p) {
+        load_with(p, [](auto * q) { return *q; });
     }
 };
 

@@ -5,8 +5,9 @@
 //   S[key][row] = K[key][:] . Q[row][:]        A = keys as they are unpacked, B = queries
 //   O[dim][row] += V^T[dim][key] P[key][row]   A = values, two keys to a register, B = P
 // Every cached element is an f16 number (kv_q4.cuh), so A is exact; Q is scaled by a power of two per row into f16's range
-// (an f32 query is the sum of two f16 numbers), P goes in as the sum of two f16 numbers: both products then carry 21 bits and
-// more, the sums are f32.
+// (an f32 query is the sum of two f16 numbers), and for an f32 output P goes in as the sum of two f16 numbers, so that both
+// products carry 21 bits and more; a 16-bit output takes P as one f16 number, whose half step of 2^-11 per weight averages
+// out under the output's own. The sums are f32.
 //
 // Few rows: the bytes of the cache bound it (1.125 bytes per key and dimension against 4 flops a row), so a warp takes 16 keys
 // at a time straight from global memory into the registers that the tensor cores read -- the k index of a product may be any
@@ -42,33 +43,33 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return r;
 }
 
-// One thread's share of 16 keys and values. With lane = 4 g + t it holds, of keys g and g + 8, the D/8 bytes from
-// t D/8 on, and of values 2t, 2t+1, 2t+8, 2t+9 the D/16 bytes from g D/16 on: what the A operands of both products take.
-template <int D> struct Tile16 {
-    static constexpr int KW = D / 32, VW = D / 64, KS = D == 256 ? 2 : 1;
-    Words<KW>            k[2];
-    Words<VW>            v[4];
-    uint16_t             ks[2][KS], vs[4];
+// 16 keys and values of a warp in shared memory. With lane = 4 g + t a thread takes, of keys g and g + 8, the D/8 bytes from
+// t D/8 on, and of values 2t, 2t+1, 2t+8, 2t+9 the D/16 bytes from g D/16 on: what the A operands of both products take. The
+// pitches spread the lanes of every such access over all banks.
+template <int D> struct Stage16 {
+    static constexpr int KP = D == 256 ? 144 : D / 2, VP = D / 2 + 16;
+    static constexpr int V = 16 * KP, KS = V + 16 * VP, VS = KS + D, BYTES = VS + D;
+    static constexpr int KW = D / 32, VW = D / 64;
 
-    __device__ __forceinline__ void load(const KvQ4 & kv, int64_t row, int g, int t) {
-        const uint8_t *  kc = kv.kc + row * (D / 2) + t * (D / 8);
-        const uint16_t * ksp = kv.ks + row * (D / 32) + t * D / 128;
+    // the copies of one warp, 16 bytes a lane: the rows of a tile are consecutive in the pool
+    static __device__ __forceinline__ void fill(uint32_t st, const KvQ4 & kv, uint32_t row, int lane) {
+        const uint8_t * kc = kv.kc + (uint64_t) row * (D / 2) + lane * 16;
+        const uint8_t * vc = kv.vc + (uint64_t) row * (D / 2) + lane * 16;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            k[i].load(kc + (g + 8 * i) * (D / 2));
-#pragma unroll
-            for (int b = 0; b < KS; b++) {
-                ks[i][b] = __ldg(ksp + (g + 8 * i) * (D / 32) + b);
-            }
+        for (int i = 0; i < D / 64; i++) {
+            const int c = lane + 32 * i, j = c / (D / 32), x = c % (D / 32) * 16;
+            copy16(st + j * KP + x, kc + 512 * i);
+            copy16(st + V + j * VP + x, vc + 512 * i);
         }
-        const uint8_t *  vc = kv.vc + row * (D / 2) + g * (D / 16);
-        const uint16_t * vsp = kv.vs + row * (D / 32) + g * D / 256;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int j = 2 * t + (i & 1) + (i & 2) * 4;
-            v[i].load(vc + j * (D / 2));
-            vs[i] = __ldg(vsp + j * (D / 32));
+        if (lane < D / 8) {
+            const bool      val = lane >= D / 16;
+            const uint8_t * sc  = reinterpret_cast<const uint8_t *>(val ? kv.vs : kv.ks) + (uint64_t) row * (D / 16) +
+                                 (val ? lane - D / 16 : lane) * 16;
+            copy16(st + KS + lane * 16, sc);
         }
+    }
+    static __device__ __forceinline__ void copy16(uint32_t dst, const void * src) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     }
 };
 
@@ -78,8 +79,13 @@ __device__ __forceinline__ int dim_of(int b, int hi) {
 }
 
 // One block: up to 8 NT rows (r = new token * G + query head of the group) of one sequence and kv head, over one chunk of keys.
+// blocks of an SM that the registers are held to
+template <int T, int D, int NT> constexpr int kSplitBlocks = D == 256 || NT == 2 ? 2 : T == ACB_TYPE_F32 ? 4 : 5;
+
+template <int D> constexpr int kStages = D == 256 ? 3 : 4;
+
 template <int T, int D, int NT>
-__global__ void __launch_bounds__(32 * kSplitWarps) attn_q4_split_kernel(const AttnQ4Args a) {
+__global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn_q4_split_kernel(const AttnQ4Args a) {
     constexpr int  KT  = D / 16;  // k steps of Q.K
     constexpr int  MT  = D / 16;  // 16-dimension tiles of the output
     constexpr int  QP  = T == ACB_TYPE_F32 ? 2 : 1;
@@ -87,7 +93,8 @@ __global__ void __launch_bounds__(32 * kSplitWarps) attn_q4_split_kernel(const A
     using T1           = typename io<T>::t;
     __shared__ int   s_hi[R], s_lo[R];
     __shared__ float s_m[kSplitWarps][R], s_l[kSplitWarps][R];
-    __shared__ float s_o[R][D];
+    extern __shared__ __align__(16) uint8_t smem[];  // the warps' rings, then the sums of the warps' parts
+    float (*s_o)[D + 4] = reinterpret_cast<float (*)[D + 4]>(smem);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int rt = blockIdx.x / a.n_split, split = blockIdx.x - rt * a.n_split, hk = blockIdx.y, s = blockIdx.z;
     ptx::grid_dep_launch();
@@ -138,15 +145,41 @@ __global__ void __launch_bounds__(32 * kSplitWarps) attn_q4_split_kernel(const A
         const T1 * q = reinterpret_cast<const T1 *>(a.q) + (row0 + i) * a.q_stride + (int64_t) (hk * a.G + r % a.G) * D;
         float      f[KT][4], mx = 0.0f;
 #pragma unroll
-        for (int w = 0; w < D / 32; w++) {
-            const int b = t * (D / 8) + 4 * w;
+        for (int w = 0; w < D / 64; w++) {
+            // 8 bytes of codes are two runs of 8 dimensions: their low halves and their high halves
+            const int b = t * (D / 8) + 8 * w;
+            float     z[2][8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                // order of unpack4: bytes 0 and 2 low, 0 and 2 high, 1 and 3 low, 1 and 3 high
-                const int   d = dim_of(b + (e >> 2) + 2 * (e & 1), (e >> 1) & 1);
-                const float v = i < n ? io<T>::to_f(q[d]) : 0.0f;
-                f[2 * w + (e >> 2)][e & 3] = v;
-                mx                         = fmaxf(mx, fabsf(v));
+            for (int h = 0; h < 2; h++) {
+                const T1 * src = q + dim_of(b, h);
+                if (i >= n) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        z[h][e] = 0.0f;
+                    }
+                } else if (a.q_vec) {
+#pragma unroll
+                    for (int v = 0; v < 8 / vec16<T>::N; v++) {
+                        vec16<T> in;
+                        in.load_nc(src + v * vec16<T>::N);
+#pragma unroll
+                        for (int e = 0; e < vec16<T>::N; e++) {
+                            z[h][v * vec16<T>::N + e] = in.get(e);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        z[h][e] = io<T>::to_f(src[e]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                // order of unpack4 in a word: bytes 0 and 2 low, 0 and 2 high, 1 and 3 low, 1 and 3 high
+                const float v                         = z[(e >> 1) & 1][4 * (e >> 3) + ((e >> 2) & 1) + 2 * (e & 1)];
+                f[4 * w + 2 * (e >> 3) + ((e >> 2) & 1)][e & 3] = v;
+                mx                                    = fmaxf(mx, fabsf(v));
             }
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
@@ -188,28 +221,17 @@ __global__ void __launch_bounds__(32 * kSplitWarps) attn_q4_split_kernel(const A
 
     const int hi_min = p0;  // the first row's last key: keys up to it are seen by all rows that exist
     const int tb0    = (j0 & ~15) + 16 * warp;
-    Tile16<D> tile;
-    int       pg = tb0 < j1 ? a.kv.page_of(s, tb0) : -1;
-    if (tb0 < j1 && pg >= 0) {
-        tile.load(a.kv, a.kv.row(pg, hk, tb0), g, t);
-    }
-    for (int tb = tb0; tb < j1; tb += 16 * kSplitWarps) {
-        const Tile16<D> cur = tile;
-        const int       cpg = pg;
-        const int       nb  = tb + 16 * kSplitWarps;
-        if (nb < j1) {
-            pg = a.kv.page_of(s, nb);
-            if (pg >= 0) {
-                tile.load(a.kv, a.kv.row(pg, hk, nb), g, t);
-            }
-        }
-        if (cpg < 0) {
-            if (lane == 0 && a.err) {
-                atomicOr(a.err, ACB_DEVERR_PAGE_RANGE);
-            }
-            continue;
-        }
+    using St = Stage16<D>;
+    constexpr int  STEP = 16 * kSplitWarps, NST = kStages<D>;
+    const uint32_t ring = ptx::smem_u32(smem) + warp * (NST * St::BYTES);
+    const uint8_t * mine = smem + warp * (NST * St::BYTES);
+
+    auto take = [&](const int tb, const uint8_t * st) {
         // scores
+        Words<St::KW>    k[2];
+        const uint16_t * ksc = reinterpret_cast<const uint16_t *>(st + St::KS) + g * (D / 32) + t * D / 128;
+        k[0].load_shared(st + g * St::KP + t * (D / 8));
+        k[1].load_shared(st + (g + 8) * St::KP + t * (D / 8));
         float S[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -218,8 +240,8 @@ __global__ void __launch_bounds__(32 * kSplitWarps) attn_q4_split_kernel(const A
 #pragma unroll
         for (int w = 0; w < D / 32; w++) {
             uint32_t x[4], y[4];
-            unpack4(cur.k[0].w[w], __half2half2(__ushort_as_half(cur.ks[0][w * Tile16<D>::KS / (D / 32)])), x);
-            unpack4(cur.k[1].w[w], __half2half2(__ushort_as_half(cur.ks[1][w * Tile16<D>::KS / (D / 32)])), y);
+            unpack4(k[0].w[w], __half2half2(__ushort_as_half(ksc[w / 4])), x);
+            unpack4(k[1].w[w], __half2half2(__ushort_as_half(ksc[8 * (D / 32) + w / 4])), y);
             const uint32_t a0[4] = { x[0], y[0], x[1], y[1] }, a1[4] = { x[2], y[2], x[3], y[3] };
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
@@ -278,13 +300,23 @@ __global__ void __launch_bounds__(32 * kSplitWarps) attn_q4_split_kernel(const A
                 l[nt][0] += x;
                 l[nt][1] += y;
                 const __half2 hi = __floats2half2_rn(x, y);
-                const float2  b  = __half22float2(hi);
                 ph[nt][h]        = transpose8x8(u32_of(hi));
-                pl[nt][h]        = transpose8x8(u32_of(__floats2half2_rn(x - b.x, y - b.y)));
+                if (QP == 2) {
+                    const float2 b = __half22float2(hi);
+                    pl[nt][h]      = transpose8x8(u32_of(__floats2half2_rn(x - b.x, y - b.y)));
+                }
             }
         }
-        uint32_t vs01 = (uint32_t) cur.vs[0] | ((uint32_t) cur.vs[1] << 16);
-        uint32_t vs23 = (uint32_t) cur.vs[2] | ((uint32_t) cur.vs[3] << 16);
+        Words<St::VW> v[4];
+        uint16_t      vs[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int j = 2 * t + (i & 1) + (i & 2) * 4;
+            v[i].load_shared(st + St::V + j * St::VP + g * (D / 16));
+            vs[i] = reinterpret_cast<const uint16_t *>(st + St::VS)[j * (D / 32) + g * D / 256];
+        }
+        uint32_t vs01 = (uint32_t) vs[0] | ((uint32_t) vs[1] << 16);
+        uint32_t vs23 = (uint32_t) vs[2] | ((uint32_t) vs[3] << 16);
         if (edge) {
             // a scale that is no number must not reach the rows that do not see its key (0 * NaN): it is taken out here and
             // put on the rows that do see it one by one
@@ -292,15 +324,14 @@ __global__ void __launch_bounds__(32 * kSplitWarps) attn_q4_split_kernel(const A
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int j = tb + 2 * t + (i & 1) + (i & 2) * 4;
-                if ((cur.vs[i] & 0x7C00u) == 0x7C00u) {
+                if ((vs[i] & 0x7C00u) == 0x7C00u) {
                     (i < 2 ? vs01 : vs23) &= (i & 1) ? 0x0000FFFFu : 0xFFFF0000u;
                     any |= j >= j0 && j < j1;
                 }
             }
             if (__any_sync(0xffffffffu, any)) {
-                const int64_t row = a.kv.row(cpg, hk, tb);
                 for (int j = max(tb, j0); j < min(tb + 16, j1); j++) {
-                    const uint16_t d = __ldg(a.kv.vs + (row + j - tb) * (D / 32) + g * D / 256);
+                    const uint16_t d = reinterpret_cast<const uint16_t *>(st + St::VS)[(j - tb) * (D / 32) + g * D / 256];
                     if ((d & 0x7C00u) == 0x7C00u) {
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
@@ -325,23 +356,63 @@ __global__ void __launch_bounds__(32 * kSplitWarps) attn_q4_split_kernel(const A
             for (int half = 0; half < 2; half++) {
                 const uint32_t sel = half ? 0x7632u : 0x5410u;
                 uint32_t       x[4], y[4];  // bytes 2 half, 2 half + 1: low, high, low, high nibble of two keys each
-                unpack4(__byte_perm(cur.v[0].w[w], cur.v[1].w[w], sel), half2_of(vs01), x);
-                unpack4(__byte_perm(cur.v[2].w[w], cur.v[3].w[w], sel), half2_of(vs23), y);
+                unpack4(__byte_perm(v[0].w[w], v[1].w[w], sel), half2_of(vs01), x);
+                unpack4(__byte_perm(v[2].w[w], v[3].w[w], sel), half2_of(vs23), y);
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
                     const int      mt   = w * 4 + half * 2 + b;
                     const uint32_t f[4] = { x[2 * b], x[2 * b + 1], y[2 * b], y[2 * b + 1] };
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        mma16816(o[mt][nt], f, pl[nt][0], pl[nt][1]);
+                        if (QP == 2) {
+                            mma16816(o[mt][nt], f, pl[nt][0], pl[nt][1]);
+                        }
                         mma16816(o[mt][nt], f, ph[nt][0], ph[nt][1]);
                     }
                 }
             }
         }
+    };
+    // NST - 1 tiles under way in this warp's ring (registers for a tile ahead instead cost a third of the warps: 186 us where
+    // this takes REPLACE), the page of the next one looked up a turn before its copies
+    int      pg   = tb0 < j1 ? a.kv.page_of(s, tb0) : 0;
+    uint32_t lost = 0;  // bit of a stage: its page is not in the pool
+    auto     fetch = [&](int tb, int slot) {
+        if (tb < j1) {
+            lost = (lost & ~(1u << slot)) | (uint32_t) (pg < 0) << slot;
+            if (pg >= 0) {
+                St::fill(ring + slot * St::BYTES, a.kv, a.kv.row(pg, hk, tb), lane);
+            }
+            if (tb + STEP < j1) {
+                pg = a.kv.page_of(s, tb + STEP);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < NST - 1; i++) {
+        fetch(tb0 + i * STEP, i);
     }
+    int slot = 0;
+    for (int tb = tb0; tb < j1; tb += STEP) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(NST - 2) : "memory");
+        __syncwarp();  // all lanes' copies of this stage are there, and all are done with the one that is filled next
+        const int free = slot == 0 ? NST - 1 : slot - 1;
+        fetch(tb + (NST - 1) * STEP, free);
+        if ((lost >> slot) & 1u) {
+            if (lane == 0 && a.err) {
+                atomicOr(a.err, ACB_DEVERR_PAGE_RANGE);
+            }
+        } else {
+            take(tb, mine + slot * St::BYTES);
+        }
+        slot = slot == NST - 1 ? 0 : slot + 1;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 
-    // the four warps' parts, joined in the warps' order
+    // The four warps' parts, joined in the warps' order: each leaves its sums in shared memory as its registers hold them (value
+    // v of lane x at 32 v + x), and then adds up a quarter of them.
+    __syncthreads();  // the rings are done with
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -356,31 +427,32 @@ __global__ void __launch_bounds__(32 * kSplitWarps) attn_q4_split_kernel(const A
             }
         }
     }
-    __syncthreads();
-    for (int w = 0; w < kSplitWarps; w++) {
-        if (warp == w) {
+    constexpr int NV   = MT * NT * 4;  // values of a lane
+    float *       part = reinterpret_cast<float *>(smem);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int   r = nt * 8 + 2 * t + h;
-                    const float M = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-                    const float f = m[nt][h] == -INFINITY ? 0.0f : ex2(m[nt][h] - M);
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-#pragma unroll
-                        for (int q = 0; q < 2; q++) {
-                            float *     p = &s_o[r][dim_of(g * (D / 16) + mt, q)];
-                            const float v = o[mt][nt][h + 2 * q];
-                            const float x = m[nt][h] == -INFINITY && v == v ? 0.0f : v * f;
-                            *p            = w == 0 ? x : *p + x;
-                        }
-                    }
-                }
-            }
-        }
-        __syncthreads();
+    for (int v = 0; v < NV; v++) {
+        part[(warp * NV + v) * 32 + lane] = o[v / (4 * NT)][v / 4 % NT][v % 4];
     }
+    __syncthreads();
+    float sum[NV / kSplitWarps];
+#pragma unroll
+    for (int k = 0; k < NV / kSplitWarps; k++) {
+        const int   v = warp * (NV / kSplitWarps) + k, r = (v / 4 % NT) * 8 + 2 * t + (v & 1);
+        const float M = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+        sum[k]        = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kSplitWarps; w++) {
+            const float x = part[(w * NV + v) * 32 + lane], mw = s_m[w][r];
+            sum[k] += mw == -INFINITY && x == x ? 0.0f : x * ex2(mw - M);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NV / kSplitWarps; k++) {
+        const int v = warp * (NV / kSplitWarps) + k, r = (v / 4 % NT) * 8 + 2 * t + (v & 1);
+        s_o[r][dim_of(g * (D / 16) + v / (4 * NT), (v >> 1) & 1)] = sum[k];
+    }
+    __syncthreads();
     for (int e = threadIdx.x; e < R * D / 4; e += 32 * kSplitWarps) {
         const int rr = e / (D / 4), d = (e % (D / 4)) * 4;
         const int r = r0 + rr, i = r / a.G;
@@ -508,7 +580,11 @@ Plan make_plan(const acb_kv_q4 * kv, int n_heads, int max_q, int max_kv, int win
     p.tiles              = (int) ((rows + 8 * p.nt - 1) / (8 * p.nt));
     const int64_t keys   = window > 0 && (int64_t) window + max_q < max_kv ? (int64_t) window + max_q : max_kv;
     const int64_t tasks  = (int64_t) p.tiles * kv->n_kv_heads * kv->n_seq;
-    const int64_t splits = (int64_t) num_sms() * 12 / tasks;
+    // One part per block of a full GPU where that cuts each sequence's keys at least four times; otherwise the parts of
+    // sequences of very different lengths are to even out, so six times as many. (96 sequences of 200-8192 keys: 198 us at
+    // two parts each, 177 at six; two of 131071: 124 us at 111 parts, REPLACE at 46.)
+    const int64_t slots  = (int64_t) num_sms() * 5;
+    const int64_t splits = slots / tasks >= 4 ? slots / tasks : 6 * slots / tasks;
     const int64_t cuts   = (max_kv + kMinChunk - 1) / kMinChunk;
     if (splits <= 1 || cuts <= 1) {
         p.n_split = 1;
@@ -588,6 +664,7 @@ extern "C" acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int t
     a.o          = o;
     a.o_stride   = o_stride;
     a.err        = err_flag;
+    a.q_vec      = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_stride * type_size(type) % 16 == 0;
     a.chunk      = p.chunk;
     a.n_split    = p.n_split;
     a.part_ml    = reinterpret_cast<float2 *>(work);
@@ -599,7 +676,14 @@ extern "C" acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int t
     const Kernel kern = type == ACB_TYPE_F32   ? split_kernel<ACB_TYPE_F32>(D, p.nt)
                         : type == ACB_TYPE_F16 ? split_kernel<ACB_TYPE_F16>(D, p.nt)
                                                : split_kernel<ACB_TYPE_BF16>(D, p.nt);
-    kern<<<dim3((unsigned) (p.tiles * p.n_split), (unsigned) kv->n_kv_heads, (unsigned) kv->n_seq), 32 * kSplitWarps, 0,
+    const size_t smem = (size_t) kSplitWarps * (D == 64 ? kStages<64> * Stage16<64>::BYTES : D == 128 ? kStages<128> * Stage16<128>::BYTES
+                                                                                                : kStages<256> * Stage16<256>::BYTES);
+    const cudaError_t ea = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
+    if (ea != cudaSuccess) {
+        set_last_cuda_error(ea);
+        return ACB_ERR_CUDA;
+    }
+    kern<<<dim3((unsigned) (p.tiles * p.n_split), (unsigned) kv->n_kv_heads, (unsigned) kv->n_seq), 32 * kSplitWarps, smem,
            (cudaStream_t) stream>>>(a);
     const acb_status st = launch_status();
     if (st != ACB_OK || p.n_split == 1) {

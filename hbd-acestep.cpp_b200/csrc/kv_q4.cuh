@@ -23,9 +23,9 @@ struct KvQ4 {
         const int pg = __ldg(table + (int64_t) s * table_stride + (p >> shift));
         return (unsigned) pg < (unsigned) n_pages ? pg : -1;
     }
-    // row number of (page, kv head, slot) in units of one head's token row
-    __device__ __forceinline__ int64_t row(int pg, int h, int p) const {
-        return (((int64_t) pg * nkv + h) << shift) + (p & (page - 1));
+    // row number of (page, kv head, slot) in units of one head's token row: below 2^32 (kv_q4_check)
+    __device__ __forceinline__ uint32_t row(int pg, int h, int p) const {
+        return (((uint32_t) pg * (uint32_t) nkv + (uint32_t) h) << shift) + (uint32_t) (p & (page - 1));
     }
 };
 
@@ -42,7 +42,8 @@ inline acb_status kv_q4_check(const acb_kv_q4 * kv, KvQ4 * out) {
     }
     if ((kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256) || kv->page_size < 16 ||
         kv->page_size > 4096 || (kv->page_size & (kv->page_size - 1)) != 0 ||
-        (int64_t) kv->max_pages * kv->page_size > (1 << 30)) {
+        (int64_t) kv->max_pages * kv->page_size > (1 << 30) ||
+        (int64_t) kv->n_pages * kv->n_kv_heads > (int64_t) UINT32_MAX / kv->page_size) {
         return ACB_ERR_UNSUPPORTED;
     }
     int shift = 0;
