@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
     constexpr int  R   = 8 * NT;
     using T1           = typename io<T>::t;
     __shared__ int   s_hi[R], s_lo[R];
-    __shared__ float s_m[kSplitWarps][R], s_l[kSplitWarps][R];
+    __shared__ float s_m[kSplitWarps][R], s_l[kSplitWarps][R], s_top[R];
     extern __shared__ __align__(16) uint8_t smem[];  // the warps' rings, then the sums of the warps' parts
     float (*s_o)[D + 4] = reinterpret_cast<float (*)[D + 4]>(smem);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -187,7 +187,8 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
         // 2^e with mx / 2^e in [1, 2): exponent field of mx, kept where 2^-e is a number
         int e = (int) (__float_as_uint(mx) >> 23);
         e     = mx == 0.0f || e == 255 ? 127 : min(max(e, 1), 253);
-        const float down = __uint_as_float((uint32_t) (254 - e) << 23);
+        // the scale's sign goes into the query: what is left is above 0, so that a masked score stays -inf
+        const float down = a.scale_log2 == 0.0f ? 0.0f : copysignf(__uint_as_float((uint32_t) (254 - e) << 23), a.scale_log2);
         const float up   = __uint_as_float((uint32_t) e << 23);
 #pragma unroll
         for (int k = 0; k < KT; k++) {
@@ -202,16 +203,18 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
                 }
             }
         }
-        const float fs = a.scale_log2 * up;
+        const float fs = fmaxf(fabsf(a.scale_log2) * up, 1.2e-38f);
         // scores come out with the row in the column index: rows 2t and 2t + 1, held by the lanes with g = 2t, 2t + 1
         sc[nt][0] = __shfl_sync(0xffffffffu, fs, 8 * t);
         sc[nt][1] = __shfl_sync(0xffffffffu, fs, 8 * t + 4);
     }
 
-    float o[MT][NT][4], m[NT][2], l[NT][2];
+    // weights are 2^(score sc + lift); a score above thr makes lift follow (-inf: no key seen yet)
+    float o[MT][NT][4], lift[NT][2], thr[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        m[nt][0] = m[nt][1] = -INFINITY;
+        lift[nt][0] = lift[nt][1] = 0.0f;
+        thr[nt][0] = thr[nt][1] = -INFINITY;
         l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
@@ -254,37 +257,44 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
         }
         // a tile that some row does not see whole: -inf for what it does not see, and the values that no row sees left out
         const bool edge = tb < full0 || tb < j0 || tb + 15 > hi_min || tb + 15 >= j1;
-        bool       grow = false;
+        if (edge) {
+            asm volatile("" ::: "memory");  // a branch: these instructions are for few tiles
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
+            for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                S[nt][e] *= sc[nt][e & 1];
-                if (edge) {
+                for (int e = 0; e < 4; e++) {
                     const int j = tb + g + 8 * (e >> 1), r = nt * 8 + 2 * t + (e & 1);
                     if (j < max(j0, s_lo[r]) || j > min(j1 - 1, s_hi[r])) {
                         S[nt][e] = -INFINITY;
                     }
                 }
-                grow = grow || S[nt][e] > m[nt][e & 1] + kLag;
             }
+        }
+        bool grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            grow = grow || fmaxf(S[nt][0], S[nt][2]) > thr[nt][0] || fmaxf(S[nt][1], S[nt][3]) > thr[nt][1];
         }
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    float x = fmaxf(m[nt][h], fmaxf(S[nt][h], S[nt][h + 2]));
+                    float x = fmaxf(S[nt][h], S[nt][h + 2]);
                     x       = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x       = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x       = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    const float f = x == -INFINITY ? 1.0f : ex2(m[nt][h] - x);
-                    m[nt][h]      = x;
-                    l[nt][h] *= f;
+                    if (x > thr[nt][h]) {
+                        const float to = kLift - x * sc[nt][h];
+                        const float f  = thr[nt][h] == -INFINITY ? 1.0f : ex2(to - lift[nt][h]);
+                        lift[nt][h]    = to;
+                        thr[nt][h]     = x + kLag / sc[nt][h];
+                        l[nt][h] *= f;
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        o[mt][nt][h] *= f;
-                        o[mt][nt][h + 2] *= f;
+                        for (int mt = 0; mt < MT; mt++) {
+                            o[mt][nt][h] *= f;
+                            o[mt][nt][h + 2] *= f;
+                        }
                     }
                 }
             }
@@ -292,11 +302,10 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
         uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const float m0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0] - kLift;
-            const float m1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1] - kLift;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const float x = ex2(S[nt][2 * h] - m0), y = ex2(S[nt][2 * h + 1] - m1);
+                const float x = ex2(fmaf(S[nt][2 * h], sc[nt][0], lift[nt][0]));
+                const float y = ex2(fmaf(S[nt][2 * h + 1], sc[nt][1], lift[nt][1]));
                 l[nt][0] += x;
                 l[nt][1] += y;
                 const __half2 hi = __floats2half2_rn(x, y);
@@ -318,6 +327,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
         uint32_t vs01 = (uint32_t) vs[0] | ((uint32_t) vs[1] << 16);
         uint32_t vs23 = (uint32_t) vs[2] | ((uint32_t) vs[3] << 16);
         if (edge) {
+            asm volatile("" ::: "memory");
             // a scale that is no number must not reach the rows that do not see its key (0 * NaN): it is taken out here and
             // put on the rows that do see it one by one
             uint32_t any = 0;
@@ -373,8 +383,8 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
             }
         }
     };
-    // NST - 1 tiles under way in this warp's ring (registers for a tile ahead instead cost a third of the warps: 186 us where
-    // this takes REPLACE), the page of the next one looked up a turn before its copies
+    // NST - 1 tiles under way in this warp's ring (registers for a tile ahead instead cost two fifths of the warps: 186 us for
+    // the 96 sequences where this takes 159), the page of the next one looked up a turn before its copies
     int      pg   = tb0 < j1 ? a.kv.page_of(s, tb0) : 0;
     uint32_t lost = 0;  // bit of a stage: its page is not in the pool
     auto     fetch = [&](int tb, int slot) {
@@ -422,7 +432,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
             x += __shfl_xor_sync(0xffffffffu, x, 8);
             x += __shfl_xor_sync(0xffffffffu, x, 16);
             if (g == 0) {
-                s_m[warp][nt * 8 + 2 * t + h] = m[nt][h];
+                s_m[warp][nt * 8 + 2 * t + h] = thr[nt][h] == -INFINITY ? -INFINITY : -lift[nt][h];
                 s_l[warp][nt * 8 + 2 * t + h] = x;
             }
         }
@@ -434,16 +444,29 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
         part[(warp * NV + v) * 32 + lane] = o[v / (4 * NT)][v / 4 % NT][v % 4];
     }
     __syncthreads();
+    // what each warp's sums are taken by, and the rows' sums of weights
+    if (threadIdx.x < R) {
+        const int   r = threadIdx.x;
+        const float M = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+        float       L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kSplitWarps; w++) {
+            const float f = s_m[w][r] == -INFINITY ? 0.0f : ex2(s_m[w][r] - M);
+            L += s_l[w][r] * f;
+            s_m[w][r] = f;
+        }
+        s_top[r] = M;
+        s_l[0][r] = L;
+    }
+    __syncthreads();
     float sum[NV / kSplitWarps];
 #pragma unroll
     for (int k = 0; k < NV / kSplitWarps; k++) {
-        const int   v = warp * (NV / kSplitWarps) + k, r = (v / 4 % NT) * 8 + 2 * t + (v & 1);
-        const float M = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-        sum[k]        = 0.0f;
+        const int v = warp * (NV / kSplitWarps) + k, r = (v / 4 % NT) * 8 + 2 * t + (v & 1);
+        sum[k]      = 0.0f;
 #pragma unroll
         for (int w = 0; w < kSplitWarps; w++) {
-            const float x = part[(w * NV + v) * 32 + lane], mw = s_m[w][r];
-            sum[k] += mw == -INFINITY && x == x ? 0.0f : x * ex2(mw - M);
+            sum[k] += part[(w * NV + v) * 32 + lane] * s_m[w][r];
         }
     }
     __syncthreads();
@@ -461,12 +484,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
         if (p < 0 || c < c0 || c > c1) {  // no key of this row in this chunk
             continue;
         }
-        const float M  = fmaxf(fmaxf(s_m[0][rr], s_m[1][rr]), fmaxf(s_m[2][rr], s_m[3][rr]));
-        float       L  = 0.0f;
-        for (int w = 0; w < kSplitWarps; w++) {
-            const float x = s_l[w][rr];
-            L += s_m[w][rr] == -INFINITY && x == x ? 0.0f : x * ex2(s_m[w][rr] - M);
-        }
+        const float   L   = s_l[0][rr];
         const float4  v   = *reinterpret_cast<const float4 *>(&s_o[rr][d]);
         const int64_t tok = row0 + i;
         const int     h   = hk * a.G + r % a.G;
@@ -481,7 +499,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
             const int64_t slot = (tok * a.Nh + h) * a.n_split + c % a.n_split;
             *reinterpret_cast<float4 *>(a.part_o + slot * D + d) = v;
             if (d == 0) {
-                a.part_ml[slot] = make_float2(M, L);
+                a.part_ml[slot] = make_float2(s_top[rr], L);
             }
         }
     }
@@ -564,9 +582,10 @@ template <int T> Kernel join_kernel(int D) {
 }
 
 // How the keys are cut. Rows of one kv head in tiles of 8 or 16 (8 for heads of 256, whose sums fill the registers); chunks
-// of a multiple of 64 keys (four warps of 16), as many as it takes to give every SM a few blocks to choose from, but
-// none below 256 keys: a chunk's part costs its rows 4 (D + 2) bytes twice, against 1.125 D bytes a key.
-constexpr int kMinChunk = 256;
+// of a multiple of 64 keys (four warps of 16), as many as fill the GPU, but none below 256 keys: a chunk's part costs its rows
+// 4 (D + 2) bytes twice, against 1.125 D bytes a key. A call of so few rows and heads that 256 keys a block would leave
+// most SMs idle goes down to 128 (one sequence of 1536 keys, 8 kv heads: 10.1 us at 256, 8.9 at 128; 24 sequences of up to
+// 4000 with drafts: 15.2 at 256, 19.5 at 128).
 
 struct Plan {
     int     nt, tiles, chunk, n_split;
@@ -581,11 +600,12 @@ Plan make_plan(const acb_kv_q4 * kv, int n_heads, int max_q, int max_kv, int win
     const int64_t keys   = window > 0 && (int64_t) window + max_q < max_kv ? (int64_t) window + max_q : max_kv;
     const int64_t tasks  = (int64_t) p.tiles * kv->n_kv_heads * kv->n_seq;
     // One part per block of a full GPU where that cuts each sequence's keys at least four times; otherwise the parts of
-    // sequences of very different lengths are to even out, so six times as many. (96 sequences of 200-8192 keys: 198 us at
-    // two parts each, 177 at six; two of 131071: 124 us at 111 parts, REPLACE at 46.)
+    // sequences of very different lengths are to even out, so six times as many. (96 sequences of 200-8192 keys: 185 us at
+    // three times, 159 at six; two of 131071: 124 us at 111 parts each, 99 at 46.)
     const int64_t slots  = (int64_t) num_sms() * 5;
     const int64_t splits = slots / tasks >= 4 ? slots / tasks : 6 * slots / tasks;
-    const int64_t cuts   = (max_kv + kMinChunk - 1) / kMinChunk;
+    const int64_t least  = tasks * 4 <= num_sms() ? 128 : 256;
+    const int64_t cuts   = (max_kv + least - 1) / least;
     if (splits <= 1 || cuts <= 1) {
         p.n_split = 1;
         p.most    = 1;
@@ -593,7 +613,7 @@ Plan make_plan(const acb_kv_q4 * kv, int n_heads, int max_q, int max_kv, int win
         return p;
     }
     int64_t chunk = (keys + splits - 1) / splits;
-    chunk         = ((chunk < kMinChunk ? kMinChunk : chunk) + 63) / 64 * 64;
+    chunk         = ((chunk < least ? least : chunk) + 63) / 64 * 64;
     p.chunk       = (int) chunk;
     // a window's keys can begin anywhere in a chunk
     p.n_split = (int) ((keys + chunk - 1) / chunk) + (keys < max_kv ? 1 : 0);

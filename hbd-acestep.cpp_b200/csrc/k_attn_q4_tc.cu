@@ -5,7 +5,8 @@
 //   0..3, 4..7  softmax of tile 0 and of tile 1, a thread a row (a TMEM lane): 64 scores at a time: the maximum of
 //               the first half, that of the second, the second's exponentials, the first half again for its own; P takes the
 //               second half's columns as f16. (Two threads a row with both halves of one
-//               tile in registers, and the exchange that takes, held the tensor cores at 20%: 462 us where this takes REPLACE.)
+//               tile in registers, and the exchange that takes, held the tensor cores at 20%: 462 us where this takes 310; all
+//               eight warps on one tile at a time 376 us.)
 //   8..11       K: a thread a key; the 8 dimensions of a word of codes make one 16-byte unit in the order that unpack4 gives
 //               them, and Q is written in the same order (a product does not depend on the order of its k index);
 //   12..15      V^T: a thread 8 keys by 16 dimensions: the words of two keys are merged by halves, so that unpack4 gives pairs of
