@@ -439,6 +439,16 @@ def _want(name, t, dtype, dev, numel=0, contiguous=True):
                          f"is wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
+def _row_stride(name, t, width):
+    """Elements between the rows of t [T, ...], which hold width elements each (a single row may say anything)."""
+    if t.shape[0] <= 1:
+        return width
+    s = t.stride(0)
+    if s < width:
+        raise ValueError(f"{name}: rows that overlap (stride {s} for {width} elements)")
+    return s
+
+
 def rope_table_scaled(max_pos, rope_dim, base, kind=ROPE_SCALE_NONE, factor=1.0, orig_max_pos=0, beta_fast=32.0,
                       beta_slow=1.0):
     """Host table [max_pos, rope_dim] for a context longer than the trained one (angles in double)."""
@@ -456,14 +466,15 @@ def rope(x, pos, table, layout="half", inverse=False, out=None, err=None, stream
     dev = _device("rope", x)
     if out is None:
         out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
-    if out.dtype is not x.dtype or out.shape != x.shape or out.get_device() != dev or x.stride(2) != 1 or out.stride(2) != 1:
+    sx, so = x.stride(), out.stride()
+    if out.dtype is not x.dtype or out.shape != x.shape or out.get_device() != dev or sx[2] != 1 or so[2] != 1:
         raise ValueError("rope: x and out have one type, shape and device, their last dimension contiguous")
     _want("rope: pos", pos, torch.int32, dev, T)
     _want("rope: table", table, torch.float32, dev)
     if T == 0 or H == 0:
         return out
     max_pos, width = table.shape
-    _run_on("acb_rope", dev, stream, x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+    _run_on("acb_rope", dev, stream, x.data_ptr(), sx[0], sx[1], out.data_ptr(), so[0], so[1],
             dtype_id(x), T, H, D, width,
             _ROPE_LAYOUT[layout] | (ROPE_INVERSE if inverse else 0), pos.data_ptr(), table.data_ptr(), max_pos, _ptr(err))
     return out
@@ -488,13 +499,15 @@ class KVCacheQ4:
         for n, t in (("k_scales", k_scales), ("v_scales", v_scales)):
             _want("KVCacheQ4: " + n, t, torch.float16, dev)
         _want("KVCacheQ4: page_table", page_table, torch.int32, dev, 0, False)
+        if page_table.dim() == 2:
+            table_stride = _row_stride("KVCacheQ4: page_table", page_table, page_table.shape[1])
         if v_codes.shape != k_codes.shape or page_table.dim() != 2 or (page_table.shape[1] > 1 and page_table.stride(1) != 1) \
                 or any(s.shape != (n_pages, n_kv, page, half // 16) for s in (k_scales, v_scales)):
             raise ValueError("KVCacheQ4: codes [n_pages, n_kv_heads, page_size, D/2], scales [.., D/32], table [n_seq, max_pages]")
         self.tensors = (k_codes, k_scales, v_codes, v_scales, page_table)
         self.n_kv_heads, self.head_dim, self.n_seq = n_kv, 2 * half, page_table.shape[0]
         self.c = _KvQ4(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
-                       page_table.data_ptr(), max(page_table.stride(0), page_table.shape[1]), n_pages, page, n_kv, 2 * half,
+                       page_table.data_ptr(), table_stride, n_pages, page, n_kv, 2 * half,
                        self.n_seq, page_table.shape[1])
         self.device, self.dev = k_codes.device, dev
         self.ref = C.addressof(self.c)
@@ -522,15 +535,16 @@ class KVCacheQ4:
         _want("KVCacheQ4.append: k_norm", k_norm, torch.float32, dev, D)
         if n_heads > 0 and q_out is None:
             q_out = torch.empty((T, n_heads, D), dtype=q_dtype or qkv.dtype, device=self.device)
-        if n_heads > 0 and (q_out.shape != (T, n_heads, D) or q_out.stride(2) != 1 or q_out.stride(1) != D or q_out.get_device() != dev):
+        if n_heads > 0 and (q_out.shape != (T, n_heads, D) or q_out.stride()[1:] != (D, 1) or q_out.get_device() != dev):
             raise ValueError("KVCacheQ4.append: q_out [T, n_heads, head_dim] with contiguous rows is wanted")
         if T == 0:
             return q_out
         mp, rd = table.shape if table is not None else (0, 0)
-        _run_on("acb_kv_q4_append", dev, stream, self.ref, qkv.data_ptr(), dtype_id(qkv), max(qkv.stride(0), qkv.shape[1]), T,
+        _run_on("acb_kv_q4_append", dev, stream, self.ref, qkv.data_ptr(), dtype_id(qkv),
+                _row_stride("KVCacheQ4.append: qkv", qkv, qkv.shape[1]), T,
                 n_heads, _ptr(q_norm), _ptr(k_norm), eps, _ptr(table), mp, rd, _ROPE_LAYOUT[layout], seq.data_ptr(),
                 pos.data_ptr(), _ptr(q_out), dtype_id(q_out if q_out is not None else qkv),
-                max(q_out.stride(0), n_heads * D) if q_out is not None else 0, _ptr(err))
+                _row_stride("KVCacheQ4.append: q_out", q_out, n_heads * D) if q_out is not None else 0, _ptr(err))
         return q_out
 
     def read(self, seq, pos, k_out=None, v_out=None, dtype=None, err=None, stream=None):
@@ -545,12 +559,12 @@ class KVCacheQ4:
         first = k_out if k_out is not None else v_out
         for t in (k_out, v_out):
             if t is not None and (t.shape != shape or t.dtype is not first.dtype or t.stride() != first.stride()
-                                  or t.stride(2) != 1 or t.stride(1) != self.head_dim or t.get_device() != self.dev):
+                                  or t.stride()[1:] != (self.head_dim, 1) or t.get_device() != self.dev):
                 raise ValueError("KVCacheQ4.read: outputs [T, n_kv_heads, head_dim] of one type with contiguous rows are wanted")
         if T == 0:
             return k_out, v_out
         _run_on("acb_kv_q4_read", self.dev, stream, self.ref, seq.data_ptr(), pos.data_ptr(), T, _ptr(k_out), _ptr(v_out),
-                dtype_id(first), max(first.stride(0), shape[1] * shape[2]), _ptr(err))
+                dtype_id(first), _row_stride("KVCacheQ4.read", first, shape[1] * shape[2]), _ptr(err))
         return k_out, v_out
 
     def attn_workspace(self, n_tok, n_heads, max_q_len, max_kv_len):
@@ -569,13 +583,13 @@ class KVCacheQ4:
         dev, c = self.dev, self.c
         if max_kv_len is None:
             max_kv_len = c.max_pages * c.page_size
-        if q.get_device() != dev or D != self.head_dim or q.stride(2) != 1 or q.stride(1) != D:
+        if q.get_device() != dev or D != self.head_dim or q.stride()[1:] != (D, 1):
             raise ValueError("KVCacheQ4.attention: q [T, n_heads, head_dim] with contiguous rows on the cache's device is wanted")
         _want("KVCacheQ4.attention: kv_len", kv_len, torch.int32, dev, self.n_seq)
         _want("KVCacheQ4.attention: q_start", q_start, torch.int32, dev, self.n_seq + 1)
         if out is None:
             out = torch.empty((T, H, D), dtype=q.dtype, device=self.device)
-        if out.dtype is not q.dtype or out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != D or out.get_device() != dev:
+        if out.dtype is not q.dtype or out.shape != q.shape or out.stride()[1:] != (D, 1) or out.get_device() != dev:
             raise ValueError("KVCacheQ4.attention: out of q's type and shape with contiguous rows is wanted")
         if T == 0:
             return out
@@ -583,9 +597,10 @@ class KVCacheQ4:
             work = self.attn_workspace(T, H, max_q_len, max_kv_len)
         elif work.get_device() != dev or not work.is_contiguous():
             raise ValueError("KVCacheQ4.attention: the workspace is a contiguous tensor on the cache's device")
-        _run_on("acb_attn_kv_q4", dev, stream, self.ref, q.data_ptr(), dtype_id(q), max(q.stride(0), H * D), T, H, _ptr(q_start),
+        _run_on("acb_attn_kv_q4", dev, stream, self.ref, q.data_ptr(), dtype_id(q), _row_stride("KVCacheQ4.attention: q", q, H * D),
+                T, H, _ptr(q_start),
                 kv_len.data_ptr(), max_q_len, max_kv_len, window, D ** -0.5 if scale is None else scale, out.data_ptr(),
-                max(out.stride(0), H * D), _ptr(work), work.numel() * work.element_size() if work is not None else 0, _ptr(err))
+                _row_stride("KVCacheQ4.attention: out", out, H * D), _ptr(work), work.numel() * work.element_size() if work is not None else 0, _ptr(err))
         return out
 
 
@@ -636,8 +651,8 @@ def logits_rules(logits, hist=None, hist_len=None, prompt_len=None, rep=None, fr
     if mask is not None:
         _want("logits_rules: mask", mask, i32, dev)
         r.mask, r.n_masks, r.mask_stride = mask.data_ptr(), mask.shape[0], mask.shape[1]
-    _run_on("acb_logits_rules", dev, stream, logits.data_ptr(), dtype_id(logits), max(logits.stride(0), V), out.data_ptr(),
-            dtype_id(out), max(out.stride(0), V), R, V, C.addressof(r), _ptr(err))
+    _run_on("acb_logits_rules", dev, stream, logits.data_ptr(), dtype_id(logits), _row_stride("logits_rules: logits", logits, V),
+            out.data_ptr(), dtype_id(out), _row_stride("logits_rules: out", out, V), R, V, C.addressof(r), _ptr(err))
     return out
 
 

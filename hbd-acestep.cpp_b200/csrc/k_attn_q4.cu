@@ -13,6 +13,8 @@
 // at a time straight from global memory into the registers that the tensor cores read -- the k index of a product may be any
 // order of the dimensions as long as both operands agree, so a thread's share of a key is 16 consecutive bytes -- with the next
 // 16 keys already in flight. Long sequences are cut into chunks of keys, one block each; a second kernel joins the parts.
+#include <math.h>
+
 #include "attn_q4.cuh"
 #include "ptx.cuh"
 
@@ -637,7 +639,15 @@ extern "C" size_t acb_attn_kv_q4_work_bytes(const acb_kv_q4 * kv, int64_t n_tok,
         max_kv_len <= 0) {
         return 0;
     }
-    return plan_bytes(make_plan(kv, n_heads, max_q_len, max_kv_len, 0).most, kv, n_tok, n_heads);
+    // enough for every call of at most these sizes: fewer rows a sequence are cut into more chunks, so each power of two of
+    // them is asked, with the most rows that it stands for
+    size_t most = 0;
+    for (int64_t q = 1; q <= max_q_len; q *= 2) {
+        const int64_t rows  = (2 * q - 1) * kv->n_seq;
+        const size_t  bytes = plan_bytes(make_plan(kv, n_heads, (int) q, max_kv_len, 0).most, kv, rows < n_tok ? rows : n_tok, n_heads);
+        most                = bytes > most ? bytes : most;
+    }
+    return most;
 }
 
 extern "C" acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int type, int64_t q_stride, int64_t n_tok,
@@ -650,7 +660,7 @@ extern "C" acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int t
         return rc;
     }
     if (!q || !o || !kv_len || n_tok < 0 || n_heads <= 0 || n_heads % kv->n_kv_heads != 0 || max_q_len <= 0 ||
-        max_kv_len < 0 || window < 0 || !(scale == scale) || q_stride < (int64_t) n_heads * kv->head_dim ||
+        max_kv_len < 0 || window < 0 || !isfinite(scale) || q_stride < (int64_t) n_heads * kv->head_dim ||
         o_stride < (int64_t) n_heads * kv->head_dim || (!q_start && (n_tok != kv->n_seq || max_q_len != 1)) ||
         (work && !kv_q4_aligned(work))) {
         return ACB_ERR_INVALID_ARG;

@@ -185,6 +185,29 @@ def test_nan_of_a_seen_key_shows(cuda, n):
     assert bool(o.isnan().all())
 
 
+@pytest.mark.parametrize("kind,D", [("f32", 128), ("bf16", 128), ("f16", 64), ("bf16", 256)])
+@pytest.mark.parametrize("n", [3, 100])
+def test_nan_values_reach_only_the_rows_that_see_them(cuda, kind, D, n):
+    """A value scale that is NaN: the block's dimensions of the rows that see its key, and nothing else."""
+    import torch
+    rng = np.random.default_rng(21)
+    cache = _cache(rng, 1, 256, 16, 1, D)
+    q = torch.randn(n, 2, D).to(S.torch_type(kind)).cuda()
+    start, ln = torch.tensor([0, n], dtype=torch.int32).cuda(), torch.tensor([200], dtype=torch.int32).cuda()
+    ref = cache.attention(q, ln, start, n)
+    j, blk = 198, 1  # the last row but one is the first to see it
+    t = cache.tensors[4][0]
+    cache.tensors[3][int(t[j // 16]), 0, j % 16, blk] = float("nan")
+    o = cache.attention(q, ln, start, n)
+    hit = torch.zeros_like(o, dtype=torch.bool)
+    hit[n - 2:, :, blk * 32:blk * 32 + 32] = True
+    assert bool(o[hit].isnan().all())
+    assert torch.equal(o[~hit], ref[~hit])
+    w = cache.attention(q, ln, start, n, window=1)  # only row n - 2 sees key 198
+    hit[n - 1:] = False
+    assert bool(w[hit].isnan().all()) and bool(w[~hit].isfinite().all())
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n", [1, 140])
 def test_peaked_and_flat_scores(cuda, kind, n):
@@ -315,3 +338,47 @@ def test_two_streams_at_once(cuda):
                 got[i] = cache.attention(q[i], ln, work=work[i])
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+@pytest.mark.parametrize("n", [1, 5, 130])
+def test_pages_behind_4_gb(cuda, n):
+    """The same keys on the first pages of a pool and on its last, codes past 32-bit offsets: the same output."""
+    import torch
+    n_pages, page, Nkv, D = 8300, 4096, 2, 128
+    table = torch.tensor([[0, 1], [n_pages - 1, n_pages - 2]], dtype=torch.int32).cuda()
+    cache = acb.KVCacheQ4.empty(n_pages, page, Nkv, D, table)
+    kc, ks, vc, vs, _ = cache.tensors
+    for t in (kc, vc):
+        t[:2] = torch.randint(0, 256, (2, Nkv, page, D // 2), dtype=torch.uint8).cuda()
+        t[[n_pages - 1, n_pages - 2]] = t[:2].clone()
+    for t in (ks, vs):
+        t[:2] = (0.02 + 0.1 * torch.rand(2, Nkv, page, D // 32)).bfloat16().half().cuda()
+        t[[n_pages - 1, n_pages - 2]] = t[:2].clone()
+    q = torch.randn(n, 4, D).bfloat16().cuda()
+    o = cache.attention(torch.cat([q, q]), torch.tensor([5000, 5000], dtype=torch.int32).cuda(),
+                        torch.tensor([0, n, 2 * n], dtype=torch.int32).cuda(), n)
+    assert torch.equal(o[:n], o[n:]) and bool((o != 0).any())
+
+
+def test_wrappers_refuse_what_would_be_misread(cuda):
+    import torch
+    rng = np.random.default_rng(22)
+    cache = _cache(rng, 2, 64, 16, 1, 64)
+    q = torch.randn(2, 2, 64).cuda()
+    ln = torch.tensor([10, 20], dtype=torch.int32).cuda()
+    cache.attention(q, ln)
+    for bad in (lambda: cache.attention(q[:1].expand(2, 2, 64), ln), lambda: cache.attention(q, ln.long()),
+                lambda: cache.attention(q, ln.cpu()), lambda: cache.attention(q, ln[:1]), lambda: cache.attention(q[..., ::2], ln),
+                lambda: cache.attention(q, ln, out=q.half()), lambda: cache.attention(q.cpu(), ln),
+                lambda: acb.KVCacheQ4(*cache.tensors[:4], cache.tensors[4][:1].expand(2, 4)),
+                lambda: acb.KVCacheQ4(*cache.tensors[:4], cache.tensors[4].long()),
+                lambda: acb.KVCacheQ4(cache.tensors[0], cache.tensors[1][:, :, :, :1].contiguous(), *cache.tensors[2:]),
+                lambda: cache.append(torch.randn(1, 256).cuda().expand(2, 256), 2, ln, ln),
+                lambda: cache.append(torch.randn(2, 255).cuda(), 2, ln, ln),
+                lambda: cache.read(ln, ln, k_out=torch.zeros(2, 1, 64).cuda(), v_out=torch.zeros(2, 1, 64).half().cuda())):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(acb.AcbError):
+        cache.attention(torch.randn(2, 2, 64).cuda(), ln, max_kv_len=65)
+    with pytest.raises(acb.AcbError):
+        cache.attention(torch.randn(3, 2, 64).cuda(), ln)  # three rows, two sequences and no q_start

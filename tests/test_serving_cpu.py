@@ -76,7 +76,7 @@ def test_read_refusals(kw, status):
 @pytest.mark.parametrize("kw,status", [(dict(q=None), 1), (dict(o=None), 1), (dict(kv_len=None), 1), (dict(n_tok=-1), 1),
                                        (dict(n_heads=0), 1), (dict(n_heads=3, q_stride=256), 1), (dict(max_q=0), 1),
                                        (dict(max_q=2), 1), (dict(n_tok=4), 1), (dict(max_kv=-1), 1), (dict(window=-1), 1),
-                                       (dict(scale=math.nan), 1), (dict(q_stride=255), 1), (dict(o_stride=255), 1),
+                                       (dict(scale=math.nan), 1), (dict(scale=math.inf), 1), (dict(q_stride=255), 1), (dict(o_stride=255), 1),
                                        (dict(max_kv=65), 4), (dict(type=acb.Q8_0), 2)])
 def test_attention_refusals(kw, status):
     assert attn(cache(), **kw) == status
@@ -176,3 +176,18 @@ def test_wrappers_refuse_cpu_tensors():
         acb.logits_rules(torch.zeros(2, 8), mask=torch.zeros(2, 1, dtype=torch.int32))
     with pytest.raises(ValueError):
         acb.logits_rules(torch.zeros(2, 8), rep=torch.ones(2))
+
+
+def test_workspaces_cover_every_smaller_call():
+    """acb_attn_kv_q4_work_bytes: what it gives for sizes holds for all smaller rows and lengths, and a workspace is only asked
+    where there is something to split."""
+    f = acb.lib().acb_attn_kv_q4_work_bytes
+    for n_seq, heads in ((1, 4), (3, 14), (64, 32)):
+        kv = cache(n_seq=n_seq, n_kv_heads=2, head_dim=128, max_pages=1 << 12, table_stride=1 << 12, n_pages=1 << 13)
+        ref = C.addressof(kv)
+        full = f(ref, n_seq * 40, heads, 40, 60000)
+        for q in (1, 2, 3, 7, 39):
+            for n in (1, 500, 59999):
+                assert f(ref, n_seq * q, heads, q, n) <= full
+        assert f(ref, n_seq, heads, 1, 100) == 0
+        assert f(ref, 0, heads, 1, 60000) == 0 and f(ref, n_seq, heads, 0, 60000) == 0 and f(ref, n_seq, 3, 1, 60000) == 0
