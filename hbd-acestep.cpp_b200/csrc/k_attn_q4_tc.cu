@@ -27,8 +27,8 @@ namespace {
 constexpr int   kQtRows    = 128;  // of a tile
 constexpr int   kQtKeys    = 128;
 constexpr int   kQtSoft    = 8;   // softmax warps
-constexpr int   kQtUnpack  = 4;   // warps that unpack K, and as many for V
-constexpr int   kQtMma     = kQtSoft + 2 * kQtUnpack;
+constexpr int   kQtUnpack  = 4;   // unpacking warps
+constexpr int   kQtMma     = kQtSoft + kQtUnpack;  // 13 warps: up to 16 leave every thread 128 registers
 constexpr int   kQtThreads = 32 * (kQtMma + 1);
 constexpr float kQtLag     = 8.0f;  // the reference maximum moves when exceeded by more than 2^kQtLag
 constexpr float kQtLift    = 6.0f;  // P is held times 2^kQtLift: at most 2^14
@@ -40,22 +40,24 @@ template <int D> struct QtLayout {
     // TMEM columns: S/P of the tiles at 0 and 128, O at 256 and 384
 };
 
-// 64 columns of this warp's lanes
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t * r) {
+// 32 columns of this warp's lanes on their way into r, which must not be looked at before tmem_arrived(r)
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t * r) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
-        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%1"
+        "7,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
-          "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
-          "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
-          "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
-          "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-        : "r"(taddr)
-        : "memory");
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_arrived(uint32_t * r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+        asm volatile("" : "+r"(r[i]));  // no use of it moves in front of the wait
+    }
 }
 
 template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThreads, 1) attn_q4_tc_kernel(const AttnQ4Args a) {
@@ -139,155 +141,133 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
     const uint32_t tmem = *tmem_slot;
 
     if (warp >= kQtSoft && warp < kQtMma) {
-        // ---- unpacking: four warps K, four warps V ----
-        const int tid = threadIdx.x & (32 * kQtUnpack - 1);  // 0..127 of each
-        if (warp < kQtSoft + kQtUnpack) {
-            // K: this thread's key of a block
-            Words<D / 8>  kw;
+        // ---- unpacking: four warps, K and then V of each block ----
+        const int  tid = threadIdx.x & (32 * kQtUnpack - 1);  // 0..127: this thread's key of K
+        // V: 8 keys from 8 kg on (of one page: pages hold 16 or more), 16 dimensions: the 8 bytes from 8 wq on; the lanes of a
+        // store phase differ in kg
+        const int  kg = (tid & 7) | ((tid >> 6) << 3), wq = (tid >> 3) & 7;
+        const bool on = D == 128 || wq < 4;  // heads of 64 have 4 such runs
+        int        kpg = nblk > 0 ? a.kv.page_of(s, min(kb_lo * kQtKeys + tid, p1)) : 0;
+        int        vpg = nblk > 0 ? a.kv.page_of(s, min(kb_lo * kQtKeys + 8 * kg, p1)) : 0;
+        for (int i = 0; i < nblk; i++) {
+            const int  key0 = (kb_lo + i) * kQtKeys, note = i % kQtRing, next = (i + 2) % kQtRing;
+            const int  sk = i % Lay::NK, sv = i % Lay::NV;
+            const bool gone = key0 + tid > p1, k_bad = kpg < 0;
+            // everything from memory is under way before the first wait
+            const int64_t krow = k_bad ? 0 : a.kv.row(kpg, hk, min(key0 + tid, p1));
+            const uint4 * kc   = reinterpret_cast<const uint4 *>(a.kv.kc + krow * (D / 2));
+            uint4         code = __ldg(kc);
             Words<D / 64> ksw;
-            bool          k_bad = false;
-            int           pg    = nblk > 0 ? a.kv.page_of(s, min(kb_lo * kQtKeys + tid, p1)) : 0;
-            auto          load  = [&](int i) {
-                const int j = min((kb_lo + i) * kQtKeys + tid, p1);
-                k_bad       = pg < 0;
-                if (!k_bad) {
-                    const int64_t row = a.kv.row(pg, hk, j);
-                    kw.load(a.kv.kc + row * (D / 2));
-                    ksw.load(a.kv.ks + row * (D / 32));
-                }
-            };
-            if (nblk > 0) {
-                load(0);
-            }
-            for (int i = 0; i < nblk; i++) {
-                if (i + 1 < nblk) {
-                    pg = a.kv.page_of(s, min((kb_lo + i + 1) * kQtKeys + tid, p1));
-                }
-                const int sk = i % Lay::NK, note = i % kQtRing, next = (i + 2) % kQtRing;
-                if (!__all_sync(0xffffffffu, i < Lay::NK || tc_wait(&k_empty[sk], (i / Lay::NK - 1) & 1, &abort_flag, a.err))) {
-                    break;
-                }
-                // Room for the notes of block i + 2, where those of block i - 6 are: both tiles' S(i - 2) are done, so both
-                // softmaxes are past block i - 3, and no K warp is at block i + 2 before this one has filled block i. (V: the
-                // same with P.V.)
-                if (tid < 4) {
-                    bad_key[next][tid] = 0;
-                } else if (tid == 4) {
-                    bad_any[next][0] = 0;
-                }
-                const bool gone = (kb_lo + i) * kQtKeys + tid > p1;
-                if (k_bad && !gone) {
-                    atomicOr(&bad_key[note][tid >> 5], 1u << (tid & 31));
-                    bad_any[note][0] = 1;
-                    if (a.err) {
-                        atomicOr(a.err, ACB_DEVERR_PAGE_RANGE);
-                    }
-                }
-                if (k_bad || gone) {
+            ksw.load(a.kv.ks + krow * (D / 32));
+            uint2         vw[8];
+            uint16_t      vs[8];
+            if (on) {
+                const int        j   = key0 + 8 * kg;
+                const int64_t    row = vpg < 0 ? 0 : a.kv.row(vpg, hk, j);
+                const uint8_t *  c   = a.kv.vc + row * (D / 2) + wq * 8;
+                const uint16_t * d   = a.kv.vs + row * (D / 32) + (wq >> 1);
+                const int        in  = vpg < 0 ? 0 : p1 - j + 1;  // keys past the last one: none of their own
 #pragma unroll
-                    for (int w = 0; w < D / 64; w++) {
-                        ksw.w[w] = 0;
-                    }
-                }
-                uint8_t * dst = sK + sk * Lay::KB + tid * 128;
-#pragma unroll
-                for (int w = 0; w < D / 8; w++) {
-                    uint32_t r[4];
-                    unpack4(kw.w[w], half2_of(__byte_perm(ksw.w[w / 8], 0, (w / 4) & 1 ? 0x3232u : 0x1010u)), r);
-                    *reinterpret_cast<uint4 *>(dst + (w / 8) * 16384 + (((w & 7) ^ (tid & 7)) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
-                }
-                if (i + 1 < nblk) {
-                    load(i + 1);
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    ptx::mbar_arrive(&k_full[sk]);
+                for (int e = 0; e < 8; e++) {
+                    vw[e] = e < in ? __ldg(reinterpret_cast<const uint2 *>(c + e * (D / 2))) : make_uint2(0, 0);
+                    vs[e] = e < in ? __ldg(d + e * (D / 32)) : (uint16_t) 0;
                 }
             }
-        } else {
-            // V: 8 keys from 8 kg on (of one page: pages hold 16 or more), 16 dimensions: the 8 bytes from 8 wq on; the lanes of a
-            // store phase differ in kg
-            const int kg = (tid & 7) | ((tid >> 6) << 3), wq = (tid >> 3) & 7;
-            const bool on = D == 128 || wq < 4;  // heads of 64 have 4 such runs
-            uint2      vw[8];
-            uint16_t   vs[8];
-            int        pg   = nblk > 0 ? a.kv.page_of(s, min(kb_lo * kQtKeys + 8 * kg, p1)) : 0;
-            auto       load = [&](int i) {
-                const int j = (kb_lo + i) * kQtKeys + 8 * kg;
-                if (on) {
-                    const int64_t    row = pg < 0 ? 0 : a.kv.row(pg, hk, j);
-                    const uint8_t *  c   = a.kv.vc + row * (D / 2) + wq * 8;
-                    const uint16_t * d   = a.kv.vs + row * (D / 32) + (wq >> 1);
-                    const int        in  = pg < 0 ? 0 : p1 - j + 1;  // keys past the last one: none of their own
+            if (i + 1 < nblk) {
+                kpg = a.kv.page_of(s, min(key0 + kQtKeys + tid, p1));
+                vpg = a.kv.page_of(s, min(key0 + kQtKeys + 8 * kg, p1));
+            }
+            if (!__all_sync(0xffffffffu, i < Lay::NK || tc_wait(&k_empty[sk], (i / Lay::NK - 1) & 1, &abort_flag, a.err))) {
+                break;
+            }
+            // Room for the notes of block i + 2, where those of block i - 6 are: both tiles' S(i - 2) are done, so both softmaxes
+            // are past block i - 3, and no warp is at block i + 2 before this one has filled block i.
+            if (tid < 4) {
+                bad_key[next][tid] = 0;
+            } else if (tid < 6) {
+                bad_any[next][tid - 4] = 0;
+            } else if (tid >= 32 && tid < 32 + (D / 32) * 4) {
+                (&bad_val[next][0][0])[tid - 32] = 0;
+            }
+            if (k_bad && !gone) {
+                atomicOr(&bad_key[note][tid >> 5], 1u << (tid & 31));
+                bad_any[note][0] = 1;
+                if (a.err) {
+                    atomicOr(a.err, ACB_DEVERR_PAGE_RANGE);
+                }
+            }
+            uint8_t * dst  = sK + sk * Lay::KB + tid * 128;
+            uint64_t  sc64 = k_bad || gone ? 0 : D == 64 ? ksw.w[0] : (uint64_t) ksw.w[D / 64 - 1] << 32 | ksw.w[0];
+#pragma unroll 1
+            for (int b = 0; b < D / 32; b++) {  // four words, four 16-byte units
+                const uint4   w4 = code;
+                const __half2 sc = __half2half2(__ushort_as_half((uint16_t) sc64));
+                if (b + 1 < D / 32) {
+                    code = __ldg(kc + b + 1);
+                }
+                sc64 >>= 16;
+                uint8_t * d = dst + (b >> 1) * 16384;
+                const int u = 4 * (b & 1), x = tid & 7;
+                uint32_t  r[4];
+                unpack4(w4.x, sc, r);
+                *reinterpret_cast<uint4 *>(d + ((u ^ x) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+                unpack4(w4.y, sc, r);
+                *reinterpret_cast<uint4 *>(d + (((u + 1) ^ x) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+                unpack4(w4.z, sc, r);
+                *reinterpret_cast<uint4 *>(d + (((u + 2) ^ x) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+                unpack4(w4.w, sc, r);
+                *reinterpret_cast<uint4 *>(d + (((u + 3) ^ x) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                ptx::mbar_arrive(&k_full[sk]);
+            }
+            if (!__all_sync(0xffffffffu, i < Lay::NV || tc_wait(&v_empty[sv], (i / Lay::NV - 1) & 1, &abort_flag, a.err))) {
+                break;
+            }
+            if (on) {
+                uint32_t sc[4], odd = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    sc[e] = (uint32_t) vs[2 * e] | ((uint32_t) vs[2 * e + 1] << 16);
+                    // exponent field full: adding one unit carries into the sign's place
+                    odd |= ((sc[e] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+                }
+                if (odd) {
+                    uint32_t bits = 0;
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        vw[e] = e < in ? __ldg(reinterpret_cast<const uint2 *>(c + e * (D / 2))) : make_uint2(0, 0);
-                        vs[e] = e < in ? __ldg(d + e * (D / 32)) : (uint16_t) 0;
+                        if ((vs[e] & 0x7C00u) == 0x7C00u) {
+                            sc[e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                            bits |= 1u << e;
+                        }
                     }
+                    atomicOr(&bad_val[note][wq >> 1][kg >> 2], bits << (8 * (kg & 3)));
+                    bad_any[note][1] = 1;
                 }
-            };
-            if (nblk > 0) {
-                load(0);
-            }
-            for (int i = 0; i < nblk; i++) {
-                if (i + 1 < nblk) {
-                    pg = a.kv.page_of(s, min((kb_lo + i + 1) * kQtKeys + 8 * kg, p1));
-                }
-                const int sv = i % Lay::NV, note = i % kQtRing, next = (i + 2) % kQtRing;
-                if (!__all_sync(0xffffffffu, i < Lay::NV || tc_wait(&v_empty[sv], (i / Lay::NV - 1) & 1, &abort_flag, a.err))) {
-                    break;
-                }
-                if (tid < (D / 32) * 4) {
-                    (&bad_val[next][0][0])[tid] = 0;
-                } else if (tid == (D / 32) * 4) {
-                    bad_any[next][1] = 0;
-                }
-                if (on) {
-                    uint32_t sc[4], odd = 0;
+                uint8_t * base = sV + sv * Lay::VB + (kg >> 3) * (D * 128);
+#pragma unroll 1
+                for (int h = 0; h < 4; h++) {  // bytes 2h and 2h + 1 of the 8
+                    uint32_t       r[4][4];    // [pair of keys][low, high of byte 2h, low, high of byte 2h + 1]
+                    const uint32_t sel = h & 1 ? 0x7632u : 0x5410u;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        sc[e] = (uint32_t) vs[2 * e] | ((uint32_t) vs[2 * e + 1] << 16);
-                        // exponent field full: adding one unit carries into the sign's place
-                        odd |= (((sc[e] & 0x7C007C00u) + 0x04000400u) & 0x80008000u);
+                        const uint32_t x = h < 2 ? vw[2 * e].x : vw[2 * e].y, y = h < 2 ? vw[2 * e + 1].x : vw[2 * e + 1].y;
+                        unpack4(__byte_perm(x, y, sel), half2_of(sc[e]), r[e]);
                     }
-                    if (odd) {
-                        uint32_t bits = 0;
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            if ((vs[e] & 0x7C00u) == 0x7C00u) {
-                                sc[e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-                                bits |= 1u << e;
-                            }
-                        }
-                        atomicOr(&bad_val[note][wq >> 1][kg >> 2], bits << (8 * (kg & 3)));
-                        bad_any[note][1] = 1;
-                    }
-                    uint8_t * base = sV + sv * Lay::VB + (kg >> 3) * (D * 128);
-#pragma unroll
-                    for (int h = 0; h < 4; h++) {  // bytes 2h and 2h + 1 of the 8
-                        uint32_t r[4][4];          // [pair of keys][low, high of byte 2h, low, high of byte 2h + 1]
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const uint32_t x = h < 2 ? vw[2 * e].x : vw[2 * e].y, y = h < 2 ? vw[2 * e + 1].x : vw[2 * e + 1].y;
-                            unpack4(__byte_perm(x, y, (h & 1) ? 0x7632u : 0x5410u), half2_of(sc[e]), r[e]);
-                        }
-#pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const int d = (wq >> 1) * 32 + (wq & 1) * 8 + 2 * h + (q >> 1) + 16 * (q & 1);
-                            *reinterpret_cast<uint4 *>(base + d * 128 + (((kg & 7) ^ (2 * h + (q >> 1))) << 4)) =
-                                make_uint4(r[0][q], r[1][q], r[2][q], r[3][q]);
-                        }
+                    for (int q = 0; q < 4; q++) {
+                        const int d = (wq >> 1) * 32 + (wq & 1) * 8 + 2 * h + (q >> 1) + 16 * (q & 1);
+                        *reinterpret_cast<uint4 *>(base + d * 128 + (((kg & 7) ^ (2 * h + (q >> 1))) << 4)) =
+                            make_uint4(r[0][q], r[1][q], r[2][q], r[3][q]);
                     }
                 }
-                if (i + 1 < nblk) {
-                    load(i + 1);
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    ptx::mbar_arrive(&v_full[sv]);
-                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                ptx::mbar_arrive(&v_full[sv]);
             }
         }
     } else if (warp == kQtMma) {
@@ -308,7 +288,7 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
                 const uint32_t v = ptx::smem_u32(sV + (i % Lay::NV) * Lay::VB);
 #pragma unroll
                 for (int kk = 0; kk < kQtKeys / 16; kk++) {
-                    umma_ts(tmem + (uint32_t) (256 + t * 128), tmem + (uint32_t) (t * 128 + 64 + kk * 8),
+                    umma_ts(tmem + (uint32_t) (256 + t * 128), tmem + (uint32_t) (t * 128 + kk * 8),
                             smem_desc_sw128(v + (kk >> 2) * (D * 128) + (kk & 3) * 32), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
                 }
             };
@@ -453,37 +433,36 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
                     see[w] &= ~bad_key[i % kQtRing][w];
                 }
             }
-            uint32_t x[64];
-            auto     hide = [&](uint32_t b0, uint32_t b1) {
+            // Rolled loops of 32 keys: the code of the four kinds of warps does not fit the instruction caches unrolled
+            uint32_t xa[32], xb[32];
+            auto     hide = [&](uint32_t * x, uint32_t bits) {
+                if (part) {
 #pragma unroll
-                for (int c = 0; c < 64; c++) {
-                    x[c] = ((c < 32 ? b0 : b1) >> (c & 31)) & 1u ? x[c] : 0xFF800000u;
-                }
-            };
-            auto top = [&]() {
-                float g[4];
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    g[c] = fmaxf(__uint_as_float(x[c]), __uint_as_float(x[c + 4]));
-#pragma unroll
-                    for (int e = 8; e < 64; e += 8) {
-                        g[c] = fmaxf(g[c], fmaxf(__uint_as_float(x[c + e]), __uint_as_float(x[c + e + 4])));
+                    for (int c = 0; c < 32; c++) {
+                        x[c] = (bits >> c) & 1u ? x[c] : 0xFF800000u;
                     }
                 }
-                return fmaxf(fmaxf(g[0], g[1]), fmaxf(g[2], g[3]));
             };
-            // keys 0..63 for their maximum, keys 64..127 to stay; then keys 0..63 once more
-            tmem_ld64(tS, x);
-            if (part) {
-                hide(see[0], see[1]);
+            float g[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
+            auto  top  = [&](const uint32_t * x) {
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    g[(c >> 1) & 3] = fmaxf(g[(c >> 1) & 3], fmaxf(__uint_as_float(x[c]), __uint_as_float(x[c + 1])));
+                }
+            };
+            tmem_ld32_start(tS, xa);
+#pragma unroll 1
+            for (int w = 0; w < 4; w += 2) {
+                tmem_arrived(xa);
+                tmem_ld32_start(tS + (uint32_t) (32 * w + 32), xb);
+                hide(xa, w == 0 ? see[0] : see[2]);
+                top(xa);
+                tmem_arrived(xb);
+                tmem_ld32_start(tS + (uint32_t) (w == 0 ? 64 : 0), xa);  // the last: the first again, for its exponentials
+                hide(xb, w == 0 ? see[1] : see[3]);
+                top(xb);
             }
-            float mx = top();
-            tmem_ld64(tS + 64, x);
-            if (part) {
-                hide(see[2], see[3]);
-            }
-            mx               = fmaxf(mx, top());
-            const float mb   = mx * sc;
+            const float mb   = fmaxf(fmaxf(g[0], g[1]), fmaxf(g[2], g[3])) * sc;
             bool        resc = false;
             float       alpha = 1.0f;
             if (m == -INFINITY) {
@@ -495,28 +474,31 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
             }
             const float nm    = m == -INFINITY ? 0.0f : kQtLift - m;
             float       ps[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
-            // P of keys k.. into columns 64 + k / 2.., over the scores of keys 64..127
-            auto weigh = [&](int half) {
+            auto weigh = [&](const uint32_t * x, int w) {
+                uint32_t ph[16];
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    uint32_t ph[16];
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float e0 = ex2_fast(fmaf(__uint_as_float(x[32 * c + 2 * e]), sc, nm));
-                        const float e1 = ex2_fast(fmaf(__uint_as_float(x[32 * c + 2 * e + 1]), sc, nm));
-                        ps[e & 1] += e0;
-                        ps[2 + (e & 1)] += e1;
-                        ph[e] = u32_of(__floats2half2_rn(e0, e1));
-                    }
-                    tmem_st16(tS + (uint32_t) (64 + 32 * half + 16 * c), ph);
+                for (int e = 0; e < 16; e++) {
+                    const float e0 = ex2_fast(fmaf(__uint_as_float(x[2 * e]), sc, nm));
+                    const float e1 = ex2_fast(fmaf(__uint_as_float(x[2 * e + 1]), sc, nm));
+                    ps[e & 1] += e0;
+                    ps[2 + (e & 1)] += e1;
+                    ph[e] = u32_of(__floats2half2_rn(e0, e1));
                 }
+                tmem_st16(tS + (uint32_t) (16 * w), ph);  // over scores that have been read (chunk w / 2)
             };
-            weigh(1);
-            tmem_ld64(tS, x);
-            if (part) {
-                hide(see[0], see[1]);
+#pragma unroll 1
+            for (int w = 0; w < 4; w += 2) {
+                tmem_arrived(xa);
+                tmem_ld32_start(tS + (uint32_t) (32 * w + 32), xb);
+                hide(xa, w == 0 ? see[0] : see[2]);
+                weigh(xa, w);  // columns 16 w.., of chunk w / 2 = w - w / 2: read, and not the one on its way
+                tmem_arrived(xb);
+                if (w == 0) {
+                    tmem_ld32_start(tS + 64, xa);
+                }
+                hide(xb, w == 0 ? see[1] : see[3]);
+                weigh(xb, w + 1);
             }
-            weigh(0);
             if (__any_sync(0xffffffffu, resc)) {  // P.V(i - 1) is done: O is whole
 #pragma unroll 1
                 for (int c = 0; c < D / 32; c++) {
