@@ -20,6 +20,7 @@ struct AttnQ4Args {
     KvQ4            kv;
     bool            q_vec;    // rows of q are 16-byte aligned
     int             chunk;    // keys of a block, a multiple of 64
+    int             tiles;    // of the rows
     int             n_split;  // chunks that the rows of one block can touch
     float *         part_o;   // [n_tok*Nh][n_split][D]: sums of P V
     float2 *        part_ml;  // [n_tok*Nh][n_split]: m (log2), l

@@ -93,12 +93,15 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
     constexpr int  QP  = T == ACB_TYPE_F32 ? 2 : 1;
     constexpr int  R   = 8 * NT;
     using T1           = typename io<T>::t;
-    __shared__ int   s_hi[R], s_lo[R];
+    __shared__ int   s_hi[R], s_lo[R], s_first[R], s_last[R];  // of the rows: last and first key, and their chunks
     __shared__ float s_m[kSplitWarps][R], s_l[kSplitWarps][R], s_top[R];
     extern __shared__ __align__(16) uint8_t smem[];  // the warps' rings, then the sums of the warps' parts
     float (*s_o)[D + 4] = reinterpret_cast<float (*)[D + 4]>(smem);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int rt = blockIdx.x / a.n_split, split = blockIdx.x - rt * a.n_split, hk = blockIdx.y, s = blockIdx.z;
+    const int hk = blockIdx.y, s = blockIdx.z;
+    const int rt = a.tiles == 1 ? 0 : blockIdx.x / a.n_split, split = blockIdx.x - rt * a.n_split;
+    // new token of row r; the division only where there is more than one
+    auto token_of = [&](int r) { return a.max_q == 1 ? (r >= a.G ? 1 : 0) : r / a.G; };
     ptx::grid_dep_launch();
     int64_t    row0;
     int        n, len;
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
         return;
     }
     // the keys that some row of this block sees
-    const int i0 = r0 / a.G, i1 = min(n - 1, (r0 + R - 1) / a.G);
+    const int i0 = token_of(r0), i1 = min(n - 1, token_of(r0 + R - 1));
     const int p0 = ok ? len - n + i0 : -1, p1 = ok ? len - n + i1 : -1;
     const int lo0 = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
     // rows that see no key are written by the first block
@@ -124,15 +127,17 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
             }
         }
     }
-    const int c  = lo0 / a.chunk + split;
+    const int c  = (lo0 > 0 ? lo0 / a.chunk : 0) + split;
     const int j0 = max(lo0, c * a.chunk), j1 = min(p1 + 1, (c + 1) * a.chunk);
     if (j0 >= j1) {
         return;
     }
     if (threadIdx.x < R) {
-        const int i = (r0 + threadIdx.x) / a.G, p = i < n ? len - n + i : -1;
-        s_hi[threadIdx.x] = p;
-        s_lo[threadIdx.x] = a.window > 0 ? max(0, p - a.window + 1) : 0;
+        const int i = token_of(r0 + threadIdx.x), p = i < n ? len - n + i : -1, lo = a.window > 0 ? max(0, p - a.window + 1) : 0;
+        s_hi[threadIdx.x]    = p;
+        s_lo[threadIdx.x]    = lo;
+        s_first[threadIdx.x] = lo > 0 ? lo / a.chunk : 0;
+        s_last[threadIdx.x]  = p >= 0 ? p / a.chunk : -1;
     }
     __syncthreads();
     // keys before full0 are behind the last row's window
@@ -143,8 +148,8 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
     float    sc[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        const int  r = r0 + nt * 8 + g, i = r / a.G;
-        const T1 * q = reinterpret_cast<const T1 *>(a.q) + (row0 + i) * a.q_stride + (int64_t) (hk * a.G + r % a.G) * D;
+        const int  r = r0 + nt * 8 + g, i = token_of(r);
+        const T1 * q = reinterpret_cast<const T1 *>(a.q) + (row0 + i) * a.q_stride + (int64_t) (hk * a.G + r - i * a.G) * D;
         float      f[KT][4], mx = 0.0f;
 #pragma unroll
         for (int w = 0; w < D / 64; w++) {
@@ -480,16 +485,14 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
     __syncthreads();
     for (int e = threadIdx.x; e < R * D / 4; e += 32 * kSplitWarps) {
         const int rr = e / (D / 4), d = (e % (D / 4)) * 4;
-        const int r = r0 + rr, i = r / a.G;
-        const int p = i < n ? s_hi[rr] : -1;
-        const int c0 = s_lo[rr] / a.chunk, c1 = p / a.chunk;
-        if (p < 0 || c < c0 || c > c1) {  // no key of this row in this chunk
+        const int r = r0 + rr, i = token_of(r), c0 = s_first[rr], c1 = s_last[rr];
+        if (c < c0 || c > c1) {  // no key of this row in this chunk (or no such row)
             continue;
         }
         const float   L   = s_l[0][rr];
         const float4  v   = *reinterpret_cast<const float4 *>(&s_o[rr][d]);
         const int64_t tok = row0 + i;
-        const int     h   = hk * a.G + r % a.G;
+        const int     h   = hk * a.G + r - i * a.G;
         if (c0 == c1) {  // every key of this row was in this chunk
             const float inv = L != 0.0f ? 1.0f / L : 0.0f;
             T1 *        y   = reinterpret_cast<T1 *>(a.o) + tok * a.o_stride + (int64_t) h * D + d;
@@ -521,7 +524,7 @@ template <int T, int D> __global__ void __launch_bounds__(32 * kJoinWarps) attn_
     int64_t    row0;
     int        n, len;
     const bool ok = seq_bounds(a, s, &row0, &n, &len);
-    const int  i = r / a.G, p = len - n + i;
+    const int  i = a.max_q == 1 ? 0 : r / a.G, p = len - n + i;
     if (!ok || i >= n || p < 0) {
         return;
     }
@@ -530,7 +533,7 @@ template <int T, int D> __global__ void __launch_bounds__(32 * kJoinWarps) attn_
         return;
     }
     const int64_t tok = row0 + i;
-    const int     h   = hk * a.G + r % a.G;
+    const int     h   = hk * a.G + r - i * a.G;
     const int64_t at  = (tok * a.Nh + h) * a.n_split;
     float         M = -INFINITY, L = 0.0f, o[E];
     for (int c = c0 + lane; c <= c1; c += 32) {
@@ -697,6 +700,7 @@ extern "C" acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int t
     a.q_vec      = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_stride * type_size(type) % 16 == 0;
     a.chunk      = p.chunk;
     a.n_split    = p.n_split;
+    a.tiles      = p.tiles;
     a.part_ml    = reinterpret_cast<float2 *>(work);
     a.part_o     = reinterpret_cast<float *>(work) + 2 * n_tok * n_heads * p.n_split;
     const int D = kv->head_dim;

@@ -5,7 +5,7 @@
 //   0..3, 4..7  softmax of tile 0 and of tile 1, a thread a row (a TMEM lane): 64 scores at a time: the maximum of
 //               the first half, that of the second, the second's exponentials, the first half again for its own; P takes the
 //               second half's columns as f16. (Two threads a row with both halves of one
-//               tile in registers, and the exchange that takes, held the tensor cores at 20%: 462 us where this takes 310; all
+//               tile in registers, and the exchange that takes, held the tensor cores at 20%: 462 us where this takes 303; all
 //               eight warps on one tile at a time 376 us.)
 //   8..11       K: a thread a key; the 8 dimensions of a word of codes make one 16-byte unit in the order that unpack4 gives
 //               them, and Q is written in the same order (a product does not depend on the order of its k index);
@@ -39,6 +39,29 @@ template <int D> struct QtLayout {
     static constexpr int TOTAL = 2 * QB + NK * KB + NV * VB;
     // TMEM columns: S/P of the tiles at 0 and 128, O at 256 and 384
 };
+
+// two f32 in one operation (sm_100)
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+
+__device__ __forceinline__ void unpack2(uint64_t v, float * x, float * y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(*x), "=f"(*y) : "l"(v));
+}
+
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 
 // 32 columns of this warp's lanes on their way into r, which must not be looked at before tmem_arrived(r)
 __device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t * r) {
@@ -473,16 +496,18 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
                 resc  = true;
             }
             const float nm    = m == -INFINITY ? 0.0f : kQtLift - m;
-            float       ps[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+            const uint64_t sc2 = pack2(sc, sc), nm2 = pack2(nm, nm);
+            uint64_t       ps[2] = { 0, 0 };  // sums of weights, two each
             auto weigh = [&](const uint32_t * x, int w) {
                 uint32_t ph[16];
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
-                    const float e0 = ex2_fast(fmaf(__uint_as_float(x[2 * e]), sc, nm));
-                    const float e1 = ex2_fast(fmaf(__uint_as_float(x[2 * e + 1]), sc, nm));
-                    ps[e & 1] += e0;
-                    ps[2 + (e & 1)] += e1;
-                    ph[e] = u32_of(__floats2half2_rn(e0, e1));
+                    float e0, e1;
+                    unpack2(fma2(pack2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), sc2, nm2), &e0, &e1);
+                    e0        = ex2_fast(e0);
+                    e1        = ex2_fast(e1);
+                    ps[e & 1] = add2(ps[e & 1], pack2(e0, e1));
+                    ph[e]     = u32_of(__floats2half2_rn(e0, e1));
                 }
                 tmem_st16(tS + (uint32_t) (16 * w), ph);  // over scores that have been read (chunk w / 2)
             };
@@ -511,7 +536,10 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
                     tmem_st32(tO + (uint32_t) (c * 32), o);
                 }
             }
-            l = l * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
+            float s0, s1, s2, s3;
+            unpack2(ps[0], &s0, &s1);
+            unpack2(ps[1], &s2, &s3);
+            l = l * alpha + ((s0 + s1) + (s2 + s3));
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
