@@ -15,6 +15,8 @@
 // 16 keys already in flight. Long sequences are cut into chunks of keys, one block each; a second kernel joins the parts.
 #include <math.h>
 
+#include <type_traits>
+
 #include "attn_q4.cuh"
 #include "ptx.cuh"
 
@@ -53,21 +55,27 @@ template <int D> struct Stage16 {
     static constexpr int V = 16 * KP, KS = V + 16 * VP, VS = KS + D, BYTES = VS + D;
     static constexpr int KW = D / 32, VW = D / 64;
 
-    // the copies of one warp, 16 bytes a lane: the rows of a tile are consecutive in the pool
-    static __device__ __forceinline__ void fill(uint32_t st, const KvQ4 & kv, uint32_t row, int lane) {
-        const uint8_t * kc = kv.kc + (uint64_t) row * (D / 2) + lane * 16;
-        const uint8_t * vc = kv.vc + (uint64_t) row * (D / 2) + lane * 16;
+    // the copies of one warp, 16 bytes a lane: the rows of a tile are consecutive in the pool. What a lane copies and where to:
+    const uint8_t * kc;
+    const uint8_t * vc;
+    const uint8_t * sc;
+    uint32_t        kd, vd;
+
+    __device__ __forceinline__ Stage16(const KvQ4 & kv, int lane)
+        : kc(kv.kc + lane * 16), vc(kv.vc + lane * 16),
+          sc(reinterpret_cast<const uint8_t *>(lane < D / 16 ? kv.ks : kv.vs) + lane % (D / 16) * 16),
+          kd(lane / (D / 32) * KP + lane % (D / 32) * 16), vd(V + lane / (D / 32) * VP + lane % (D / 32) * 16) {}
+
+    __device__ __forceinline__ void fill(uint32_t st, uint32_t row, int lane) const {
+        const uint8_t * k = kc + (uint64_t) row * (D / 2);
+        const uint8_t * v = vc + (uint64_t) row * (D / 2);
 #pragma unroll
         for (int i = 0; i < D / 64; i++) {
-            const int c = lane + 32 * i, j = c / (D / 32), x = c % (D / 32) * 16;
-            copy16(st + j * KP + x, kc + 512 * i);
-            copy16(st + V + j * VP + x, vc + 512 * i);
+            copy16(st + kd + i * (1024 / D) * KP, k + 512 * i);
+            copy16(st + vd + i * (1024 / D) * VP, v + 512 * i);
         }
         if (lane < D / 8) {
-            const bool      val = lane >= D / 16;
-            const uint8_t * sc  = reinterpret_cast<const uint8_t *>(val ? kv.vs : kv.ks) + (uint64_t) row * (D / 16) +
-                                 (val ? lane - D / 16 : lane) * 16;
-            copy16(st + KS + lane * 16, sc);
+            copy16(st + KS + lane * 16, sc + (uint64_t) row * (D / 16));
         }
     }
     static __device__ __forceinline__ void copy16(uint32_t dst, const void * src) {
@@ -229,14 +237,17 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
         }
     }
 
-    const int hi_min = p0;  // the first row's last key: keys up to it are seen by all rows that exist
     const int tb0    = (j0 & ~15) + 16 * warp;
     using St = Stage16<D>;
     constexpr int  STEP = 16 * kSplitWarps, NST = kStages<D>;
     const uint32_t ring = ptx::smem_u32(smem) + warp * (NST * St::BYTES);
     const uint8_t * mine = smem + warp * (NST * St::BYTES);
+    const St        mover(a.kv, lane);
 
-    auto take = [&](const int tb, const uint8_t * st) {
+    // A tile; EDGE: one that some row does not see whole, with -inf for what it does not see and the values that no row sees
+    // left out. The others, nearly all, have none of that in their code.
+    auto take = [&](auto edge_tile, const int tb, const uint8_t * st) {
+        constexpr bool EDGE = decltype(edge_tile)::value;
         // scores
         Words<St::KW>    k[2];
         const uint16_t * ksc = reinterpret_cast<const uint16_t *>(st + St::KS) + g * (D / 32) + t * D / 128;
@@ -262,10 +273,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
                 }
             }
         }
-        // a tile that some row does not see whole: -inf for what it does not see, and the values that no row sees left out
-        const bool edge = tb < full0 || tb < j0 || tb + 15 > hi_min || tb + 15 >= j1;
-        if (edge) {
-            asm volatile("" ::: "memory");  // a branch: these instructions are for few tiles
+        if (EDGE) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -333,8 +341,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
         }
         uint32_t vs01 = (uint32_t) vs[0] | ((uint32_t) vs[1] << 16);
         uint32_t vs23 = (uint32_t) vs[2] | ((uint32_t) vs[3] << 16);
-        if (edge) {
-            asm volatile("" ::: "memory");
+        if (EDGE) {
             // a scale that is no number must not reach the rows that do not see its key (0 * NaN): it is taken out here and
             // put on the rows that do see it one by one
             uint32_t any = 0;
@@ -398,7 +405,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
         if (tb < j1) {
             lost = (lost & ~(1u << slot)) | (uint32_t) (pg < 0) << slot;
             if (pg >= 0) {
-                St::fill(ring + slot * St::BYTES, a.kv, a.kv.row(pg, hk, tb), lane);
+                mover.fill(ring + slot * St::BYTES, a.kv.row(pg, hk, tb), lane);
             }
             if (tb + STEP < j1) {
                 pg = a.kv.page_of(s, tb + STEP);
@@ -421,7 +428,11 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
                 atomicOr(a.err, ACB_DEVERR_PAGE_RANGE);
             }
         } else {
-            take(tb, mine + slot * St::BYTES);
+            if (tb < full0 || tb < j0 || tb + 15 > p0 || tb + 15 >= j1) {
+                take(std::true_type{}, tb, mine + slot * St::BYTES);
+            } else {
+                take(std::false_type{}, tb, mine + slot * St::BYTES);
+            }
         }
         slot = slot == NST - 1 ? 0 : slot + 1;
     }
