@@ -432,11 +432,14 @@ def _device(name, t):
 
 
 def _want(name, t, dtype, dev, numel=0, contiguous=True):
-    """Refuses a tensor that the kernels would misread: another type, another device, gaps, too few elements."""
-    if t is not None and (t.dtype is not dtype or t.get_device() != dev or t.numel() < numel
-                          or (contiguous and not t.is_contiguous())):
+    """Address of t (None: 0). Refuses a tensor that the kernels would misread: another type, another device, gaps, too few
+    elements."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.get_device() != dev or t.numel() < numel or (contiguous and not t.is_contiguous()):
         raise ValueError(f"{name}: a {'contiguous ' if contiguous else ''}{dtype} tensor on GPU {dev} of {numel} elements or more "
                          f"is wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
 def _row_stride(name, t, width):
@@ -469,14 +472,13 @@ def rope(x, pos, table, layout="half", inverse=False, out=None, err=None, stream
     sx, so = x.stride(), out.stride()
     if out.dtype is not x.dtype or out.shape != x.shape or out.get_device() != dev or sx[2] != 1 or so[2] != 1:
         raise ValueError("rope: x and out have one type, shape and device, their last dimension contiguous")
-    _want("rope: pos", pos, torch.int32, dev, T)
-    _want("rope: table", table, torch.float32, dev)
+    at_pos, at_table = _want("rope: pos", pos, torch.int32, dev, T), _want("rope: table", table, torch.float32, dev)
     if T == 0 or H == 0:
         return out
     max_pos, width = table.shape
     _run_on("acb_rope", dev, stream, x.data_ptr(), sx[0], sx[1], out.data_ptr(), so[0], so[1],
             dtype_id(x), T, H, D, width,
-            _ROPE_LAYOUT[layout] | (ROPE_INVERSE if inverse else 0), pos.data_ptr(), table.data_ptr(), max_pos, _ptr(err))
+            _ROPE_LAYOUT[layout] | (ROPE_INVERSE if inverse else 0), at_pos, at_table, max_pos, _ptr(err))
     return out
 
 
@@ -528,11 +530,12 @@ class KVCacheQ4:
         T, D, dev = qkv.shape[0], self.head_dim, self.dev
         if qkv.get_device() != dev or qkv.stride(1) != 1 or qkv.shape[1] < (n_heads + 2 * self.n_kv_heads) * D:
             raise ValueError("KVCacheQ4.append: qkv [T, (n_heads + 2 n_kv_heads) * head_dim] on the cache's device is wanted")
-        _want("KVCacheQ4.append: seq", seq, torch.int32, dev, T)
-        _want("KVCacheQ4.append: pos", pos, torch.int32, dev, T)
-        _want("KVCacheQ4.append: table", table, torch.float32, dev)
-        _want("KVCacheQ4.append: q_norm", q_norm, torch.float32, dev, D)
-        _want("KVCacheQ4.append: k_norm", k_norm, torch.float32, dev, D)
+        i32, f32 = torch.int32, torch.float32
+        at_seq = _want("KVCacheQ4.append: seq", seq, i32, dev, T)
+        at_pos = _want("KVCacheQ4.append: pos", pos, i32, dev, T)
+        at_table = _want("KVCacheQ4.append: table", table, f32, dev)
+        at_qn = _want("KVCacheQ4.append: q_norm", q_norm, f32, dev, D)
+        at_kn = _want("KVCacheQ4.append: k_norm", k_norm, f32, dev, D)
         if n_heads > 0 and q_out is None:
             q_out = torch.empty((T, n_heads, D), dtype=q_dtype or qkv.dtype, device=self.device)
         if n_heads > 0 and (q_out.shape != (T, n_heads, D) or q_out.stride()[1:] != (D, 1) or q_out.get_device() != dev):
@@ -541,9 +544,8 @@ class KVCacheQ4:
             return q_out
         mp, rd = table.shape if table is not None else (0, 0)
         _run_on("acb_kv_q4_append", dev, stream, self.ref, qkv.data_ptr(), dtype_id(qkv),
-                _row_stride("KVCacheQ4.append: qkv", qkv, qkv.shape[1]), T,
-                n_heads, _ptr(q_norm), _ptr(k_norm), eps, _ptr(table), mp, rd, _ROPE_LAYOUT[layout], seq.data_ptr(),
-                pos.data_ptr(), _ptr(q_out), dtype_id(q_out if q_out is not None else qkv),
+                _row_stride("KVCacheQ4.append: qkv", qkv, qkv.shape[1]), T, n_heads, at_qn, at_kn, eps, at_table, mp, rd,
+                _ROPE_LAYOUT[layout], at_seq, at_pos, _ptr(q_out), dtype_id(q_out if q_out is not None else qkv),
                 _row_stride("KVCacheQ4.append: q_out", q_out, n_heads * D) if q_out is not None else 0, _ptr(err))
         return q_out
 
@@ -551,8 +553,8 @@ class KVCacheQ4:
         """The cached keys and values at (seq, pos) as [T, n_kv_heads, D]: both when neither output is given."""
         import torch
         T, shape = seq.numel(), (seq.numel(), self.n_kv_heads, self.head_dim)
-        _want("KVCacheQ4.read: seq", seq, torch.int32, self.dev)
-        _want("KVCacheQ4.read: pos", pos, torch.int32, self.dev, T)
+        at_seq = _want("KVCacheQ4.read: seq", seq, torch.int32, self.dev)
+        at_pos = _want("KVCacheQ4.read: pos", pos, torch.int32, self.dev, T)
         if k_out is None and v_out is None:
             k_out = torch.empty(shape, dtype=dtype or torch.float16, device=self.device)
             v_out = torch.empty_like(k_out)
@@ -563,7 +565,7 @@ class KVCacheQ4:
                 raise ValueError("KVCacheQ4.read: outputs [T, n_kv_heads, head_dim] of one type with contiguous rows are wanted")
         if T == 0:
             return k_out, v_out
-        _run_on("acb_kv_q4_read", self.dev, stream, self.ref, seq.data_ptr(), pos.data_ptr(), T, _ptr(k_out), _ptr(v_out),
+        _run_on("acb_kv_q4_read", self.dev, stream, self.ref, at_seq, at_pos, T, _ptr(k_out), _ptr(v_out),
                 dtype_id(first), _row_stride("KVCacheQ4.read", first, shape[1] * shape[2]), _ptr(err))
         return k_out, v_out
 
@@ -585,8 +587,8 @@ class KVCacheQ4:
             max_kv_len = c.max_pages * c.page_size
         if q.get_device() != dev or D != self.head_dim or q.stride()[1:] != (D, 1):
             raise ValueError("KVCacheQ4.attention: q [T, n_heads, head_dim] with contiguous rows on the cache's device is wanted")
-        _want("KVCacheQ4.attention: kv_len", kv_len, torch.int32, dev, self.n_seq)
-        _want("KVCacheQ4.attention: q_start", q_start, torch.int32, dev, self.n_seq + 1)
+        at_len = _want("KVCacheQ4.attention: kv_len", kv_len, torch.int32, dev, self.n_seq)
+        at_start = _want("KVCacheQ4.attention: q_start", q_start, torch.int32, dev, self.n_seq + 1)
         if out is None:
             out = torch.empty((T, H, D), dtype=q.dtype, device=self.device)
         if out.dtype is not q.dtype or out.shape != q.shape or out.stride()[1:] != (D, 1) or out.get_device() != dev:
@@ -598,8 +600,7 @@ class KVCacheQ4:
         elif work.get_device() != dev or not work.is_contiguous():
             raise ValueError("KVCacheQ4.attention: the workspace is a contiguous tensor on the cache's device")
         _run_on("acb_attn_kv_q4", dev, stream, self.ref, q.data_ptr(), dtype_id(q), _row_stride("KVCacheQ4.attention: q", q, H * D),
-                T, H, _ptr(q_start),
-                kv_len.data_ptr(), max_q_len, max_kv_len, window, D ** -0.5 if scale is None else scale, out.data_ptr(),
+                T, H, at_start, at_len, max_q_len, max_kv_len, window, D ** -0.5 if scale is None else scale, out.data_ptr(),
                 _row_stride("KVCacheQ4.attention: out", out, H * D), _ptr(work), work.numel() * work.element_size() if work is not None else 0, _ptr(err))
         return out
 
@@ -623,34 +624,41 @@ def logits_rules(logits, hist=None, hist_len=None, prompt_len=None, rep=None, fr
         out = torch.empty((R, V), dtype=out_dtype or logits.dtype, device=logits.device)
     if out.shape != logits.shape or out.get_device() != dev or logits.stride(1) != 1 or out.stride(1) != 1:
         raise ValueError("logits_rules: logits and out [R, V] with contiguous rows are wanted")
-    _want("logits_rules: hist_len", hist_len, i32, dev, R)
-    _want("logits_rules: prompt_len", prompt_len, i32, dev, R)
-    _want("logits_rules: rep", rep, f32, dev, R)
-    _want("logits_rules: freq", freq, f32, dev, R)
-    _want("logits_rules: pres", pres, f32, dev, R)
-    _want("logits_rules: mask_row", mask_row, i32, dev, R)
+    at_len = _want("logits_rules: hist_len", hist_len, i32, dev, R)
+    at_prompt = _want("logits_rules: prompt_len", prompt_len, i32, dev, R)
+    at_rep = _want("logits_rules: rep", rep, f32, dev, R)
+    at_freq = _want("logits_rules: freq", freq, f32, dev, R)
+    at_pres = _want("logits_rules: pres", pres, f32, dev, R)
+    at_row = _want("logits_rules: mask_row", mask_row, i32, dev, R)
+    at_hist = _want("logits_rules: hist", hist, i32, dev)
+    at_ids = _want("logits_rules: bias_ids", bias_ids, i32, dev)
+    at_mask = _want("logits_rules: mask", mask, i32, dev)
     if R == 0:
         return out
-    r = _LogitRules(mask_row=_ptr(mask_row))
+    n_hist = n_bias = bias_stride = n_masks = words = 0
+    at_val = None
     if hist is not None:
-        _want("logits_rules: hist", hist, i32, dev)
         if hist.dim() != 2 or hist.shape[0] < R:
             raise ValueError("logits_rules: hist [R, L] is wanted")
+        n_hist = hist.shape[1]
     elif rep is not None or freq is not None or pres is not None:
         raise ValueError("logits_rules: penalties go by a history")
-    if hist is not None and hist.shape[1] > 0:
-        r.hist, r.hist_stride, r.hist_len, r.prompt_len = hist.data_ptr(), hist.shape[1], _ptr(hist_len), _ptr(prompt_len)
-        r.rep, r.freq, r.pres = _ptr(rep), _ptr(freq), _ptr(pres)
+    if n_hist == 0:  # nothing to go by
+        at_hist = at_len = at_prompt = at_rep = at_freq = at_pres = None
     if bias_ids is not None and bias_ids.numel() > 0:
-        _want("logits_rules: bias_ids", bias_ids, i32, dev)
-        _want("logits_rules: bias_val", bias_val, f32, dev, bias_ids.numel())
-        r.bias_ids, r.bias_val, r.n_bias = bias_ids.data_ptr(), _ptr(bias_val), bias_ids.shape[-1]
-        r.bias_stride = r.n_bias if bias_ids.dim() == 2 else 0
-        if bias_ids.dim() == 2 and bias_ids.shape[0] < R:
+        at_val = _want("logits_rules: bias_val", bias_val, f32, dev, bias_ids.numel())
+        n_bias = bias_ids.shape[-1]
+        bias_stride = n_bias if bias_ids.dim() == 2 else 0
+        if bias_ids.dim() > 2 or (bias_ids.dim() == 2 and bias_ids.shape[0] < R):
             raise ValueError("logits_rules: a bias list for every row, or one for all, is wanted")
+    else:
+        at_ids = None
     if mask is not None:
-        _want("logits_rules: mask", mask, i32, dev)
-        r.mask, r.n_masks, r.mask_stride = mask.data_ptr(), mask.shape[0], mask.shape[1]
+        n_masks, words = mask.shape
+        if mask_row is None and n_masks < R:
+            raise ValueError("logits_rules: a mask for every row, or mask_row, is wanted")
+    r = _LogitRules(at_hist, n_hist, at_len, at_prompt, at_rep, at_freq, at_pres, at_ids, at_val, bias_stride, n_bias, n_masks,
+                    at_mask, words, at_row)
     _run_on("acb_logits_rules", dev, stream, logits.data_ptr(), dtype_id(logits), _row_stride("logits_rules: logits", logits, V),
             out.data_ptr(), dtype_id(out), _row_stride("logits_rules: out", out, V), R, V, C.addressof(r), _ptr(err))
     return out

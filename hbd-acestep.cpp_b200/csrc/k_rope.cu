@@ -4,10 +4,13 @@
 // With z = a + i b for a pair and w = c + i s its table entry, the rotation is z' = z w (w's conjugate for the
 // inverse): 6 flops on 2 elements against a read and a write of both, so the memory bounds it. The vector form takes 16
 // bytes at a time (with half pairs, 16 bytes of each half), a block one or more whole tokens, so that the angles of a token come
-// from L1 for all its heads; where alignment or an odd width forbids that, a warp takes a head pair by pair. 8191 tokens of 24
-// heads of 192, bf16, 64 of them rotated as interleaved pairs: 32 us, 4.7 TB/s of 151 MB (pair by pair: 86 us); threads for
-// whole turns of a token's vectors, not for the next power of two: 40 us before that.
+// from L1 for all its heads; where alignment or an odd width forbids that, it goes two elements at a time. 8191 tokens of 24
+// heads of 192, bf16, 64 of them rotated as interleaved pairs: 32 us, 4.7 TB/s of 151 MB (a warp to a head, pair by
+// pair: 86 us); threads for the next power of two of a token's vectors: 40 us. 4960 tokens of 29 heads of 110, f16, 66 of them
+// rotated as half pairs: 31 us (a warp to a head 47).
 #include <math.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -28,40 +31,77 @@ struct RopeArgs {
     bool            half, inverse, in_place;
 };
 
-// one warp per (token, head), a lane per pair
-template <int T> __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs a) {
-    using E            = typename io<T>::t;
-    const int     lane = threadIdx.x & 31;
-    const int64_t item = (int64_t) blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (item >= a.n_tok * a.n_heads) {
+// Units of two elements, the rotated pairs and then the pairs that are copied. threadIdx.x runs over a token's units (head by
+// head), threadIdx.y over the block's tokens. WIDE: two neighbours are one aligned word.
+template <int T, bool HALF, bool WIDE> __global__ void __launch_bounds__(256) rope_pair_kernel(const RopeArgs a, uint32_t units,
+                                                                                                uint32_t magic) {
+    using E         = typename io<T>::t;
+    constexpr int U = 4;
+    const int64_t t = (int64_t) blockIdx.x * blockDim.y + threadIdx.y;
+    if (t >= a.n_tok) {
         return;
     }
-    const int64_t t = item / a.n_heads;
-    const int     h = (int) (item - t * a.n_heads);
-    const E *     x = reinterpret_cast<const E *>(a.src) + t * a.sts + h * a.shs;
-    E *           y = reinterpret_cast<E *>(a.dst) + t * a.dts + h * a.dhs;
-    const int     p = __ldg(a.pos + t);
-    if (p < 0 || p >= a.max_pos) {
-        if (lane == 0 && a.err) {
-            atomicOr(a.err, ACB_DEVERR_POS_RANGE);
-        }
-        for (int i = lane; i < a.D; i += 32) {
-            y[i] = io<T>::from_f(0.0f);
-        }
-        return;
+    const int  p   = __ldg(a.pos + t);
+    const bool bad = p < 0 || p >= a.max_pos;
+    if (bad && threadIdx.x == 0 && a.err) {
+        atomicOr(a.err, ACB_DEVERR_POS_RANGE);
     }
-    const float * w = a.table + (int64_t) p * a.R;
-    for (int i = lane; i < a.R / 2; i += 32) {
-        const float c  = __ldg(w + 2 * i);
-        const float s  = a.inverse ? -__ldg(w + 2 * i + 1) : __ldg(w + 2 * i + 1);
-        const int   ia = a.half ? i : 2 * i, ib = a.half ? i + a.R / 2 : 2 * i + 1;
-        const float u = io<T>::to_f(x[ia]), v = io<T>::to_f(x[ib]);
-        y[ia] = io<T>::from_f(__fsub_rn(__fmul_rn(u, c), __fmul_rn(v, s)));
-        y[ib] = io<T>::from_f(__fadd_rn(__fmul_rn(u, s), __fmul_rn(v, c)));
-    }
-    if (!a.in_place) {
-        for (int i = a.R + lane; i < a.D; i += 32) {
-            y[i] = x[i];
+    const float *  w = a.table + (int64_t) (bad ? 0 : p) * a.R;
+    const E *      x = reinterpret_cast<const E *>(a.src) + t * a.sts;
+    E *            y = reinterpret_cast<E *>(a.dst) + t * a.dts;
+    const uint32_t n = (uint32_t) a.n_heads * units;
+    const int      rot = a.R / 2;
+    union Two {
+        E e[2];
+        typename std::conditional<sizeof(E) == 2, uint32_t, uint2>::type word;
+    };
+    for (uint32_t i0 = threadIdx.x; i0 < n; i0 += U * blockDim.x) {
+        Two      v[U];
+        uint32_t h[U];
+        int      u[U];
+#pragma unroll
+        for (int k = 0; k < U; k++) {  // all loads before any store
+            const uint32_t i = i0 + k * blockDim.x;
+            if (i < n) {
+                h[k] = units == 1 ? i : __umulhi(i, magic);
+                u[k] = (int) (i - h[k] * units);
+                const E * q = x + (int64_t) h[k] * a.shs;
+                if (HALF && u[k] < rot) {
+                    v[k].e[0] = q[u[k]];
+                    v[k].e[1] = q[u[k] + rot];
+                } else if (WIDE) {
+                    v[k].word = *reinterpret_cast<const decltype(v[k].word) *>(q + 2 * u[k]);
+                } else {
+                    v[k].e[0] = q[2 * u[k]];
+                    v[k].e[1] = q[2 * u[k] + 1];
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            if (i0 + k * blockDim.x >= n) {
+                break;
+            }
+            E * q = y + (int64_t) h[k] * a.dhs;
+            if (bad) {
+                v[k].e[0] = v[k].e[1] = io<T>::from_f(0.0f);
+            } else if (u[k] < rot) {
+                const float c = __ldg(w + 2 * u[k]), s0 = __ldg(w + 2 * u[k] + 1), s = a.inverse ? -s0 : s0;
+                const float f = io<T>::to_f(v[k].e[0]), g = io<T>::to_f(v[k].e[1]);
+                v[k].e[0]     = io<T>::from_f(__fsub_rn(__fmul_rn(f, c), __fmul_rn(g, s)));
+                v[k].e[1]     = io<T>::from_f(__fadd_rn(__fmul_rn(f, s), __fmul_rn(g, c)));
+            } else if (a.in_place) {
+                continue;
+            }
+            if (HALF && u[k] < rot) {
+                q[u[k]]       = v[k].e[0];
+                q[u[k] + rot] = v[k].e[1];
+            } else if (WIDE) {
+                *reinterpret_cast<decltype(v[k].word) *>(q + 2 * u[k]) = v[k].word;
+            } else {
+                q[2 * u[k]]     = v[k].e[0];
+                q[2 * u[k] + 1] = v[k].e[1];
+            }
         }
     }
 }
@@ -148,31 +188,38 @@ bool rope_vector(const RopeArgs & a, int type) {
     const int64_t v = 16 / type_size(type);
     const int64_t r = a.half ? a.R / 2 : a.R;
     return (reinterpret_cast<uintptr_t>(a.src) | reinterpret_cast<uintptr_t>(a.dst) | reinterpret_cast<uintptr_t>(a.table)) % 16 == 0 &&
-           (a.sts | a.shs | a.dts | a.dhs) % v == 0 && a.D % v == 0 && r % v == 0 && a.R % 4 == 0 && a.n_heads <= 4096;
+           (a.sts | a.shs | a.dts | a.dhs) % v == 0 && a.D % v == 0 && r % v == 0 && a.R % 4 == 0;
 }
 
 template <int T> void rope_launch(const RopeArgs & a, cudaStream_t st) {
-    if (!rope_vector(a, T)) {
-        rope_kernel<T><<<(unsigned) ((a.n_tok * a.n_heads + 7) / 8), 256, 0, st>>>(a);
-        return;
-    }
     constexpr int  V     = vec16<T>::N;
+    const bool     vec   = rope_vector(a, T);
     const uint32_t rot   = (uint32_t) (a.half ? a.R / 2 : a.R) / V;
-    const uint32_t units = rot + (uint32_t) (a.D - a.R) / V;
+    const uint32_t units = vec ? rot + (uint32_t) (a.D - a.R) / V : (uint32_t) a.D / 2;
     const uint32_t n     = (uint32_t) a.n_heads * units;
-    // i / units as the high word of i * magic: exact while i * units < 2^32 (4096 heads of at most 256 units)
+    // i / units as the high word of i * magic: exact while i * units < 2^32 (2^14 heads of at most 2^9 units)
     const uint32_t magic = units == 1 ? 0 : (uint32_t) ((0x100000000ull + units - 1) / units);
-    // each thread takes two units a time, as few idle as whole warps allow; what a small token leaves of 256 threads takes
-    // further tokens
-    const uint32_t turns = (n + 511) / 512;
-    const uint32_t bx    = ((n + 2 * turns - 1) / (2 * turns) + 31) / 32 * 32;
+    // each thread takes two vectors or four pairs a turn, as few idle as whole warps allow; what a small token leaves of 256
+    // threads takes further tokens
+    const uint32_t each  = vec ? 2 : 4;
+    const uint32_t turns = (n + 256 * each - 1) / (256 * each);
+    const uint32_t bx    = ((n + each * turns - 1) / (each * turns) + 31) / 32 * 32;
     const dim3     block(bx, 256 / bx);
     const unsigned grid = (unsigned) ((a.n_tok + block.y - 1) / block.y);
-    if (a.half) {
-        rope_vec_kernel<T, true><<<grid, block, 0, st>>>(a, rot, units, magic);
-    } else {
-        rope_vec_kernel<T, false><<<grid, block, 0, st>>>(a, rot, units, magic);
+    if (vec) {
+        if (a.half) {
+            rope_vec_kernel<T, true><<<grid, block, 0, st>>>(a, rot, units, magic);
+        } else {
+            rope_vec_kernel<T, false><<<grid, block, 0, st>>>(a, rot, units, magic);
+        }
+        return;
     }
+    const int64_t two  = 2 * type_size(T);
+    const bool    wide = (reinterpret_cast<uintptr_t>(a.src) | reinterpret_cast<uintptr_t>(a.dst)) % two == 0 &&
+                      (a.sts | a.shs | a.dts | a.dhs) % 2 == 0;
+    const auto kern = a.half ? (wide ? rope_pair_kernel<T, true, true> : rope_pair_kernel<T, true, false>)
+                             : (wide ? rope_pair_kernel<T, false, true> : rope_pair_kernel<T, false, false>);
+    kern<<<grid, block, 0, st>>>(a, units, magic);
 }
 
 }  // namespace
@@ -201,7 +248,7 @@ extern "C" acb_status acb_rope(const void * src, int64_t src_tok_stride, int64_t
     if ((n_in > 1 && inner < head_dim) || (n_out > 1 && outer < (n_in > 1 ? (n_in - 1) * inner : 0) + head_dim)) {
         return ACB_ERR_INVALID_ARG;
     }
-    if (!is_io_type(type) || head_dim > 1024 || n_tok > (int64_t) INT32_MAX * 8 / n_heads) {
+    if (!is_io_type(type) || head_dim > 1024 || n_heads > 16384 || n_tok > (int64_t) INT32_MAX) {
         return ACB_ERR_UNSUPPORTED;
     }
     if (n_tok == 0) {

@@ -709,7 +709,7 @@ ACB_API acb_status acb_rope_table_scaled_host(float * table, int max_pos, int ro
  * the layout and (c, s) = rope_table[pos[t]][2i..2i+1], a' = a c - b s, b' = a s + b c in f32, each product and sum
  * rounded, then rounded to the type of src and dst (F32, F16 or BF16, the same for both). Element (t, h, d) is
  * src[t*src_tok_stride + h*src_head_stride + d], dst likewise; dst is src itself (the same pointer and strides) or apart
- * from it. head_dim even, at most 1024; rope_dim even, in [2, head_dim]. rope_table [max_pos][rope_dim] on the device. A
+ * from it. head_dim even, at most 1024; n_heads at most 16384; rope_dim even, in [2, head_dim]. rope_table [max_pos][rope_dim] on the device. A
  * position outside [0, max_pos) flags ACB_DEVERR_POS_RANGE and its rows are written as zeros. acb_qk_norm_rope is the
  * whole-head NeoX form with the norm in front. */
 ACB_API acb_status acb_rope(const void * src, int64_t src_tok_stride, int64_t src_head_stride, void * dst,

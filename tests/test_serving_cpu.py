@@ -93,7 +93,7 @@ def rope(src=P, sts=128, shs=64, dst=P, dts=128, dhs=64, type=acb.F32, n_tok=2, 
                                        (dict(max_pos=0), 1), (dict(dts=256), 1), (dict(shs=0, dhs=0), 1),
                                        (dict(sts=64, dts=64), 1), (dict(dst=P + 64, dhs=32), 1),
                                        (dict(type=acb.Q8_0), 2), (dict(D=1026, R=2, sts=4096, dts=4096, shs=2048, dhs=2048), 2),
-                                       (dict(n_tok=1 << 40), 2)])
+                                       (dict(n_tok=1 << 40), 2), (dict(n_heads=16385, sts=1 << 21, dts=1 << 21), 2)])
 def test_rope_refusals(kw, status):
     assert rope(**kw) == status
 
