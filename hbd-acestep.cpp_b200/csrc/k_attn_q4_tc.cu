@@ -30,11 +30,12 @@ namespace acb {
 namespace {
 
 constexpr int   kQtRows    = 128;  // of a tile
-constexpr int   kQtKeys    = 128;
+constexpr int   kQtKeys    = 128;  // of a block; scores come 64 keys at a time
+constexpr int   kQtHalf    = kQtKeys / 2;
 constexpr int   kQtSoft    = 8;   // softmax warps
 constexpr int   kQtUnpack  = 4;   // unpacking warps
-constexpr int   kQtMma     = kQtSoft + kQtUnpack;  // 13 warps: up to 16 leave every thread 128 registers
-constexpr int   kQtThreads = 32 * (kQtMma + 1);
+constexpr int   kQtMma     = kQtSoft + kQtUnpack;  // and the next: 14 warps, up to 16 leave every thread 128 registers
+constexpr int   kQtThreads = 32 * (kQtMma + 2);
 constexpr float kQtLag     = 8.0f;  // the reference maximum moves when exceeded by more than 2^kQtLag
 constexpr float kQtLift    = 6.0f;  // P is held times 2^kQtLift: at most 2^14
 constexpr int   kQtRing    = 8;     // blocks whose notes are kept
@@ -42,7 +43,7 @@ constexpr int   kQtRing    = 8;     // blocks whose notes are kept
 template <int D> struct QtLayout {
     static constexpr int QB = kQtRows * D * 2, KB = kQtKeys * D * 2, VB = kQtKeys * D * 2, NK = 2, NV = 2;
     static constexpr int TOTAL = 2 * QB + NK * KB + NV * VB;
-    // TMEM columns: S/P of the tiles at 0 and 128, O at 256 and 384
+    // TMEM columns: S/P of a tile's halves of a block at 128 t and 128 t + 64, O at 256 and 384
 };
 
 // two f32 in one operation (sm_100)
@@ -88,6 +89,40 @@ __device__ __forceinline__ void tmem_arrived(uint32_t * r) {
     }
 }
 
+// The products' warp runs as one, with everything in uniform registers, and one lane of it issues. A thread alone between
+// branches spends more time on moving descriptors and looking at barriers than the tensor cores on the products.
+constexpr uint32_t kQtDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // smem_desc_sw128's upper word
+
+__device__ __forceinline__ void issue_ss(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 da, {%2, %6};\n\tmov.b64 db, {%3, %6};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%1], da, db, %4, p;\n\t}" ::"r"(leader),
+        "r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "r"(kQtDescHi));
+}
+
+__device__ __forceinline__ void issue_ts(uint32_t leader, uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\tsetp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 db, {%3, %6};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], db, %4, p;\n\t}" ::"r"(leader),
+        "r"(d), "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(acc), "r"(kQtDescHi));
+}
+
+__device__ __forceinline__ void issue_commit(uint32_t leader, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}" ::"r"(leader),
+        "r"(bar)
+        : "memory");
+}
+
+// of a warp; what is there already costs one look
+__device__ __forceinline__ bool warp_wait(uint64_t * bar, uint32_t parity, volatile int * abort_flag, int * err) {
+    return __all_sync(0xffffffffu, ptx::mbar_try_wait(bar, parity)) ||
+           __all_sync(0xffffffffu, tc_wait(bar, parity, abort_flag, err));
+}
+
 template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThreads, 1) attn_q4_tc_kernel(const AttnQ4Args a) {
     using Lay = QtLayout<D>;
     using T1  = typename io<T>::t;
@@ -100,10 +135,10 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
     uint64_t * k_empty = k_full + Lay::NK;
     uint64_t * v_full  = k_empty + Lay::NK;
     uint64_t * v_empty = v_full + Lay::NV;
-    uint64_t * s_full  = v_empty + Lay::NV;  // [2], of the tiles: S(i) is there, and P.V(i - 1) done
-    uint64_t * p_full  = s_full + 2;         // [2]
-    uint64_t * o_done  = p_full + 2;         // [2]
-    uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(o_done + 2);
+    // [2 t + h], tile t and half h of a block. Phase i of s_full: S(i, h) is there, and P.V(i - 1, h) done
+    uint64_t * s_full  = v_empty + Lay::NV;
+    uint64_t * p_full  = s_full + 4;
+    uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(p_full + 4);
     __shared__ volatile int abort_flag;
     // notes on a block, for what hardly ever happens: keys whose page is not in the pool, and per 32 dimensions the keys whose
     // value scale is no number (their values are left out of the product, where 0 * NaN would reach the rows that do not see
@@ -136,16 +171,15 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
         ptx::mbar_init(q_full, kQtSoft / 2 * tiles);
         for (int i = 0; i < Lay::NK; i++) {
             ptx::mbar_init(&k_full[i], kQtUnpack);
-            ptx::mbar_init(&k_empty[i], 1);
+            ptx::mbar_init(&k_empty[i], tiles);
         }
         for (int i = 0; i < Lay::NV; i++) {
             ptx::mbar_init(&v_full[i], kQtUnpack);
-            ptx::mbar_init(&v_empty[i], 1);
+            ptx::mbar_init(&v_empty[i], tiles);
         }
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < 4; i++) {
             ptx::mbar_init(&s_full[i], 1);
             ptx::mbar_init(&p_full[i], kQtSoft / 2);
-            ptx::mbar_init(&o_done[i], 1);
         }
         ptx::fence_mbar_init();
     }
@@ -205,7 +239,7 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
                 kpg = a.kv.page_of(s, min(key0 + kQtKeys + tid, p1));
                 vpg = a.kv.page_of(s, min(key0 + kQtKeys + 8 * kg, p1));
             }
-            if (!__all_sync(0xffffffffu, i < Lay::NK || tc_wait(&k_empty[sk], (i / Lay::NK - 1) & 1, &abort_flag, a.err))) {
+            if (i >= Lay::NK && !warp_wait(&k_empty[sk], (i / Lay::NK - 1) & 1, &abort_flag, a.err)) {
                 break;
             }
             // Room for the notes of block i + 2, where those of block i - 6 are: both tiles' S(i - 2) are done, so both softmaxes
@@ -251,7 +285,7 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
             if (lane == 0) {
                 ptx::mbar_arrive(&k_full[sk]);
             }
-            if (!__all_sync(0xffffffffu, i < Lay::NV || tc_wait(&v_empty[sv], (i / Lay::NV - 1) & 1, &abort_flag, a.err))) {
+            if (i >= Lay::NV && !warp_wait(&v_empty[sv], (i / Lay::NV - 1) & 1, &abort_flag, a.err)) {
                 break;
             }
             if (on) {
@@ -298,60 +332,68 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
                 ptx::mbar_arrive(&v_full[sv]);
             }
         }
-    } else if (warp == kQtMma) {
-        if (lane == 0 && nblk > 0 && tc_wait(q_full, 0, &abort_flag, a.err)) {
+    } else if (warp >= kQtMma) {
+        // ---- products of tile t ----
+        const int      n_blk = __reduce_max_sync(0xffffffffu, warp - kQtMma < tiles ? nblk : 0);
+        const int      t     = __reduce_max_sync(0xffffffffu, warp - kQtMma);
+        const uint32_t tm    = __reduce_max_sync(0xffffffffu, tmem) + (uint32_t) (t * 128);
+        const uint32_t base  = __reduce_max_sync(0xffffffffu, ptx::smem_u32(sQ)) >> 4;  // addresses of descriptors
+        const uint32_t bar_s = __reduce_max_sync(0xffffffffu, ptx::smem_u32(s_full + 2 * t));
+        const uint32_t leader = lane == 0;
+        if (n_blk > 0 && warp_wait(q_full, 0, &abort_flag, a.err)) {
             tc_fence_after();
-            constexpr uint32_t idesc_s = idesc_kind_f16(128, kQtKeys, true);
+            constexpr uint32_t idesc_s = idesc_kind_f16(128, kQtHalf, true);
             constexpr uint32_t idesc_o = idesc_kind_f16(128, D, true);
-            auto issue_s = [&](int t, int i) {
-                const uint32_t q = ptx::smem_u32(sQ + t * Lay::QB), k = ptx::smem_u32(sK + (i % Lay::NK) * Lay::KB);
+            auto issue_s = [&](int i, int h) {
+                const uint32_t q = base + (uint32_t) t * (Lay::QB / 16);
+                const uint32_t k = base + (uint32_t) (2 * Lay::QB + (i % Lay::NK) * Lay::KB + h * kQtHalf * 128) / 16;
 #pragma unroll
                 for (int kk = 0; kk < D / 16; kk++) {
-                    const uint32_t off = (uint32_t) ((kk >> 2) * 16384 + (kk & 3) * 32);
-                    umma_f16kind(tmem + (uint32_t) (t * 128), smem_desc_sw128(q + off), smem_desc_sw128(k + off), idesc_s, kk > 0);
+                    const uint32_t off = (uint32_t) ((kk >> 2) * 16384 + (kk & 3) * 32) / 16;
+                    issue_ss(leader, tm + (uint32_t) (h * kQtHalf), q + off, k + off, idesc_s, kk > 0);
                 }
-                umma_commit(&s_full[t]);
+                issue_commit(leader, bar_s + (uint32_t) h * 8);
             };
-            auto issue_pv = [&](int t, int i) {
-                const uint32_t v = ptx::smem_u32(sV + (i % Lay::NV) * Lay::VB);
+            auto issue_pv = [&](int i, int h) {
+                const uint32_t v = base + (uint32_t) (2 * Lay::QB + Lay::NK * Lay::KB + (i % Lay::NV) * Lay::VB + h * D * 128) / 16;
 #pragma unroll
-                for (int kk = 0; kk < kQtKeys / 16; kk++) {
-                    umma_ts(tmem + (uint32_t) (256 + t * 128), tmem + (uint32_t) (t * 128 + kk * 8),
-                            smem_desc_sw128(v + (kk >> 2) * (D * 128) + (kk & 3) * 32), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+                for (int kk = 0; kk < kQtHalf / 16; kk++) {
+                    issue_ts(leader, tm + 256, tm + (uint32_t) (h * kQtHalf + kk * 8), v + kk * 2, idesc_o,
+                             (i > 0 || h > 0 || kk > 0) ? 1u : 0u);
                 }
             };
-            bool ok = tc_wait(&k_full[0], 0, &abort_flag, a.err);
+            bool ok = warp_wait(&k_full[0], 0, &abort_flag, a.err);
             if (ok) {
                 tc_fence_after();
-                for (int t = 0; t < tiles; t++) {
-                    issue_s(t, 0);
-                }
-                umma_commit(&k_empty[0]);
+                issue_s(0, 0);
+                issue_s(0, 1);
+                issue_commit(leader, ptx::smem_u32(&k_empty[0]));
             }
-            for (int i = 0; ok && i < nblk; i++) {
-                const bool more = i + 1 < nblk;
-                for (int t = 0; ok && t < tiles; t++) {
-                    ok = tc_wait(&p_full[t], i & 1, &abort_flag, a.err) &&
-                         (t > 0 || tc_wait(&v_full[i % Lay::NV], (i / Lay::NV) & 1, &abort_flag, a.err));
+            for (int i = 0; ok && i < n_blk; i++) {
+                const bool more = i + 1 < n_blk;
+                ok = warp_wait(&v_full[i % Lay::NV], (i / Lay::NV) & 1, &abort_flag, a.err);
+#pragma unroll 1
+                for (int h = 0; ok && h < 2; h++) {
+                    ok = warp_wait(&p_full[2 * t + h], i & 1, &abort_flag, a.err);
                     if (!ok) {
                         break;
                     }
                     tc_fence_after();
-                    issue_pv(t, i);
+                    issue_pv(i, h);
                     if (!more) {
-                        umma_commit(&o_done[t]);
+                        issue_commit(leader, bar_s + (uint32_t) h * 8);
                         continue;
                     }
-                    ok = t > 0 || tc_wait(&k_full[(i + 1) % Lay::NK], ((i + 1) / Lay::NK) & 1, &abort_flag, a.err);
+                    ok = h > 0 || warp_wait(&k_full[(i + 1) % Lay::NK], ((i + 1) / Lay::NK) & 1, &abort_flag, a.err);
                     if (ok) {
                         tc_fence_after();
-                        issue_s(t, i + 1);
+                        issue_s(i + 1, h);
                     }
                 }
                 if (ok) {
-                    umma_commit(&v_empty[i % Lay::NV]);
+                    issue_commit(leader, ptx::smem_u32(&v_empty[i % Lay::NV]));
                     if (more) {
-                        umma_commit(&k_empty[(i + 1) % Lay::NK]);
+                        issue_commit(leader, ptx::smem_u32(&k_empty[(i + 1) % Lay::NK]));
                     }
                 }
             }
@@ -439,56 +481,42 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
                 }
             }
         };
-        for (int i = 0; i < nblk; i++) {
-            ok = __all_sync(0xffffffffu, tc_wait(&s_full[t], i & 1, &abort_flag, a.err));
+        for (int j = 0; j < 2 * nblk; j++) {
+            const int i = j >> 1, h = j & 1;
+            ok = warp_wait(&s_full[2 * t + h], i & 1, &abort_flag, a.err);
             if (!ok) {
                 break;
             }
             tc_fence_after();
-            if (i > 0) {
+            const uint32_t tH = tS + (uint32_t) (h * kQtHalf);
+            uint32_t       xa[32], xb[32];
+            tmem_ld32_start(tH, xa);
+            tmem_ld32_start(tH + 32, xb);
+            if (h == 0 && i > 0) {
                 look_at_values(i - 1);
             }
-            const int key0 = (kb_lo + i) * kQtKeys;
-            // bit c of see[w]: key key0 + 32 w + c is seen; looked at only where one is not
-            uint32_t   see[4];
-            const bool part = __any_sync(0xffffffffu, key0 + kQtKeys - 1 > p || key0 < lo || bad_any[i % kQtRing][0]);
+            const int  key0 = (kb_lo + i) * kQtKeys + h * kQtHalf;
+            const bool part = __any_sync(0xffffffffu, key0 + kQtHalf - 1 > p || key0 < lo || bad_any[i % kQtRing][0]);
+            tmem_arrived(xa);
+            tmem_arrived(xb);
             if (part) {
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    const int k = key0 + 32 * w;
-                    see[w]      = p < k ? 0u : p >= k + 31 ? ~0u : (2u << (p - k)) - 1u;
-                    see[w] &= lo <= k ? ~0u : lo > k + 31 ? 0u : ~0u << (lo - k);
-                    see[w] &= ~bad_key[i % kQtRing][w];
-                }
-            }
-            // Rolled loops of 32 keys: the code of the four kinds of warps does not fit the instruction caches unrolled
-            uint32_t xa[32], xb[32];
-            auto     hide = [&](uint32_t * x, uint32_t bits) {
-                if (part) {
+                auto hide = [&](uint32_t * x, int w) {  // bit c of see: key k + c is seen
+                    const int k   = key0 + 32 * w;
+                    uint32_t  see = p < k ? 0u : p >= k + 31 ? ~0u : (2u << (p - k)) - 1u;
+                    see &= lo <= k ? ~0u : lo > k + 31 ? 0u : ~0u << (lo - k);
+                    see &= ~bad_key[i % kQtRing][2 * h + w];
 #pragma unroll
                     for (int c = 0; c < 32; c++) {
-                        x[c] = (bits >> c) & 1u ? x[c] : 0xFF800000u;
+                        x[c] = (see >> c) & 1u ? x[c] : 0xFF800000u;
                     }
-                }
-            };
+                };
+                hide(xa, 0);
+                hide(xb, 1);
+            }
             float g[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
-            auto  top  = [&](const uint32_t * x) {
 #pragma unroll
-                for (int c = 0; c < 32; c += 2) {
-                    g[(c >> 1) & 3] = fmaxf(g[(c >> 1) & 3], fmaxf(__uint_as_float(x[c]), __uint_as_float(x[c + 1])));
-                }
-            };
-            tmem_ld32_start(tS, xa);
-#pragma unroll 1
-            for (int w = 0; w < 4; w += 2) {
-                tmem_arrived(xa);
-                tmem_ld32_start(tS + (uint32_t) (32 * w + 32), xb);
-                hide(xa, w == 0 ? see[0] : see[2]);
-                top(xa);
-                tmem_arrived(xb);
-                tmem_ld32_start(tS + (uint32_t) (w == 0 ? 64 : 0), xa);  // the last: the first again, for its exponentials
-                hide(xb, w == 0 ? see[1] : see[3]);
-                top(xb);
+            for (int c = 0; c < 32; c++) {
+                g[c & 3] = fmaxf(g[c & 3], fmaxf(__uint_as_float(xa[c]), __uint_as_float(xb[c])));
             }
             const float mb   = fmaxf(fmaxf(g[0], g[1]), fmaxf(g[2], g[3])) * sc;
             bool        resc = false;
@@ -514,22 +542,18 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
                     ps[e & 1] = add2(ps[e & 1], pack2(e0, e1));
                     ph[e]     = u32_of(__floats2half2_rn(e0, e1));
                 }
-                tmem_st16(tS + (uint32_t) (16 * w), ph);  // over scores that have been read (chunk w / 2)
+                tmem_st16(tH + (uint32_t) (16 * w), ph);  // over the scores, which are all here
             };
-#pragma unroll 1
-            for (int w = 0; w < 4; w += 2) {
-                tmem_arrived(xa);
-                tmem_ld32_start(tS + (uint32_t) (32 * w + 32), xb);
-                hide(xa, w == 0 ? see[0] : see[2]);
-                weigh(xa, w);  // columns 16 w.., of chunk w / 2 = w - w / 2: read, and not the one on its way
-                tmem_arrived(xb);
-                if (w == 0) {
-                    tmem_ld32_start(tS + 64, xa);
+            weigh(xa, 0);
+            weigh(xb, 1);
+            if (__any_sync(0xffffffffu, resc)) {
+                // O is whole once P.V of the half before is done: the other half's next phase (of S of the half after, or of the end)
+                ok = j == 0 || warp_wait(&s_full[2 * t + (h ^ 1)], ((j + 1) >> 1) & 1, &abort_flag, a.err);
+                if (!ok) {
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    break;
                 }
-                hide(xb, w == 0 ? see[1] : see[3]);
-                weigh(xb, w + 1);
-            }
-            if (__any_sync(0xffffffffu, resc)) {  // P.V(i - 1) is done: O is whole
+                tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < D / 32; c++) {
                     uint32_t o[32];
@@ -549,11 +573,11 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                ptx::mbar_arrive(&p_full[t]);
+                ptx::mbar_arrive(&p_full[2 * t + h]);
             }
         }
         if (ok && nblk > 0) {
-            ok = __all_sync(0xffffffffu, tc_wait(&o_done[t], 0, &abort_flag, a.err));
+            ok = warp_wait(&s_full[2 * t], nblk & 1, &abort_flag, a.err) && warp_wait(&s_full[2 * t + 1], nblk & 1, &abort_flag, a.err);
             tc_fence_after();
             if (ok) {
                 look_at_values(nblk - 1);
