@@ -1,25 +1,28 @@
 // k_attn_q4_tc.cu -- attention over the paged 4-bit KV cache for chunks of prompts, on the 5th-generation tensor cores.
 //
 // One CTA per 256 rows (new token * G + query head of the group) of a sequence and kv head, in two tiles of 128; key blocks of
-// 128. Every cached value is an f16 number, so nothing is rounded on the way into the tiles. 13 warps (16 and fewer leave a
+// 128. Every cached value is an f16 number, so nothing is rounded on the way into the tiles. 14 warps (16 and fewer leave a
 // thread 128 registers):
-//   0..3, 4..7  softmax of tile 0 and of tile 1, a thread a row (a TMEM lane): 32 scores at a time, the next on their way, once
-//               for the maximum and once for the exponentials; P goes back over them as f16. (Two threads a row with both
-//               halves of one tile in registers, and the exchange that takes, held the tensor cores at 20%: 462 us where this
-//               takes 303; all eight warps on one tile at a time 376 us.)
+//   0..3, 4..7  softmax of tile 0 and of tile 1, a thread a row (a TMEM lane): 64 scores of half a block at a time, in registers
+//               once for the maximum and the exponentials; P goes back over them as f16;
 //   8..11       unpacking. K: a thread a key; the 8 dimensions of a word of codes make one 16-byte unit in the order that
 //               unpack4 gives them, and Q is written in the same order (a product does not depend on the order of its k
 //               index). V^T: a thread 8 keys by 16 dimensions: the words of two keys are merged by halves, so that unpack4
 //               gives pairs of keys, and four pairs make the 16-byte unit of a dimension;
-//   12          one thread issues the products: S = Q K^T from shared memory, O += P V with P from TMEM. P.V of a tile is
-//               followed by its next S, which may then take P's place; meanwhile the other tile's softmax runs.
-// Per key block and tile the tensor cores need 1024 cycles (D = 128) and so do the exponentials; shared memory moves 128 bytes a
-// cycle during Q K^T. The unpacking is shared by the tiles.
+//   12, 13      the products of tile 0 and of tile 1: S = Q K^T of 64 keys from shared memory, O += P V with P from TMEM. The two
+//               halves of a block have score columns of their own, so that while the softmax is at one the other's next scores
+//               are computed: a softmax never waits for its own product.
+// Per key block and tile the tensor cores need 1280 cycles (D = 128; products of 64 columns are bound by shared memory, 48
+// cycles where 32 would do) and the exponentials 1024.
 //
-// 4 sequences with 1200-2048 new rows over 2048-5000 keys (16/8 heads of 128, bf16): 303 us, 585 TFLOP/s; the tensor cores
-// are 32% busy. A tile's turn is its bound: softmax 3000 cycles (maximum 950, exponentials 1900), products 1200, signals 700,
-// of which the other tile's turn covers a part; P.V by halves as P comes (342 us), seven warps that unpack K or V as it
-// falls (366) and unrolled loops of 64 scores (310, instruction fetch) were slower.
+// 4 sequences with 1200-2048 new rows over 2048-5000 keys (16/8 heads of 128, bf16): 248 us, 714 TFLOP/s; a block takes 4400
+// cycles, all of which both softmaxes are at work (wait and load 550, maximum 220, exponentials 1000-1400, signals 150 of a
+// half), as is the unpacking; issue is 52% busy, the exponentials' unit 46%, and the last blocks of the grid leave 16% of
+// the SMs idle. Slower were: scores of whole blocks, whose turn waits for the products (303 us); one warp for both tiles'
+// products (295, and 393 by a thread behind branches instead of a warp in uniform registers); teams of four warps for K and for V
+// with the registers split by setmaxnreg (254); the next half's scores on their way under the exponentials (269); weights
+// taken before the maximum is known and repeated where it moves (260); loads of codes along the rows (250, a quarter of the
+// cache traffic); two threads a row (462), eight warps on one tile (376), the products issued by softmax warps (363).
 //
 // Every wait is bounded, as in k_attn_tc.cu.
 #include "attn_q4.cuh"
@@ -69,24 +72,25 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 
-// 32 columns of this warp's lanes on their way into r, which must not be looked at before tmem_arrived(r)
-__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t * r) {
+// 64 columns of this warp's lanes. Load and wait are one statement: nothing can move or copy r in between, and the pairs stay
+// where two-element operations want them.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t * r) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%1"
-        "7,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-}
-
-__device__ __forceinline__ void tmem_arrived(uint32_t * r) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; i++) {
-        asm volatile("" : "+r"(r[i]));  // no use of it moves in front of the wait
-    }
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+          "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+          "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+          "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        : "r"(taddr)
+        : "memory");
 }
 
 // The products' warp runs as one, with everything in uniform registers, and one lane of it issues. A thread alone between
@@ -489,34 +493,30 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
             }
             tc_fence_after();
             const uint32_t tH = tS + (uint32_t) (h * kQtHalf);
-            uint32_t       xa[32], xb[32];
-            tmem_ld32_start(tH, xa);
-            tmem_ld32_start(tH + 32, xb);
             if (h == 0 && i > 0) {
                 look_at_values(i - 1);
             }
             const int  key0 = (kb_lo + i) * kQtKeys + h * kQtHalf;
             const bool part = __any_sync(0xffffffffu, key0 + kQtHalf - 1 > p || key0 < lo || bad_any[i % kQtRing][0]);
-            tmem_arrived(xa);
-            tmem_arrived(xb);
+            uint32_t   x[kQtHalf];
+            tmem_ld64(tH, x);
             if (part) {
-                auto hide = [&](uint32_t * x, int w) {  // bit c of see: key k + c is seen
+#pragma unroll
+                for (int w = 0; w < 2; w++) {  // bit c of see: key k + c is seen
                     const int k   = key0 + 32 * w;
                     uint32_t  see = p < k ? 0u : p >= k + 31 ? ~0u : (2u << (p - k)) - 1u;
                     see &= lo <= k ? ~0u : lo > k + 31 ? 0u : ~0u << (lo - k);
                     see &= ~bad_key[i % kQtRing][2 * h + w];
 #pragma unroll
                     for (int c = 0; c < 32; c++) {
-                        x[c] = (see >> c) & 1u ? x[c] : 0xFF800000u;
+                        x[32 * w + c] = (see >> c) & 1u ? x[32 * w + c] : 0xFF800000u;
                     }
-                };
-                hide(xa, 0);
-                hide(xb, 1);
+                }
             }
             float g[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
 #pragma unroll
-            for (int c = 0; c < 32; c++) {
-                g[c & 3] = fmaxf(g[c & 3], fmaxf(__uint_as_float(xa[c]), __uint_as_float(xb[c])));
+            for (int c = 0; c < kQtHalf; c += 2) {
+                g[(c >> 1) & 3] = fmaxf(g[(c >> 1) & 3], fmaxf(__uint_as_float(x[c]), __uint_as_float(x[c + 1])));
             }
             const float mb   = fmaxf(fmaxf(g[0], g[1]), fmaxf(g[2], g[3])) * sc;
             bool        resc = false;
@@ -531,21 +531,20 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
             const float nm    = m == -INFINITY ? 0.0f : kQtLift - m;
             const uint64_t sc2 = pack2(sc, sc), nm2 = pack2(nm, nm);
             uint64_t       ps[2] = { 0, 0 };  // sums of weights, two each
-            auto weigh = [&](const uint32_t * x, int w) {
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
                 uint32_t ph[16];
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     float e0, e1;
-                    unpack2(fma2(pack2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), sc2, nm2), &e0, &e1);
+                    unpack2(fma2(pack2(__uint_as_float(x[32 * w + 2 * e]), __uint_as_float(x[32 * w + 2 * e + 1])), sc2, nm2), &e0, &e1);
                     e0        = ex2_fast(e0);
                     e1        = ex2_fast(e1);
                     ps[e & 1] = add2(ps[e & 1], pack2(e0, e1));
                     ph[e]     = u32_of(__floats2half2_rn(e0, e1));
                 }
                 tmem_st16(tH + (uint32_t) (16 * w), ph);  // over the scores, which are all here
-            };
-            weigh(xa, 0);
-            weigh(xb, 1);
+            }
             if (__any_sync(0xffffffffu, resc)) {
                 // O is whole once P.V of the half before is done: the other half's next phase (of S of the half after, or of the end)
                 ok = j == 0 || warp_wait(&s_full[2 * t + (h ^ 1)], ((j + 1) >> 1) & 1, &abort_flag, a.err);
