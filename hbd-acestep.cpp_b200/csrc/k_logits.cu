@@ -3,9 +3,12 @@
 //
 // A block owns a slice of one row. It notes in shared memory what the history and the bias list say of its columns, streams the
 // slice through (as it is, or -inf where the mask is closed), and then changes the few columns that were noted, a thread each.
-// The row's bytes bound it. The history is read once by every block of its row, so there are only as many slices as fill
-// the GPU: cut into 19 slices a row, the histories of 128 rows of 151936 were over half of the work: 49-62 us in four forms against
-// the slices' 36 (2.9 TB/s of the row's bytes; without rules the same stream takes 26).
+// The row's bytes bound it. f32 rows are written 32 bytes a thread at once: in two stores of 16, each half of a sector, the plain
+// stream of 128 rows of 151936 (bf16 to f32) takes 26 us, in one 18.7 (6.2 TB/s). The history is read once by every block of
+// its row, so there are only as many slices as fill the GPU: cut into 19 slices a row, the histories of 128 rows were over
+// half of the work (49-62 us in four forms). With all rules and histories of up to 4100 tokens the slices take 28.4 us: four
+// warps note beside the stream, and the noted columns follow it. All warps streaming once they have noted gave nothing (30), nor
+// did a second kernel that notes while the first streams (40).
 //
 // A column's word holds the last bias entry of the column (its number + 1 above kBiasBit, by a maximum), whether the prompt
 // has it, and how often the answer does: whole numbers, so the order of the atomics does not show. The words are found by
@@ -24,6 +27,27 @@ constexpr int      kBiasBit   = 21;
 constexpr uint32_t kInPrompt  = 1u << 20;
 constexpr uint32_t kCountMask = kInPrompt - 1;  // histories and bias lists are limited to what the fields hold
 constexpr uint32_t kNoColumn  = 0xFFFFFFFFu;
+
+// 8 elements of a row, whole sectors at once where they are 32 bytes on their boundary
+template <int T> __device__ __forceinline__ void store8(typename io<T>::t * y, const float * v, bool wide) {
+    if constexpr (T == ACB_TYPE_F32) {
+        if (wide) {
+            asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(y), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+                         "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                         : "memory");
+            return;
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 8 / vec16<T>::N; q++) {
+        vec16<T> out;
+#pragma unroll
+        for (int e = 0; e < vec16<T>::N; e++) {
+            out.set(e, v[q * vec16<T>::N + e]);
+        }
+        out.store(y + q * vec16<T>::N);
+    }
+}
 
 struct RulesArgs {
     const void *    x;
@@ -88,6 +112,45 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_rules_kernel(const RulesA
         }
         return &words[k - k0];
     };
+    // Of U tokens at once (none where v < 0), by whole warps: what each would wait for, all wait for together, and the slots
+    // that are new cost a warp one addition. One after the other, four warps took 20 us for 4100 tokens.
+    constexpr int U = 8;
+    auto words_of = [&](const int * v, uint32_t ** w) {
+        uint32_t k[U], s[U], old[U], fresh[U];
+        int      n_fresh = 0, to = 0;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            bad |= v[u] >= a.V;
+            const int64_t at = v[u] - c0;
+            k[u]             = v[u] >= 0 && at >= 0 && at < n ? (uint32_t) at : kNoColumn;
+            s[u]             = (k[u] * 2654435761u) >> a.shift;
+            old[u]           = k[u] == kNoColumn ? k[u] : atomicCAS(&words[s[u]], kNoColumn, k[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            while (k[u] != kNoColumn && old[u] != kNoColumn && old[u] != k[u]) {
+                s[u]   = (s[u] + 1) & (a.slots - 1);
+                old[u] = atomicCAS(&words[s[u]], kNoColumn, k[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            fresh[u] = __ballot_sync(0xffffffffu, k[u] != kNoColumn && old[u] == kNoColumn);
+            n_fresh += __popc(fresh[u]);
+        }
+        if ((tid & 31) == 0) {
+            to = atomicAdd(&n_taken, n_fresh);
+        }
+        to = __shfl_sync(0xffffffffu, to, 0);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if ((fresh[u] >> (tid & 31)) & 1u) {
+                taken[to + __popc(fresh[u] & ((1u << (tid & 31)) - 1))] = (uint16_t) s[u];
+            }
+            to += __popc(fresh[u]);
+            w[u] = k[u] == kNoColumn ? nullptr : &words[a.slots + s[u]];
+        }
+    };
     const int  nt   = a.noters;
     auto       sync = [&] { asm volatile("bar.sync 1, %0;" ::"r"(nt) : "memory"); };
     auto       note = [&](int k0, int k1) {  // called by the first nt threads
@@ -100,6 +163,44 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_rules_kernel(const RulesA
             *reinterpret_cast<uint4 *>(words + i) = make_uint4(z, z, z, z);
         }
         sync();
+        if (HASH && nt < kLThreads) {
+            int        v[U];
+            uint32_t * w[U];
+            auto       take = [&](const int32_t * list, int i, int m) {
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    v[u] = i + u * nt < m ? __ldg(list + i + u * nt) : -1;
+                }
+            };
+            for (int i0 = 0; i0 < n_bias; i0 += U * nt) {
+                take(bids, i0 + tid, n_bias);
+                words_of(v, w);
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (w[u]) {
+                        atomicMax(w[u], (uint32_t) (i0 + tid + u * nt + 1) << kBiasBit);
+                    }
+                }
+            }
+            if (n_bias > 0) {
+                sync();
+            }
+            for (int i0 = 0; i0 < len; i0 += U * nt) {
+                take(hist, i0 + tid, len);
+                words_of(v, w);
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (w[u]) {
+                        if (i0 + tid + u * nt < np) {
+                            atomicOr(w[u], kInPrompt);
+                        } else {
+                            atomicAdd(w[u], 1u);
+                        }
+                    }
+                }
+            }
+            return;
+        }
         for (int i = tid; i < n_bias; i += nt) {
             if (uint32_t * w = word_of(__ldg(bids + i), k0, k1)) {
                 atomicMax(w, (uint32_t) (i + 1) << kBiasBit);
@@ -108,7 +209,6 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_rules_kernel(const RulesA
         if (n_bias > 0) {
             sync();  // a maximum of whole words: before anything is counted in them
         }
-        constexpr int U = 8;
         for (int i0 = tid; i0 < len; i0 += U * nt) {
             int v[U];
 #pragma unroll
@@ -145,7 +245,6 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_rules_kernel(const RulesA
     };
     // m words found by at(i, &column), i of this thread's share: logits and masks of several at once, since each comes from far
     auto change = [&](int m, auto at) {
-        constexpr int U = 8;
         for (int i0 = tid; i0 < m; i0 += U * kLThreads) {
             int      k[U];
             uint32_t w[U], open[U];
@@ -177,7 +276,8 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_rules_kernel(const RulesA
     const int  sts   = HASH && use && nt < kLThreads ? kLThreads - nt : kLThreads;
     if (st < 0) {
     } else if constexpr (VEC) {
-        constexpr int U = 4, NI = 8 / vec16<TI>::N, NO = 8 / vec16<TO>::N;
+        const bool    wide = (reinterpret_cast<uintptr_t>(a.y) | (uintptr_t) a.ldo * sizeof(EO)) % 32 == 0;  // slices begin on 256 columns
+        constexpr int U = 4, NI = 8 / vec16<TI>::N;
         for (int k0 = st * 8; k0 < n; k0 += U * sts * 8) {
             vec16<TI> in[U][NI];
             uint32_t  open[U];
@@ -196,17 +296,12 @@ __global__ void __launch_bounds__(kLThreads, 2) logits_rules_kernel(const RulesA
             for (int u = 0; u < U; u++) {
                 const int k = k0 + u * sts * 8;
                 if (k < n) {
+                    float v[8];
 #pragma unroll
-                    for (int q = 0; q < NO; q++) {
-                        vec16<TO> out;
-#pragma unroll
-                        for (int e = 0; e < vec16<TO>::N; e++) {
-                            const int   j = q * vec16<TO>::N + e;
-                            const float v = in[u][j / vec16<TI>::N].get(j % vec16<TI>::N);
-                            out.set(e, (open[u] >> j) & 1u ? v : -INFINITY);
-                        }
-                        out.store(y + k + q * vec16<TO>::N);
+                    for (int j = 0; j < 8; j++) {
+                        v[j] = (open[u] >> j) & 1u ? in[u][j / vec16<TI>::N].get(j % vec16<TI>::N) : -INFINITY;
                     }
+                    store8<TO>(y + k, v, wide);
                 }
             }
         }

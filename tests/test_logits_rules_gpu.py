@@ -182,3 +182,30 @@ def test_streams_graph_and_repeats(cuda):
         y = acb.logits_rules(x, hist, lens, freq=f)
     s.synchronize()
     assert torch.equal(y, ref)
+
+
+@pytest.mark.parametrize("V,L,B,pad", [(40008, 4000, 2000, 0), (40001, 4100, 7, 0), (40008, 1, 1, 4), (33000, 2500, 0, 8)])
+def test_long_slices_of_many_rows(cuda, V, L, B, pad):
+    """Enough rows that a block has tens of thousands of columns and few of its warps look at the history; with pad 4 the
+    output's rows lie 16 but not 32 bytes apart from a boundary."""
+    import torch
+    rng = np.random.default_rng(V + L)
+    R = 128
+    x = torch.from_numpy((rng.standard_normal((R, V)) * 4).astype(np.float32)).to(torch.bfloat16)
+    hist = rng.integers(-1, V, (R, L)).astype(np.int32)
+    hist[:, ::5] = rng.integers(V // 2, V // 2 + 600, hist[:, ::5].shape)  # often named, next to one another
+    lens, prompt = rng.integers(0, L + 1, R).astype(np.int32), rng.integers(0, L + 1, R).astype(np.int32)
+    lens[:2] = L
+    rep, freq, pres = (rng.uniform(a, b, R).astype(np.float32) for a, b in ((0.7, 1.6), (-0.5, 0.9), (-1, 1)))
+    bias = [rng.integers(-1, V, (R, B)).astype(np.int32), rng.standard_normal((R, B)).astype(np.float32)] if B else None
+    bits = rng.random((2, V)) < 0.6
+    mrow = rng.integers(-1, 2, R).astype(np.int32)
+    c = lambda a: torch.from_numpy(a).cuda()  # noqa: E731
+    out = torch.full((R, V + pad), 7.0).cuda()
+    err = torch.zeros(1, dtype=torch.int32).cuda()
+    acb.logits_rules(x.cuda(), c(hist), c(lens), c(prompt), c(rep), c(freq), c(pres), c(bias[0]) if B else None,
+                     c(bias[1]) if B else None, _words(bits), c(mrow), out=out[:, :V], err=err)
+    assert int(err) == 0 and (out[:, V:] == 7).all()
+    some = [0, 1, 50, R - 1]
+    _check(out[some, :V].cpu().numpy().astype(np.float64), x[some].float().numpy(), len(some), "f32", hist[some], lens[some], prompt[some],
+           rep[some], freq[some], pres[some], [b[some] for b in bias] if B else None, bits, mrow[some])
