@@ -1,28 +1,31 @@
 // k_attn_q4_tc.cu -- attention over the paged 4-bit KV cache for chunks of prompts, on the 5th-generation tensor cores.
 //
 // One CTA per 256 rows (new token * G + query head of the group) of a sequence and kv head, in two tiles of 128; key blocks of
-// 128. Every cached value is an f16 number, so nothing is rounded on the way into the tiles. 14 warps (16 and fewer leave a
-// thread 128 registers):
+// 128. Every cached value is an f16 number, so nothing is rounded on the way into the tiles. 16 warps, the most that leave a
+// thread 128 registers:
 //   0..3, 4..7  softmax of tile 0 and of tile 1, a thread a row (a TMEM lane): 64 scores of half a block at a time, in registers
 //               once for the maximum and the exponentials; P goes back over them as f16;
-//   8..11       unpacking. K: a thread a key; the 8 dimensions of a word of codes make one 16-byte unit in the order that
-//               unpack4 gives them, and Q is written in the same order (a product does not depend on the order of its k
-//               index). V^T: a thread 8 keys by 16 dimensions: the words of two keys are merged by halves, so that unpack4
+//   8..11       unpacking V^T: a thread 8 keys by 16 dimensions: the words of two keys are merged by halves, so that unpack4
 //               gives pairs of keys, and four pairs make the 16-byte unit of a dimension;
-//   12, 13      the products of tile 0 and of tile 1: S = Q K^T of 64 keys from shared memory, O += P V with P from TMEM. The two
+//   12, 13      unpacking K: a thread two keys; the 8 dimensions of a word of codes make one 16-byte unit in the order that
+//               unpack4 gives them, and Q is written in the same order (a product does not depend on the order of its k
+//               index);
+//   14, 15      the products of tile 0 and of tile 1: S = Q K^T of 64 keys from shared memory, O += P V with P from TMEM. The two
 //               halves of a block have score columns of their own, so that while the softmax is at one the other's next scores
 //               are computed: a softmax never waits for its own product.
 // Per key block and tile the tensor cores need 1280 cycles (D = 128; products of 64 columns are bound by shared memory, 48
 // cycles where 32 would do) and the exponentials 1024.
 //
-// 4 sequences with 1200-2048 new rows over 2048-5000 keys (16/8 heads of 128, bf16): 248 us, 714 TFLOP/s; a block takes 4400
-// cycles, all of which both softmaxes are at work (wait and load 550, maximum 220, exponentials 1000-1400, signals 150 of a
-// half), as is the unpacking; issue is 52% busy, the exponentials' unit 46%, and the last blocks of the grid leave 16% of
-// the SMs idle. Slower were: scores of whole blocks, whose turn waits for the products (303 us); one warp for both tiles'
-// products (295, and 393 by a thread behind branches instead of a warp in uniform registers); teams of four warps for K and for V
-// with the registers split by setmaxnreg (254); the next half's scores on their way under the exponentials (269); weights
-// taken before the maximum is known and repeated where it moves (260); loads of codes along the rows (250, a quarter of the
-// cache traffic); two threads a row (462), eight warps on one tile (376), the products issued by softmax warps (363).
+// 4 sequences with 1200-2048 new rows over 2048-5000 keys (16/8 heads of 128, bf16): 244 us, 726 TFLOP/s. A block takes about
+// 4300 cycles, all of which both softmaxes are at work (of a half: wait and load 550, maximum 220, exponentials 1000-1400, signals
+// 150). No part bounds it alone: with four unpacking warps (248 us), taking out the exponentials left 243, the products 239,
+// three quarters of the unpacking 222, the last and either of the others 200; issue is 52% busy, and the last blocks of the
+// grid leave 16% of the SMs idle. Slower were: scores of whole blocks, whose turn waits for the products (303 us); one warp for
+// both tiles' products (295, and 393 by a thread behind branches instead of a warp in uniform registers); four warps each
+// for K and for V with the registers split by setmaxnreg (254); the next half's scores on their way under the
+// exponentials (269); weights taken before the maximum is known and repeated where it moves (260), or with their sum
+// in the maximum's place (256); loads of codes along the rows (a quarter of the cache traffic, 250); every sequence's own last
+// rows first (251); two threads a row (462), eight warps on one tile (376), the products issued by softmax warps (363).
 //
 // Every wait is bounded, as in k_attn_tc.cu.
 #include "attn_q4.cuh"
@@ -36,8 +39,8 @@ constexpr int   kQtRows    = 128;  // of a tile
 constexpr int   kQtKeys    = 128;  // of a block; scores come 64 keys at a time
 constexpr int   kQtHalf    = kQtKeys / 2;
 constexpr int   kQtSoft    = 8;   // softmax warps
-constexpr int   kQtUnpack  = 4;   // unpacking warps
-constexpr int   kQtMma     = kQtSoft + kQtUnpack;  // and the next: 14 warps, up to 16 leave every thread 128 registers
+constexpr int   kQtUnpackV = 4, kQtUnpackK = 2;  // unpacking warps
+constexpr int   kQtMma     = kQtSoft + kQtUnpackV + kQtUnpackK;  // and the next: up to 16 warps leave every thread 128 registers
 constexpr int   kQtThreads = 32 * (kQtMma + 2);
 constexpr float kQtLag     = 8.0f;  // the reference maximum moves when exceeded by more than 2^kQtLag
 constexpr float kQtLift    = 6.0f;  // P is held times 2^kQtLift: at most 2^14
@@ -174,11 +177,11 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
         abort_flag = 0;
         ptx::mbar_init(q_full, kQtSoft / 2 * tiles);
         for (int i = 0; i < Lay::NK; i++) {
-            ptx::mbar_init(&k_full[i], kQtUnpack);
+            ptx::mbar_init(&k_full[i], kQtUnpackK);
             ptx::mbar_init(&k_empty[i], tiles);
         }
         for (int i = 0; i < Lay::NV; i++) {
-            ptx::mbar_init(&v_full[i], kQtUnpack);
+            ptx::mbar_init(&v_full[i], kQtUnpackV);
             ptx::mbar_init(&v_empty[i], tiles);
         }
         for (int i = 0; i < 4; i++) {
@@ -207,133 +210,157 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
     const uint32_t tmem = *tmem_slot;
 
     if (warp >= kQtSoft && warp < kQtMma) {
-        // ---- unpacking: four warps, K and then V of each block ----
-        const int  tid = threadIdx.x & (32 * kQtUnpack - 1);  // 0..127: this thread's key of K
-        // V: 8 keys from 8 kg on (of one page: pages hold 16 or more), 16 dimensions: the 8 bytes from 8 wq on; the lanes of a
-        // store phase differ in kg
-        const int  kg = (tid & 7) | ((tid >> 6) << 3), wq = (tid >> 3) & 7;
-        const bool on = D == 128 || wq < 4;  // heads of 64 have 4 such runs
-        int        kpg = nblk > 0 ? a.kv.page_of(s, min(kb_lo * kQtKeys + tid, p1)) : 0;
-        int        vpg = nblk > 0 ? a.kv.page_of(s, min(kb_lo * kQtKeys + 8 * kg, p1)) : 0;
-        for (int i = 0; i < nblk; i++) {
-            const int  key0 = (kb_lo + i) * kQtKeys, note = i % kQtRing, next = (i + 2) % kQtRing;
-            const int  sk = i % Lay::NK, sv = i % Lay::NV;
-            const bool gone = key0 + tid > p1, k_bad = kpg < 0;
-            // everything from memory is under way before the first wait
-            const int64_t krow = k_bad ? 0 : a.kv.row(kpg, hk, min(key0 + tid, p1));
-            const uint4 * kc   = reinterpret_cast<const uint4 *>(a.kv.kc + krow * (D / 2));
-            uint4         code = __ldg(kc);
-            Words<D / 64> ksw;
-            ksw.load(a.kv.ks + krow * (D / 32));
-            uint2         vw[8];
-            uint16_t      vs[8];
-            if (on) {
-                const int        j   = key0 + 8 * kg;
-                const int64_t    row = vpg < 0 ? 0 : a.kv.row(vpg, hk, j);
-                const uint8_t *  c   = a.kv.vc + row * (D / 2) + wq * 8;
-                const uint16_t * d   = a.kv.vs + row * (D / 32) + (wq >> 1);
-                const int        in  = vpg < 0 ? 0 : p1 - j + 1;  // keys past the last one: none of their own
+        if (warp >= kQtSoft + kQtUnpackV) {
+            // ---- unpacking K: a thread two keys ----
+            const int tid = threadIdx.x - 32 * (kQtSoft + kQtUnpackV);
+            int       kpg[2] = { 0, 0 };
+            if (nblk > 0) {
+                kpg[0] = a.kv.page_of(s, min(kb_lo * kQtKeys + tid, p1));
+                kpg[1] = a.kv.page_of(s, min(kb_lo * kQtKeys + tid + 64, p1));
+            }
+            for (int i = 0; i < nblk; i++) {
+                const int     key0 = (kb_lo + i) * kQtKeys, note = i % kQtRing, next = (i + 2) % kQtRing, sk = i % Lay::NK;
+                // from memory before the wait
+                const uint4 * kc[2];
+                uint4         code[2];
+                Words<D / 64> ksw[2];
+                bool          bad[2];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    vw[e] = e < in ? __ldg(reinterpret_cast<const uint2 *>(c + e * (D / 2))) : make_uint2(0, 0);
-                    vs[e] = e < in ? __ldg(d + e * (D / 32)) : (uint16_t) 0;
+                for (int e = 0; e < 2; e++) {
+                    const int     key  = key0 + tid + 64 * e;
+                    const int64_t krow = kpg[e] < 0 ? 0 : a.kv.row(kpg[e], hk, min(key, p1));
+                    bad[e]  = kpg[e] < 0;
+                    kc[e]   = reinterpret_cast<const uint4 *>(a.kv.kc + krow * (D / 2));
+                    code[e] = __ldg(kc[e]);
+                    ksw[e].load(a.kv.ks + krow * (D / 32));
+                    if (i + 1 < nblk) {
+                        kpg[e] = a.kv.page_of(s, min(key + kQtKeys, p1));
+                    }
                 }
-            }
-            if (i + 1 < nblk) {
-                kpg = a.kv.page_of(s, min(key0 + kQtKeys + tid, p1));
-                vpg = a.kv.page_of(s, min(key0 + kQtKeys + 8 * kg, p1));
-            }
-            if (i >= Lay::NK && !warp_wait(&k_empty[sk], (i / Lay::NK - 1) & 1, &abort_flag, a.err)) {
-                break;
-            }
-            // Room for the notes of block i + 2, where those of block i - 6 are: both tiles' S(i - 2) are done, so both softmaxes
-            // are past block i - 3, and no warp is at block i + 2 before this one has filled block i.
-            if (tid < 4) {
-                bad_key[next][tid] = 0;
-            } else if (tid < 6) {
-                bad_any[next][tid - 4] = 0;
-            } else if (tid >= 32 && tid < 32 + (D / 32) * 4) {
-                (&bad_val[next][0][0])[tid - 32] = 0;
-            }
-            if (k_bad && !gone) {
-                atomicOr(&bad_key[note][tid >> 5], 1u << (tid & 31));
-                bad_any[note][0] = 1;
-                if (a.err) {
-                    atomicOr(a.err, ACB_DEVERR_PAGE_RANGE);
+                if (i >= Lay::NK && !warp_wait(&k_empty[sk], (i / Lay::NK - 1) & 1, &abort_flag, a.err)) {
+                    break;
                 }
-            }
-            uint8_t * dst  = sK + sk * Lay::KB + tid * 128;
-            uint64_t  sc64 = k_bad || gone ? 0 : D == 64 ? ksw.w[0] : (uint64_t) ksw.w[D / 64 - 1] << 32 | ksw.w[0];
-#pragma unroll 1
-            for (int b = 0; b < D / 32; b++) {  // four words, four 16-byte units
-                const uint4   w4 = code;
-                const __half2 sc = __half2half2(__ushort_as_half((uint16_t) sc64));
-                if (b + 1 < D / 32) {
-                    code = __ldg(kc + b + 1);
+                // Room for the notes of block i + 2, where those of block i - 6 are: both tiles' S(i - 2) are done, so both
+                // softmaxes are past block i - 3, and no warp is at block i + 2 before this one has filled block i (V of block
+                // i + 2 takes the place of block i's, whose products come after).
+                if (tid < 4) {
+                    bad_key[next][tid] = 0;
+                } else if (tid < 6) {
+                    bad_any[next][tid - 4] = 0;
+                } else if (tid >= 32 && tid < 32 + (D / 32) * 4) {
+                    (&bad_val[next][0][0])[tid - 32] = 0;
                 }
-                sc64 >>= 16;
-                uint8_t * d = dst + (b >> 1) * 16384;
-                const int u = 4 * (b & 1), x = tid & 7;
-                uint32_t  r[4];
-                unpack4(w4.x, sc, r);
-                *reinterpret_cast<uint4 *>(d + ((u ^ x) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
-                unpack4(w4.y, sc, r);
-                *reinterpret_cast<uint4 *>(d + (((u + 1) ^ x) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
-                unpack4(w4.z, sc, r);
-                *reinterpret_cast<uint4 *>(d + (((u + 2) ^ x) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
-                unpack4(w4.w, sc, r);
-                *reinterpret_cast<uint4 *>(d + (((u + 3) ^ x) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                ptx::mbar_arrive(&k_full[sk]);
-            }
-            if (i >= Lay::NV && !warp_wait(&v_empty[sv], (i / Lay::NV - 1) & 1, &abort_flag, a.err)) {
-                break;
-            }
-            if (on) {
-                uint32_t sc[4], odd = 0;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    sc[e] = (uint32_t) vs[2 * e] | ((uint32_t) vs[2 * e + 1] << 16);
-                    // exponent field full: adding one unit carries into the sign's place
-                    odd |= ((sc[e] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
-                }
-                if (odd) {
-                    uint32_t bits = 0;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        if ((vs[e] & 0x7C00u) == 0x7C00u) {
-                            sc[e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-                            bits |= 1u << e;
+                for (int e = 0; e < 2; e++) {
+                    const int  key  = tid + 64 * e;
+                    const bool gone = key0 + key > p1;
+                    if (bad[e] && !gone) {
+                        atomicOr(&bad_key[note][key >> 5], 1u << (key & 31));
+                        bad_any[note][0] = 1;
+                        if (a.err) {
+                            atomicOr(a.err, ACB_DEVERR_PAGE_RANGE);
                         }
                     }
-                    atomicOr(&bad_val[note][wq >> 1][kg >> 2], bits << (8 * (kg & 3)));
-                    bad_any[note][1] = 1;
-                }
-                uint8_t * base = sV + sv * Lay::VB + (kg >> 3) * (D * 128);
+                    uint8_t * dst  = sK + sk * Lay::KB + key * 128;
+                    uint64_t  sc64 = bad[e] || gone ? 0 : D == 64 ? ksw[e].w[0] : (uint64_t) ksw[e].w[D / 64 - 1] << 32 | ksw[e].w[0];
 #pragma unroll 1
-                for (int h = 0; h < 4; h++) {  // bytes 2h and 2h + 1 of the 8
-                    uint32_t       r[4][4];    // [pair of keys][low, high of byte 2h, low, high of byte 2h + 1]
-                    const uint32_t sel = h & 1 ? 0x7632u : 0x5410u;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const uint32_t x = h < 2 ? vw[2 * e].x : vw[2 * e].y, y = h < 2 ? vw[2 * e + 1].x : vw[2 * e + 1].y;
-                        unpack4(__byte_perm(x, y, sel), half2_of(sc[e]), r[e]);
+                    for (int b = 0; b < D / 32; b++) {  // four words, four 16-byte units
+                        const uint4   w4 = code[e];
+                        const __half2 sc = __half2half2(__ushort_as_half((uint16_t) sc64));
+                        if (b + 1 < D / 32) {
+                            code[e] = __ldg(kc[e] + b + 1);
+                        }
+                        sc64 >>= 16;
+                        uint8_t * d = dst + (b >> 1) * 16384;
+                        const int u = 4 * (b & 1), x = tid & 7;
+                        uint32_t  r[4];
+                        unpack4(w4.x, sc, r);
+                        *reinterpret_cast<uint4 *>(d + ((u ^ x) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+                        unpack4(w4.y, sc, r);
+                        *reinterpret_cast<uint4 *>(d + (((u + 1) ^ x) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+                        unpack4(w4.z, sc, r);
+                        *reinterpret_cast<uint4 *>(d + (((u + 2) ^ x) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
+                        unpack4(w4.w, sc, r);
+                        *reinterpret_cast<uint4 *>(d + (((u + 3) ^ x) << 4)) = make_uint4(r[0], r[1], r[2], r[3]);
                     }
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const int d = (wq >> 1) * 32 + (wq & 1) * 8 + 2 * h + (q >> 1) + 16 * (q & 1);
-                        *reinterpret_cast<uint4 *>(base + d * 128 + (((kg & 7) ^ (2 * h + (q >> 1))) << 4)) =
-                            make_uint4(r[0][q], r[1][q], r[2][q], r[3][q]);
-                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::mbar_arrive(&k_full[sk]);
                 }
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                ptx::mbar_arrive(&v_full[sv]);
+        } else {
+            // ---- unpacking V: a thread 8 keys from 8 kg on (of one page: pages hold 16 or more), 16 dimensions: the 8 bytes from
+            // 8 wq on; the lanes of a store phase differ in kg ----
+            const int  tid = threadIdx.x & (32 * kQtUnpackV - 1), kg = (tid & 7) | ((tid >> 6) << 3), wq = (tid >> 3) & 7;
+            const bool on = D == 128 || wq < 4;  // heads of 64 have 4 such runs
+            int        vpg = nblk > 0 ? a.kv.page_of(s, min(kb_lo * kQtKeys + 8 * kg, p1)) : 0;
+            for (int i = 0; i < nblk; i++) {
+                const int key0 = (kb_lo + i) * kQtKeys, note = i % kQtRing, sv = i % Lay::NV;
+                uint2     vw[8];
+                uint16_t  vs[8];
+                if (on) {
+                    const int        j   = key0 + 8 * kg;
+                    const int64_t    row = vpg < 0 ? 0 : a.kv.row(vpg, hk, j);
+                    const uint8_t *  c   = a.kv.vc + row * (D / 2) + wq * 8;
+                    const uint16_t * d   = a.kv.vs + row * (D / 32) + (wq >> 1);
+                    const int        in  = vpg < 0 ? 0 : p1 - j + 1;  // keys past the last one: none of their own
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        vw[e] = e < in ? __ldg(reinterpret_cast<const uint2 *>(c + e * (D / 2))) : make_uint2(0, 0);
+                        vs[e] = e < in ? __ldg(d + e * (D / 32)) : (uint16_t) 0;
+                    }
+                }
+                if (i + 1 < nblk) {
+                    vpg = a.kv.page_of(s, min(key0 + kQtKeys + 8 * kg, p1));
+                }
+                if (i >= Lay::NV && !warp_wait(&v_empty[sv], (i / Lay::NV - 1) & 1, &abort_flag, a.err)) {
+                    break;
+                }
+                if (on) {
+                    uint32_t sc[4], odd = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        sc[e] = (uint32_t) vs[2 * e] | ((uint32_t) vs[2 * e + 1] << 16);
+                        // exponent field full: adding one unit carries into the sign's place
+                        odd |= ((sc[e] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+                    }
+                    if (odd) {
+                        uint32_t bits = 0;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            if ((vs[e] & 0x7C00u) == 0x7C00u) {
+                                sc[e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                                bits |= 1u << e;
+                            }
+                        }
+                        atomicOr(&bad_val[note][wq >> 1][kg >> 2], bits << (8 * (kg & 3)));
+                        bad_any[note][1] = 1;
+                    }
+                    uint8_t * base = sV + sv * Lay::VB + (kg >> 3) * (D * 128);
+#pragma unroll 1
+                    for (int h = 0; h < 4; h++) {  // bytes 2h and 2h + 1 of the 8
+                        uint32_t       r[4][4];    // [pair of keys][low, high of byte 2h, low, high of byte 2h + 1]
+                        const uint32_t sel = h & 1 ? 0x7632u : 0x5410u;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t x = h < 2 ? vw[2 * e].x : vw[2 * e].y, y = h < 2 ? vw[2 * e + 1].x : vw[2 * e + 1].y;
+                            unpack4(__byte_perm(x, y, sel), half2_of(sc[e]), r[e]);
+                        }
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const int d = (wq >> 1) * 32 + (wq & 1) * 8 + 2 * h + (q >> 1) + 16 * (q & 1);
+                            *reinterpret_cast<uint4 *>(base + d * 128 + (((kg & 7) ^ (2 * h + (q >> 1))) << 4)) =
+                                make_uint4(r[0][q], r[1][q], r[2][q], r[3][q]);
+                        }
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::mbar_arrive(&v_full[sv]);
+                }
             }
         }
     } else if (warp >= kQtMma) {
