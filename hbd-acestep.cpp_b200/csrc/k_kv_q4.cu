@@ -10,11 +10,12 @@
 // The bytes of q, k and v bound it. The fast form: a block per token, a thread 8 consecutive elements of a head, so that a
 // block of 32 is four lanes, a rotation's partner is in the thread (interleaved) or another lane's (half), and the angles of
 // a thread's elements serve every head that it takes. Rows that are not 16-byte aligned, or rotated widths that do not fall on
-// vectors, go a warp to a head through shared memory. 17002 tokens of 16 + 8 + 8 heads of 128, bf16, normed and rotated: 103 us,
-// 2.1 TB/s of 217 MB, and 23 us for reading the rows back as f16 (4.7 TB/s of 109 MB). Both together 126 us; a warp to a head
-// 330, codes by a division each 205, one loop over rows of all kinds 167, five blocks an SM instead of seven 152. 1100
-// instructions for the four rows of a warp hold the append there (issue slots 68% busy): the codes are 100 a row, the norm's
-// sum in double 60, the rotation's exchange 50.
+// vectors, go a warp to a head through shared memory. 17002 tokens of 16 + 8 + 8 heads of 128, bf16, normed and rotated: 89 us,
+// 2.4 TB/s of 217 MB, and 23 us for reading the rows back as f16 (4.7 TB/s of 109 MB). Both together 112 us; a warp to a head
+// 330, codes by a division each 205, one loop over rows of all kinds 167, four warps to every token 126, four rows a thread in
+// flight instead of two 136 (one: 116), room for 28 warps an SM 114 (the rotation spills), for 20 116. 1100
+// instructions for the four rows of a warp hold the append there: the codes are 100 a row, the norm's sum in double 60, the
+// rotation's exchange 50.
 #include "kv_q4.cuh"
 
 namespace acb {
@@ -194,12 +195,13 @@ template <int TI, int TQ, int D> __global__ void __launch_bounds__(256) kv_q4_ap
 
 // LPR lanes to a head's row; ROPE 0: none, 1: half pairs, 2: interleaved. The rows of q, k and v are gone through one kind
 // after the other, U rows a thread in flight, each kind's first rows loaded before anything else.
-constexpr int kAppendWarps = 4;
+constexpr int kAppendWarps = 4;  // of a block at most
+constexpr int kAppendRoom  = 24;  // warps of an SM
 
 template <int TI, int TQ, int D, int ROPE>
-__global__ void __launch_bounds__(32 * kAppendWarps, 7) kv_q4_append_vec_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(32 * kAppendWarps, kAppendRoom / kAppendWarps) kv_q4_append_vec_kernel(const AppendArgs a) {
     constexpr int LPR = D / 8, RPW = 32 / LPR, VI = vec16<TI>::N, VQ = vec16<TQ>::N, U = TI == ACB_TYPE_F32 ? 1 : 2;
-    constexpr int TURN = kAppendWarps * RPW;  // rows of one row a thread
+    const int     TURN = (int) (blockDim.x >> 5) * RPW;  // rows of one row a thread
     using EI           = typename io<TI>::t;
     const int64_t t    = blockIdx.x;
     const int     lane = threadIdx.x & 31, sub = lane % LPR, d0 = sub * 8;
@@ -550,7 +552,13 @@ extern "C" acb_status acb_kv_q4_append(const acb_kv_q4 * kv, const void * qkv, i
                       : type == ACB_TYPE_F16 ? append_kernel<ACB_TYPE_F16>(tq, D, rope)
                                              : append_kernel<ACB_TYPE_BF16>(tq, D, rope);
     if (vec) {
-        kern<<<(unsigned) n_tok, 32 * kAppendWarps, 0, (cudaStream_t) stream>>>(a);
+        // as many warps for a token as keep all tokens on the GPU at once: 8 tokens (16 + 8 + 8 heads of 128, bf16) take 4.2 us by
+        // 4 warps and 11.2 by one, 1184 take 9.7 by 2 (10.8, 13.4 by 4, 1), and 8192 take 47 by one and 54 by 4
+        int warps = kAppendWarps;
+        while (warps > 1 && n_tok * warps > (int64_t) kAppendRoom * num_sms()) {
+            warps /= 2;
+        }
+        kern<<<(unsigned) n_tok, 32 * warps, 0, (cudaStream_t) stream>>>(a);
     } else {
         kern<<<(unsigned) ((n_tok * nh + 7) / 8), 256, 0, (cudaStream_t) stream>>>(a);
     }
