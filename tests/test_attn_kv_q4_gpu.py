@@ -382,3 +382,68 @@ def test_wrappers_refuse_what_would_be_misread(cuda):
         cache.attention(torch.randn(2, 2, 64).cuda(), ln, max_kv_len=65)
     with pytest.raises(acb.AcbError):
         cache.attention(torch.randn(3, 2, 64).cuda(), ln)  # three rows, two sequences and no q_start
+
+
+@pytest.mark.parametrize("kind,D,G", [("bf16", 128, 1), ("f16", 128, 2), ("bf16", 64, 1), ("f32", 128, 1)])
+@pytest.mark.parametrize("n", [70, 300])
+def test_references_that_keep_moving(cuda, kind, D, G, n):
+    """Scores that rise by 60 along 2400 keys, in steps of one page: the reference moves in nearly every block, while products of
+    the blocks before are under way."""
+    import torch
+    rng = np.random.default_rng(D + n)
+    L = 2400
+    cache = _cache(rng, 1, L, 16, 1, D)
+    kc, ks = cache.tensors[0], cache.tensors[1]
+    kc.fill_(0xFF)  # code 15: +7
+    j = torch.arange(L).cuda()
+    d = ((j // 16 + 1).float() * 16 / L).bfloat16().half()
+    t = cache.tensors[4].long()[0]
+    ks[t[j // 16], 0, j % 16] = d[:, None].expand(L, D // 32).contiguous()
+    q = torch.full((n, G, D), 0.5).to(S.torch_type(kind)).cuda()
+    scale = 60 / (3.5 * D)
+    o = cache.attention(q, torch.tensor([L], dtype=torch.int32).cuda(), torch.tensor([0, n], dtype=torch.int32).cuda(), n, scale=scale)
+    _check(cache, q, o, [n], [L], 0, scale, kind)
+
+
+@pytest.mark.parametrize("kind,D", [("bf16", 128), ("f16", 64), ("f32", 128)])
+@pytest.mark.parametrize("window", [0, 900])
+def test_holes_and_nan_values_along_many_blocks(cuda, kind, D, window):
+    """Pages outside the pool and value scales that are NaN, in blocks far apart and next to each other, for 300 rows of two heads
+    over 2400 keys: the holes take no part, a NaN reaches the rows that see its key in its dimensions."""
+    import torch
+    rng = np.random.default_rng(D + window)
+    n, L, P, scale = 300, 2400, 16, 0.1
+    cache = _cache(rng, 1, L, P, 1, D)
+    k, v = _held(cache, 0, L)
+    k, v = k[:, 0], v[:, 0].copy()
+    holes = [1, 9, 76, 77, 90, 141, 149]  # pages
+    nans = [(1160, 0), (1250, 1), (1300, 0), (2200, 1), (2201, 0), (2350, 1)] if window else [(2150, 0), (2200, 1), (2201, 0), (2350, 1)]
+    t = cache.tensors[4][0]
+    for j, b in nans:
+        cache.tensors[3][int(t[j // P]), 0, j % P, b] = float("nan")
+        v[j, 32 * b:32 * b + 32] = 0
+    for i, pg in enumerate(holes):
+        t[pg] = 10 ** 6 if i % 2 else -1
+    q = torch.from_numpy(rng.standard_normal((n, 2, D)).astype(np.float32)).to(S.torch_type(kind)).cuda()
+    err = torch.zeros(1, dtype=torch.int32).cuda()
+    o = cache.attention(q, torch.tensor([L], dtype=torch.int32).cuda(), torch.tensor([0, n], dtype=torch.int32).cuda(), n, window=window,
+                        scale=scale, err=err).float().cpu().numpy().astype(np.float64)
+    assert int(err) == 16
+    key, pos = np.arange(L), L - n + np.arange(n)
+    seen = (key[None] <= pos[:, None]) & ~np.isin(key // P, holes)[None]
+    if window:
+        seen &= key[None] > pos[:, None] - window
+    nan = np.zeros((n, D), bool)
+    for j, b in nans:
+        nan[seen[:, j], 32 * b:32 * b + 32] = True
+    for h in range(2):
+        x = q[:, h].float().cpu().numpy().astype(np.float64)
+        s = np.where(seen, scale * (x @ k.T), -np.inf)
+        w = np.exp(s - s.max(1, keepdims=True))
+        w /= w.sum(1, keepdims=True)
+        ref, A = w @ v, w @ np.abs(v)
+        s1 = (scale * (np.abs(x) @ np.abs(k).T)).max(1)[:, None]
+        ds = (D + 4) * 2.0 ** -24 * s1 + (2.0 ** -21 * s1 if kind != "f32" else 0)
+        tol = A * (2 * ds + 2.0 ** -15 + (2.0 ** -11 if kind != "f32" else 0)) + 2.0 ** -31 * np.abs(v).sum(0)
+        tol = tol + S.HALF_STEP[kind] * (np.abs(ref) + tol) + (2.0 ** -25 if kind == "f16" else 0)
+        assert np.isnan(o[:, h][nan]).all() and (np.abs(o[:, h] - ref) <= tol)[~nan].all()

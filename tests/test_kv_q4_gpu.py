@@ -186,3 +186,29 @@ def test_offsets_past_32_bits(cuda):
     assert bool((cache.tensors[0][n_pages - 1, :, 4095] != 0).any()) and bool((cache.tensors[0][n_pages - 1, :, 17] != 0).any())
     o = cache.attention(x[:1, :2 * D].reshape(1, 2, D).cuda(), torch.tensor([18], dtype=torch.int32).cuda(), window=1)
     assert float((o[0].float() - v[2]).abs().max()) <= 2.0 ** -22 * float(v[2].abs().max())  # one key: its value
+
+
+@pytest.mark.parametrize("T", [700, 1500, 4000])
+@pytest.mark.parametrize("kind,D,layout,R", [("bf16", 128, "half", 128), ("f16", 64, "interleaved", 32), ("f32", 256, "half", 64)])
+def test_many_tokens(cuda, kind, D, layout, R, T):
+    """More tokens than the GPU holds with all their warps at once, with padding among them, next to the same tokens few at a time."""
+    import torch
+    rng = np.random.default_rng(T + D)
+    Nh, Nkv, page = 3, 2, 64
+    n_pages = -(-T // page)
+    table = torch.from_numpy(rng.permutation(n_pages).reshape(1, -1).astype(np.int32)).cuda()
+    x = torch.from_numpy(rng.standard_normal((T, (Nh + 2 * Nkv) * D)).astype(np.float32)).to(S.torch_type(kind)).cuda()
+    pos = torch.from_numpy(rng.permutation(T).astype(np.int32)).cuda()
+    seq = torch.from_numpy(np.where(rng.random(T) < 0.05, -1, 0).astype(np.int32)).cuda()
+    rope = acb.rope_table_scaled(T, R, 1e4).cuda()
+    w = torch.from_numpy((1 + 0.2 * rng.standard_normal(D)).astype(np.float32)).cuda()
+    all_at_once, few = (acb.KVCacheQ4.empty(n_pages, page, Nkv, D, table) for _ in range(2))
+    q = torch.zeros((T, Nh, D), dtype=x.dtype).cuda()
+    q2 = torch.zeros_like(q)
+    all_at_once.append(x, Nh, seq, pos, rope, layout, w, w, q_out=q)
+    for a in range(0, T, 100):
+        b = min(T, a + 100)
+        few.append(x[a:b], Nh, seq[a:b], pos[a:b], rope, layout, w, w, q_out=q2[a:b])
+    assert torch.equal(q, q2)
+    for s, t in zip(all_at_once.tensors[:4], few.tensors[:4]):
+        assert torch.equal(s, t)
