@@ -5,11 +5,12 @@
 // inverse): 6 flops on 2 elements against a read and a write of both, so the memory bounds it. The vector form takes 16
 // bytes at a time (with half pairs, 16 bytes of each half), a block one or more whole tokens, so that the angles of a token come
 // from L1 for all its heads; where alignment or an odd width forbids that, it goes two elements at a time. 8191 tokens of 24
-// heads of 192, bf16, 64 of them rotated as interleaved pairs: 32 us, 4.7 TB/s of 151 MB (a warp to a head, pair by
+// heads of 192, bf16, 64 of them rotated as interleaved pairs: 29.6 us, 5.1 TB/s of 151 MB (a warp to a head, pair by
 // pair: 86 us); threads for the next power of two of a token's vectors: 40 us. 4960 tokens of 29 heads of 110, f16, 66 of them
 // rotated as half pairs: 31 us (a warp to a head 47).
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "common.cuh"
@@ -199,12 +200,17 @@ template <int T> void rope_launch(const RopeArgs & a, cudaStream_t st) {
     const uint32_t n     = (uint32_t) a.n_heads * units;
     // i / units as the high word of i * magic: exact while i * units < 2^32 (2^14 heads of at most 2^9 units)
     const uint32_t magic = units == 1 ? 0 : (uint32_t) ((0x100000000ull + units - 1) / units);
-    // each thread takes two vectors or four pairs a turn, as few idle as whole warps allow; what a small token leaves of 256
-    // threads takes further tokens
+    // Blocks of 256 threads, of vectors smaller ones where there are more than fit at once: 8191 tokens (24 heads of 192, bf16)
+    // take 29.6 us in blocks of 64 and 32.3 in 256, 8 tokens (24 heads of 128, f32) 2.9 and 1.9. Each thread takes two vectors
+    // or four pairs a turn, as few idle as whole warps allow; what a small token leaves of a block takes further tokens.
+    uint32_t threads = 256;
+    while (vec && threads > 64 && a.n_tok * std::min(threads, n) > (int64_t) 1024 * num_sms()) {
+        threads /= 2;
+    }
     const uint32_t each  = vec ? 2 : 4;
-    const uint32_t turns = (n + 256 * each - 1) / (256 * each);
+    const uint32_t turns = (n + threads * each - 1) / (threads * each);
     const uint32_t bx    = ((n + each * turns - 1) / (each * turns) + 31) / 32 * 32;
-    const dim3     block(bx, 256 / bx);
+    const dim3     block(bx, threads / bx);
     const unsigned grid = (unsigned) ((a.n_tok + block.y - 1) / block.y);
     if (vec) {
         if (a.half) {

@@ -135,3 +135,19 @@ def test_streams_graphs_and_empty(cuda):
     torch.cuda.synchronize()
     assert torch.equal(out, acb.rope(x, pos, table))
     assert acb.rope(x[:0], pos[:0], table).shape == (0, 4, 128)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("T,H,D,R", [(3001, 24, 128, 64), (5003, 1, 64, 64), (1100, 9, 192, 16), (2500, 3, 50, 30)])
+def test_more_tokens_than_fit_at_once(cuda, kind, layout, T, H, D, R):
+    import torch
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(T, H, D, generator=g).to(S.torch_type(kind))
+    pos = torch.randint(0, 900, (T,), generator=g, dtype=torch.int32)
+    table = _table(900, R)
+    y = acb.rope(x.cuda(), pos.cuda(), table.cuda(), layout)
+    _check(y.float().cpu().numpy(), x.float().numpy(), pos.numpy(), table, layout, False, kind)
+    z = x.cuda()
+    acb.rope(z, pos.cuda(), table.cuda(), layout, out=z)
+    assert torch.equal(z, y)
