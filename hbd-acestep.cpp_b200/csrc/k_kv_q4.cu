@@ -409,15 +409,15 @@ __global__ void __launch_bounds__(256) kv_q4_read_kernel(const KvQ4 kv, const in
                                                          const int32_t * __restrict__ pos, int64_t n_tok, void * k_out,
                                                          void * v_out, int64_t stride, bool vec, int * err) {
     constexpr int IPR  = D / 16;  // items of a row
-    const int64_t item = (int64_t) blockIdx.x * 256 + threadIdx.x;
-    const int64_t rows = item / IPR;
-    const int     part = (int) (item % IPR), blk = part >> 1;
-    if (rows >= n_tok * 2 * kv.nkv) {
+    const uint32_t item = blockIdx.x * 256 + threadIdx.x;  // there are fewer than 2^31
+    const uint32_t rows = item / IPR, per = 2 * (uint32_t) kv.nkv;
+    const int      part = (int) (item % IPR), blk = part >> 1;
+    const int64_t  t    = rows / per;
+    if (t >= n_tok) {
         return;
     }
-    const int64_t t = rows / (2 * kv.nkv);
-    const int     r = (int) (rows - t * 2 * kv.nkv), h = r % kv.nkv;
-    const bool    is_v = r >= kv.nkv;
+    const int  r = (int) (rows % per), h = r < kv.nkv ? r : r - kv.nkv;
+    const bool is_v = r >= kv.nkv;
     void *        out  = is_v ? v_out : k_out;
     const int     s = __ldg(seq + t), p = __ldg(pos + t);
     if (s < 0 || !out) {
