@@ -16,6 +16,8 @@
 // flight instead of two 136 (one: 116), room for 28 warps an SM 114 (the rotation spills), for 20 116. 1100
 // instructions for the four rows of a warp hold the append there: the codes are 100 a row, the norm's sum in double 60, the
 // rotation's exchange 50.
+#include <algorithm>
+
 #include "kv_q4.cuh"
 
 namespace acb {
@@ -523,7 +525,7 @@ extern "C" acb_status acb_kv_q4_append(const acb_kv_q4 * kv, const void * qkv, i
                        (layout != ACB_ROPE_HALF && layout != ACB_ROPE_INTERLEAVED))) {
         return ACB_ERR_INVALID_ARG;
     }
-    if (!is_io_type(type) || (n_heads > 0 && !is_io_type(q_type)) || n_tok > (int64_t) INT32_MAX * 8 / nh) {
+    if (!is_io_type(type) || (n_heads > 0 && !is_io_type(q_type)) || n_tok > std::min((int64_t) INT32_MAX, (int64_t) INT32_MAX * 8 / nh)) {
         return ACB_ERR_UNSUPPORTED;
     }
     if (n_tok == 0) {

@@ -191,3 +191,7 @@ def test_workspaces_cover_every_smaller_call():
                 assert f(ref, n_seq * q, heads, q, n) <= full
         assert f(ref, n_seq, heads, 1, 100) == 0
         assert f(ref, 0, heads, 1, 60000) == 0 and f(ref, n_seq, heads, 0, 60000) == 0 and f(ref, n_seq, 3, 1, 60000) == 0
+
+
+def test_append_refuses_more_tokens_than_a_grid_has_blocks():
+    assert append(cache(), n_heads=0, n_tok=2 ** 31) == 2
