@@ -28,6 +28,8 @@
 // rows first (251); two threads a row (462), eight warps on one tile (376), the products issued by softmax warps (363).
 //
 // Every wait is bounded, as in k_attn_tc.cu.
+#include <algorithm>
+
 #include "attn_q4.cuh"
 #include "ptx.cuh"
 #include "tc.cuh"
@@ -657,9 +659,24 @@ template <int T, int D> void (*tc_kernel(bool aligned))(const AttnQ4Args) {
 
 }  // namespace
 
-// From 64 rows on (half a tile) the tiles of 128 win over tiles of 16 that unpack every key again.
+// Which form: here a block goes through all keys of up to 256 rows, 2.0 us for 128 keys, in as many waves as the blocks need; the
+// other form cuts the keys over the whole GPU, 70 ps for a key and tile of 16 rows (D = 128). So this one is faster from
+// some 180 such tiles of all sequences and kv heads for each wave on. Measured, here and there: 24 sequences of 3000 keys, 8 kv
+// heads, 16 rows each 115 us and 93, 32 rows 115 and 162; 4 of 4000, 64 rows 70 and 61, 128 rows 70 and 148; one of 20000,
+// 64 rows 314 and 65, 256 rows 360 and 200; 24 of 3000, 2 kv heads of 64, 48 rows 49 and 32, 64 rows 49 and 53. The rows are
+// taken as the sequences' mean. With few keys, or where the other form has no workspace to cut them, 64 rows are the border.
 bool attn_q4_tc_wanted(const AttnQ4Args & a, int type, int head_dim) {
-    return type != ACB_TYPE_F32 && head_dim <= 128 && (int64_t) a.max_q * a.G >= 64 && (int64_t) a.max_q * a.G <= 65535 * 2 * kQtRows;
+    const int64_t rows = (int64_t) a.max_q * a.G;
+    if (type == ACB_TYPE_F32 || head_dim > 128 || rows > 65535 * 2 * kQtRows) {
+        return false;
+    }
+    const int64_t keys = a.window > 0 ? std::min<int64_t>(a.max_kv, (int64_t) a.window + a.max_q) : a.max_kv;
+    if (rows >= 64 && (keys < 512 || a.n_split == 1)) {
+        return true;
+    }
+    const int64_t mean  = (a.n_tok * a.G + a.kv.n_seq - 1) / a.kv.n_seq, tasks = (int64_t) a.kv.n_seq * a.kv.nkv;
+    const int64_t waves = (tasks * ((mean + 2 * kQtRows - 1) / (2 * kQtRows)) + num_sms() - 1) / num_sms();
+    return keys >= 512 && tasks * ((mean + 15) / 16) >= 180 * waves;
 }
 
 acb_status attn_q4_tc_launch(const AttnQ4Args & a, int type, int head_dim, cudaStream_t st) {

@@ -401,8 +401,10 @@ def test_references_that_keep_moving(cuda, kind, D, G, n):
     ks[t[j // 16], 0, j % 16] = d[:, None].expand(L, D // 32).contiguous()
     q = torch.full((n, G, D), 0.5).to(S.torch_type(kind)).cuda()
     scale = 60 / (3.5 * D)
-    o = cache.attention(q, torch.tensor([L], dtype=torch.int32).cuda(), torch.tensor([0, n], dtype=torch.int32).cuda(), n, scale=scale)
-    _check(cache, q, o, [n], [L], 0, scale, kind)
+    for work in (None, torch.empty(1, dtype=torch.uint8).cuda()):  # the keys cut into chunks, and not
+        o = cache.attention(q, torch.tensor([L], dtype=torch.int32).cuda(), torch.tensor([0, n], dtype=torch.int32).cuda(), n, scale=scale,
+                            work=work)
+        _check(cache, q, o, [n], [L], 0, scale, kind)
 
 
 @pytest.mark.parametrize("kind,D", [("bf16", 128), ("f16", 64), ("f32", 128)])
@@ -425,25 +427,37 @@ def test_holes_and_nan_values_along_many_blocks(cuda, kind, D, window):
     for i, pg in enumerate(holes):
         t[pg] = 10 ** 6 if i % 2 else -1
     q = torch.from_numpy(rng.standard_normal((n, 2, D)).astype(np.float32)).to(S.torch_type(kind)).cuda()
-    err = torch.zeros(1, dtype=torch.int32).cuda()
-    o = cache.attention(q, torch.tensor([L], dtype=torch.int32).cuda(), torch.tensor([0, n], dtype=torch.int32).cuda(), n, window=window,
-                        scale=scale, err=err).float().cpu().numpy().astype(np.float64)
-    assert int(err) == 16
-    key, pos = np.arange(L), L - n + np.arange(n)
-    seen = (key[None] <= pos[:, None]) & ~np.isin(key // P, holes)[None]
-    if window:
-        seen &= key[None] > pos[:, None] - window
-    nan = np.zeros((n, D), bool)
-    for j, b in nans:
-        nan[seen[:, j], 32 * b:32 * b + 32] = True
-    for h in range(2):
-        x = q[:, h].float().cpu().numpy().astype(np.float64)
-        s = np.where(seen, scale * (x @ k.T), -np.inf)
-        w = np.exp(s - s.max(1, keepdims=True))
-        w /= w.sum(1, keepdims=True)
-        ref, A = w @ v, w @ np.abs(v)
-        s1 = (scale * (np.abs(x) @ np.abs(k).T)).max(1)[:, None]
-        ds = (D + 4) * 2.0 ** -24 * s1 + (2.0 ** -21 * s1 if kind != "f32" else 0)
-        tol = A * (2 * ds + 2.0 ** -15 + (2.0 ** -11 if kind != "f32" else 0)) + 2.0 ** -31 * np.abs(v).sum(0)
-        tol = tol + S.HALF_STEP[kind] * (np.abs(ref) + tol) + (2.0 ** -25 if kind == "f16" else 0)
-        assert np.isnan(o[:, h][nan]).all() and (np.abs(o[:, h] - ref) <= tol)[~nan].all()
+    for work in (None, torch.empty(1, dtype=torch.uint8).cuda()):  # the keys cut into chunks, and not
+        err = torch.zeros(1, dtype=torch.int32).cuda()
+        o = cache.attention(q, torch.tensor([L], dtype=torch.int32).cuda(), torch.tensor([0, n], dtype=torch.int32).cuda(), n, window=window,
+                            scale=scale, err=err, work=work).float().cpu().numpy().astype(np.float64)
+        assert int(err) == 16
+        key, pos = np.arange(L), L - n + np.arange(n)
+        seen = (key[None] <= pos[:, None]) & ~np.isin(key // P, holes)[None]
+        if window:
+            seen &= key[None] > pos[:, None] - window
+        nan = np.zeros((n, D), bool)
+        for j, b in nans:
+            nan[seen[:, j], 32 * b:32 * b + 32] = True
+        for h in range(2):
+            x = q[:, h].float().cpu().numpy().astype(np.float64)
+            s = np.where(seen, scale * (x @ k.T), -np.inf)
+            w = np.exp(s - s.max(1, keepdims=True))
+            w /= w.sum(1, keepdims=True)
+            ref, A = w @ v, w @ np.abs(v)
+            s1 = (scale * (np.abs(x) @ np.abs(k).T)).max(1)[:, None]
+            ds = (D + 4) * 2.0 ** -24 * s1 + (2.0 ** -21 * s1 if kind != "f32" else 0)
+            tol = A * (2 * ds + 2.0 ** -15 + (2.0 ** -11 if kind != "f32" else 0)) + 2.0 ** -31 * np.abs(v).sum(0)
+            tol = tol + S.HALF_STEP[kind] * (np.abs(ref) + tol) + (2.0 ** -25 if kind == "f16" else 0)
+            assert np.isnan(o[:, h][nan]).all() and (np.abs(o[:, h] - ref) <= tol)[~nan].all()
+
+
+@pytest.mark.parametrize("n_seq,Nkv,G,n,L", [(24, 8, 4, 4, 700), (24, 8, 4, 8, 700), (24, 8, 4, 12, 700), (2, 2, 2, 64, 900),
+                                             (12, 16, 2, 40, 600), (3, 1, 7, 100, 1500)])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_sizes_around_the_forms_borders(cuda, kind, n_seq, Nkv, G, n, L):
+    """Mean rows and sequences on both sides of where the form for chunks of prompts takes over, lengths and rows ragged."""
+    rng = np.random.default_rng(n_seq * n)
+    q_lens = [max(0, n - int(x)) for x in rng.integers(0, 3, n_seq)]
+    q_lens[0] = n
+    _run(rng, q_lens, [L - int(x) for x in rng.integers(0, L // 3, n_seq)], 64, Nkv, G, 64, kind)
