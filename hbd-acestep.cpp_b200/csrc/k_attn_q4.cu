@@ -716,9 +716,10 @@ extern "C" acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int t
     a.chunk      = p.chunk;
     a.n_split    = p.n_split;
     a.tiles      = p.tiles;
-    a.part_ml    = reinterpret_cast<float2 *>(work);
-    a.part_o     = reinterpret_cast<float *>(work) + 2 * n_tok * n_heads * p.n_split;
-    const int D = kv->head_dim;
+    const int D  = kv->head_dim;
+    // the sums first: their rows are whole multiples of 16 bytes, whatever the number of parts
+    a.part_o     = reinterpret_cast<float *>(work);
+    a.part_ml    = reinterpret_cast<float2 *>(a.part_o + n_tok * n_heads * p.n_split * D);
     if (attn_q4_tc_wanted(a, type, D)) {
         return attn_q4_tc_launch(a, type, D, (cudaStream_t) stream);
     }

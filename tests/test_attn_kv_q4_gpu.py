@@ -461,3 +461,13 @@ def test_sizes_around_the_forms_borders(cuda, kind, n_seq, Nkv, G, n, L):
     q_lens = [max(0, n - int(x)) for x in rng.integers(0, 3, n_seq)]
     q_lens[0] = n
     _run(rng, q_lens, [L - int(x) for x in rng.integers(0, L // 3, n_seq)], 64, Nkv, G, 64, kind)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("q_lens,kv_lens,Nkv,G,D,window", [
+    ([1], [300], 1, 7, 128, 0), ([1], [2100], 1, 71, 64, 0), ([1], [1300], 3, 3, 128, 0), ([3, 1, 1], [279, 50, 200], 1, 9, 64, 0),
+    ([1, 1, 1], [300, 200, 1], 1, 7, 128, 0), ([1] * 19, [2352] + [100] * 18, 1, 5, 128, 0), ([1] * 3, [700, 699, 3], 1, 5, 256, 200),
+    ([1] * 3, [2000, 1999, 3], 1, 11, 64, 200)])
+def test_odd_counts_of_parts(cuda, kind, q_lens, kv_lens, Nkv, G, D, window):
+    """Tokens, heads and chunks of keys that are all odd: the parts' rows stay on 16 bytes."""
+    _run(np.random.default_rng(G * D), q_lens, kv_lens, 16, Nkv, G, D, kind, window=window)
