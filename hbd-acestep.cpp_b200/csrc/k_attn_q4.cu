@@ -18,6 +18,7 @@
 // operations), 208 of the 420 of a tile of 16 keys; issue slots are 71% busy, the integer pipe 64%.
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "attn_q4.cuh"
@@ -609,6 +610,7 @@ template <int T> Kernel join_kernel(int D) {
 struct Plan {
     int     nt, tiles, chunk, n_split;
     int64_t most;  // n_split of any window at these sizes is at most this
+    int64_t rows;  // up to so many rows of a sequence and kv head nt and most stay as they are
 };
 
 Plan make_plan(const acb_kv_q4 * kv, int n_heads, int max_q, int max_kv, int window) {
@@ -623,15 +625,22 @@ Plan make_plan(const acb_kv_q4 * kv, int n_heads, int max_q, int max_kv, int win
     // three times, 159 at six. Two of 131071, before the warps were joined as now: 124 us at 111 parts each, 142 at 185, 180 at
     // 296.)
     const int64_t slots  = (int64_t) num_sms() * 5;
-    const int64_t splits = slots / tasks >= 4 ? slots / tasks : 6 * slots / tasks;
+    const int64_t parts  = slots / tasks >= 4 ? slots : 6 * slots;
+    const int64_t splits = parts / tasks;
     const int64_t least  = tasks * 4 <= num_sms() ? 128 : 256;
     const int64_t cuts   = (max_kv + least - 1) / least;
-    if (splits <= 1 || cuts <= 1) {
+    if (splits <= 1 || cuts <= 1) {  // and so it is for any more rows
         p.n_split = 1;
         p.most    = 1;
         p.chunk   = kNoChunk;
+        p.rows    = INT64_MAX;
         return p;
     }
+    int64_t same = parts / splits;  // the most tasks with as many splits (at 4 or more parts of `slots` the rule above is the same one)
+    if (least == 128 && same > num_sms() / 4) {
+        same = num_sms() / 4;
+    }
+    p.rows = p.nt == 1 && kv->head_dim != 256 ? 8 : same / ((int64_t) kv->n_kv_heads * kv->n_seq) * (8 * p.nt);
     int64_t chunk = (keys + splits - 1) / splits;
     chunk         = ((chunk < least ? least : chunk) + 63) / 64 * 64;
     p.chunk       = (int) chunk;
@@ -657,12 +666,14 @@ extern "C" size_t acb_attn_kv_q4_work_bytes(const acb_kv_q4 * kv, int64_t n_tok,
         max_kv_len <= 0) {
         return 0;
     }
-    // enough for every call of at most these sizes: fewer rows a sequence are cut into more chunks, so each power of two of
-    // them is asked, with the most rows that it stands for
-    size_t most = 0;
-    for (int64_t q = 1; q <= max_q_len; q *= 2) {
-        const int64_t rows  = (2 * q - 1) * kv->n_seq;
-        const size_t  bytes = plan_bytes(make_plan(kv, n_heads, (int) q, max_kv_len, 0).most, kv, rows < n_tok ? rows : n_tok, n_heads);
+    // Enough for every call of at most these sizes. Fewer rows a sequence can mean more chunks or fewer (make_plan's rule has a
+    // step), so every count of chunks that they can have is asked, with the most rows that have it.
+    const int64_t G    = n_heads / kv->n_kv_heads;
+    size_t        most = 0;
+    for (int64_t q = 1; q <= max_q_len; q++) {
+        const Plan p        = make_plan(kv, n_heads, (int) q, max_kv_len, 0);
+        q                   = std::min<int64_t>(max_q_len, p.rows / G);
+        const size_t bytes  = plan_bytes(p.most, kv, std::min<int64_t>(q * kv->n_seq, n_tok), n_heads);
         most                = bytes > most ? bytes : most;
     }
     return most;

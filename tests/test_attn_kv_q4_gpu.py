@@ -471,3 +471,23 @@ def test_sizes_around_the_forms_borders(cuda, kind, n_seq, Nkv, G, n, L):
 def test_odd_counts_of_parts(cuda, kind, q_lens, kv_lens, Nkv, G, D, window):
     """Tokens, heads and chunks of keys that are all odd: the parts' rows stay on 16 bytes."""
     _run(np.random.default_rng(G * D), q_lens, kv_lens, 16, Nkv, G, D, kind, window=window)
+
+
+@pytest.mark.parametrize("kind,n_seq,Nkv,G,D,n,L,whole", [("f32", 16, 8, 2, 128, 9, 8192, False), ("f32", 16, 8, 2, 128, 15, 8192, False),
+                                                          ("f16", 24, 2, 7, 64, 7, 4000, True), ("bf16", 1, 1, 4, 256, 200, 3000, False),
+                                                          ("f32", 24, 2, 7, 64, 7, 4000, False)])
+def test_the_workspace_is_enough_to_split(cuda, kind, n_seq, Nkv, G, D, n, L, whole):
+    """The workspace of these sizes, one made within and one with room for anything: the same chunks of keys, so the same bits.
+    whole: 24 sequences of 2 kv heads and 4 tiles of 16 rows go to the form that does not cut the keys."""
+    import torch
+    rng = np.random.default_rng(n)
+    cache = _cache(rng, n_seq, L, 64, Nkv, D)
+    q = torch.from_numpy(rng.standard_normal((n_seq * n, Nkv * G, D)).astype(np.float32)).to(S.torch_type(kind)).cuda()
+    start = torch.arange(n_seq + 1, dtype=torch.int32).cuda() * n
+    ln = torch.from_numpy(rng.integers(L // 2, L + 1, n_seq).astype(np.int32)).cuda()
+    kw = dict(q_start=start, max_q_len=n, max_kv_len=L)
+    ample = cache.attention(q, ln, work=torch.empty(1 << 30, dtype=torch.uint8).cuda(), **kw)
+    plain = cache.attention(q, ln, work=torch.empty(1, dtype=torch.uint8).cuda(), **kw)
+    assert torch.equal(ample, plain) == whole
+    assert torch.equal(cache.attention(q, ln, work=cache.attn_workspace(n_seq * n, Nkv * G, n, L), **kw), ample)
+    assert torch.equal(cache.attention(q, ln, **kw), ample)

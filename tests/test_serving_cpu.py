@@ -195,3 +195,18 @@ def test_workspaces_cover_every_smaller_call():
 
 def test_append_refuses_more_tokens_than_a_grid_has_blocks():
     assert append(cache(), n_heads=0, n_tok=2 ** 31) == 2
+
+
+@pytest.mark.parametrize("n_seq,n_kv,heads,D,first,last,keys", [
+    (16, 8, 16, 128, 9, 16, 8192), (24, 2, 14, 64, 5, 6, 4000), (24, 2, 14, 64, 7, 9, 4000), (1, 1, 1, 128, 1009, 1024, 60000),
+    (5, 4, 12, 256, 51, 53, 20000)])
+def test_workspaces_cover_every_count_of_rows(n_seq, n_kv, heads, D, first, last, keys):
+    """Calls of first..last rows a sequence fill the same number of row tiles, so their keys are cut alike and they need the same
+    bytes a row; what is enough for the most of them is enough for all in that measure."""
+    kv = cache(n_seq=n_seq, n_kv_heads=n_kv, head_dim=D, max_pages=1 << 12, table_stride=1 << 12, n_pages=1 << 13)
+    tile = 8 if D == 256 else 16
+    assert -(-first * heads // n_kv // tile) == -(-last * heads // n_kv // tile)
+    f = lambda q: acb.lib().acb_attn_kv_q4_work_bytes(C.addressof(kv), n_seq * q, heads, q, keys)  # noqa: E731
+    assert f(last) > 0
+    for q in range(first, last):
+        assert f(q) * last >= f(last) * q and f(q) <= f(last)
