@@ -22,8 +22,10 @@ struct AttnQ4Args {
     int             chunk;    // keys of a block, a multiple of 64
     int             tiles;    // of the rows
     int             n_split;  // chunks that the rows of one block can touch
-    float *         part_o;   // [n_tok*Nh][n_split][D]: sums of P V
-    float2 *        part_ml;  // [n_tok*Nh][n_split]: m (log2), l
+    int64_t         rows;     // tokens that sequences can have: n_tok, or max_q of each where that is less
+    bool            by_seq;   // parts by sequence and its new token, not by token (max_q of each is less)
+    float *         part_o;   // [rows*Nh][n_split][D]: sums of P V
+    float2 *        part_ml;  // [rows*Nh][n_split]: m (log2), l
 };
 
 // rows and keys of sequence s as the device arrays give them; false when they are outside the call's bounds

@@ -87,6 +87,11 @@ template <int D> struct Stage16 {
     }
 };
 
+// where the parts of new token i of sequence s are, in rows of all heads
+__device__ __forceinline__ int64_t part_row(const AttnQ4Args & a, int s, int i, int64_t tok) {
+    return a.by_seq ? (int64_t) s * a.max_q + i : tok;
+}
+
 // dimension of nibble `hi` of byte b of a row's codes
 __device__ __forceinline__ int dim_of(int b, int hi) {
     return (b >> 4) * 32 + (b & 15) + 16 * hi;
@@ -516,7 +521,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps, kSplitBlocks<T, D, NT>) attn
             y[2]            = io<T>::from_f(v.z * inv);
             y[3]            = io<T>::from_f(v.w * inv);
         } else {
-            const int64_t slot = (tok * a.Nh + h) * a.n_split + c % a.n_split;
+            const int64_t slot = (part_row(a, s, i, tok) * a.Nh + h) * a.n_split + c % a.n_split;
             *reinterpret_cast<float4 *>(a.part_o + slot * D + d) = v;
             if (d == 0) {
                 a.part_ml[slot] = make_float2(s_top[rr], L);
@@ -549,7 +554,7 @@ template <int T, int D> __global__ void __launch_bounds__(32 * kJoinWarps) attn_
     }
     const int64_t tok = row0 + i;
     const int     h   = hk * a.G + r - i * a.G;
-    const int64_t at  = (tok * a.Nh + h) * a.n_split;
+    const int64_t at  = (part_row(a, s, i, tok) * a.Nh + h) * a.n_split;
     float         M = -INFINITY, L = 0.0f, o[E];
     for (int c = c0 + lane; c <= c1; c += 32) {
         M = fmaxf(M, a.part_ml[at + c % a.n_split].x);
@@ -650,8 +655,13 @@ Plan make_plan(const acb_kv_q4 * kv, int n_heads, int max_q, int max_kv, int win
     return p;
 }
 
-size_t plan_bytes(int64_t n_split, const acb_kv_q4 * kv, int64_t n_tok, int n_heads) {
-    return n_split <= 1 ? 0 : (size_t) n_tok * n_heads * n_split * (kv->head_dim + 2) * sizeof(float);
+// Tokens that can have parts: a batch may be padded with rows that belong to no sequence, and then there are at most so many.
+int64_t part_rows(const acb_kv_q4 * kv, int64_t n_tok, int64_t max_q) {
+    return std::min<int64_t>(n_tok, max_q * kv->n_seq);
+}
+
+size_t plan_bytes(int64_t n_split, const acb_kv_q4 * kv, int64_t rows, int n_heads) {
+    return n_split <= 1 ? 0 : (size_t) rows * n_heads * n_split * (kv->head_dim + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -673,7 +683,7 @@ extern "C" size_t acb_attn_kv_q4_work_bytes(const acb_kv_q4 * kv, int64_t n_tok,
     for (int64_t q = 1; q <= max_q_len; q++) {
         const Plan p        = make_plan(kv, n_heads, (int) q, max_kv_len, 0);
         q                   = std::min<int64_t>(max_q_len, p.rows / G);
-        const size_t bytes  = plan_bytes(p.most, kv, std::min<int64_t>(q * kv->n_seq, n_tok), n_heads);
+        const size_t bytes  = plan_bytes(p.most, kv, part_rows(kv, n_tok, q), n_heads);
         most                = bytes > most ? bytes : most;
     }
     return most;
@@ -704,8 +714,9 @@ extern "C" acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int t
     if (n_tok == 0) {
         return ACB_OK;
     }
-    Plan p = make_plan(kv, n_heads, max_q_len, max_kv_len, window);
-    if (p.n_split > 1 && (!work || work_bytes < plan_bytes(p.n_split, kv, n_tok, n_heads))) {
+    Plan          p    = make_plan(kv, n_heads, max_q_len, max_kv_len, window);
+    const int64_t rows = part_rows(kv, n_tok, max_q_len);
+    if (p.n_split > 1 && (!work || work_bytes < plan_bytes(p.n_split, kv, rows, n_heads))) {
         p.n_split = 1;
         p.chunk   = kNoChunk;
     }
@@ -730,7 +741,9 @@ extern "C" acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int t
     const int D  = kv->head_dim;
     // the sums first: their rows are whole multiples of 16 bytes, whatever the number of parts
     a.part_o     = reinterpret_cast<float *>(work);
-    a.part_ml    = reinterpret_cast<float2 *>(a.part_o + n_tok * n_heads * p.n_split * D);
+    a.part_ml    = reinterpret_cast<float2 *>(a.part_o + rows * n_heads * p.n_split * D);
+    a.rows       = rows;
+    a.by_seq     = rows < n_tok;
     if (attn_q4_tc_wanted(a, type, D)) {
         return attn_q4_tc_launch(a, type, D, (cudaStream_t) stream);
     }

@@ -674,7 +674,7 @@ bool attn_q4_tc_wanted(const AttnQ4Args & a, int type, int head_dim) {
     if (rows >= 64 && (keys < 512 || a.n_split == 1)) {
         return true;
     }
-    const int64_t mean  = (a.n_tok * a.G + a.kv.n_seq - 1) / a.kv.n_seq, tasks = (int64_t) a.kv.n_seq * a.kv.nkv;
+    const int64_t mean  = (a.rows * a.G + a.kv.n_seq - 1) / a.kv.n_seq, tasks = (int64_t) a.kv.n_seq * a.kv.nkv;
     const int64_t waves = (tasks * ((mean + 2 * kQtRows - 1) / (2 * kQtRows)) + num_sms() - 1) / num_sms();
     return keys >= 512 && tasks * ((mean + 15) / 16) >= 180 * waves;
 }

@@ -491,3 +491,33 @@ def test_the_workspace_is_enough_to_split(cuda, kind, n_seq, Nkv, G, D, n, L, wh
     assert torch.equal(ample, plain) == whole
     assert torch.equal(cache.attention(q, ln, work=cache.attn_workspace(n_seq * n, Nkv * G, n, L), **kw), ample)
     assert torch.equal(cache.attention(q, ln, **kw), ample)
+
+
+@pytest.mark.parametrize("kind,n_seq,Nkv,G,D,n,pad,window", [
+    ("f32", 8, 8, 2, 128, 1, 56, 0), ("bf16", 8, 8, 2, 128, 1, 2040, 0), ("f16", 3, 1, 7, 64, 5, 6, 0), ("f32", 5, 2, 3, 256, 3, 1, 0),
+    ("f32", 3, 1, 5, 64, 2, 100, 700), ("bf16", 2, 2, 2, 64, 100, 1848, 0)])
+def test_padded_batches_are_as_the_batch_alone(cuda, kind, n_seq, Nkv, G, D, n, pad, window):
+    """Rows in front of, and behind, all sequences change neither the chunks nor the bits, and stay as they were."""
+    import torch
+    rng = np.random.default_rng(pad)
+    L, H = 5000, Nkv * G
+    cache = _cache(rng, n_seq, L, 64, Nkv, D)
+    lens = [n - i % 2 * (n > 1) for i in range(n_seq)]
+    lens[0] = n
+    T = sum(lens)
+    q = torch.from_numpy(rng.standard_normal((T, H, D)).astype(np.float32)).to(S.torch_type(kind)).cuda()
+    start = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32).cuda()
+    kv = [L - int(x) for x in rng.integers(0, L // 2, n_seq)]
+    kw = dict(kv_len=torch.tensor(kv, dtype=torch.int32).cuda(), max_q_len=n, max_kv_len=L, window=window)
+    ref = cache.attention(q, q_start=start, **kw)
+    ample = cache.attention(q, q_start=start, work=torch.empty(1 << 28, dtype=torch.uint8).cuda(), **kw)
+    assert torch.equal(ref, ample)
+    front = pad // 3
+    wide = torch.full((T + pad, H, D), float("nan"), dtype=q.dtype).cuda()
+    wide[front:front + T] = q
+    for work in (None, cache.attn_workspace(T + pad, H, n, L)):
+        o = torch.full_like(wide, 7.0)
+        cache.attention(wide, q_start=start + front, out=o, work=work, **kw)
+        assert torch.equal(o[front:front + T], ref)
+        assert bool((o[:front] == 7).all()) and bool((o[front + T:] == 7).all())
+    _check(cache, q, ref, lens, kv, window, D ** -0.5, kind)
