@@ -255,7 +255,8 @@ template <int T, int D, bool ALIGNED> __global__ void __launch_bounds__(kQtThrea
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const int  key  = tid + 64 * e;
-                    const bool gone = key0 + key > p1;
+                    // behind the last row, or before every row's window: no key of this block of rows, wherever its page is
+                    const bool gone = key0 + key > p1 || key0 + key < key_lo;
                     if (bad[e] && !gone) {
                         atomicOr(&bad_key[note][key >> 5], 1u << (key & 31));
                         bad_any[note][0] = 1;

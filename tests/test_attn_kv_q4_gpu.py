@@ -521,3 +521,29 @@ def test_padded_batches_are_as_the_batch_alone(cuda, kind, n_seq, Nkv, G, D, n, 
         assert torch.equal(o[front:front + T], ref)
         assert bool((o[:front] == 7).all()) and bool((o[front + T:] == 7).all())
     _check(cache, q, ref, lens, kv, window, D ** -0.5, kind)
+
+
+@pytest.mark.parametrize("kind,D", [("f32", 128), ("bf16", 128), ("f16", 64), ("bf16", 256)])
+@pytest.mark.parametrize("n,window", [(1, 100), (5, 1), (130, 100), (300, 17), (300, 333), (700, 40)])
+def test_pages_behind_the_window_may_be_gone(cuda, kind, D, n, window):
+    """A server frees the pages that lie wholly before the first row's window: no error, and the same answer."""
+    import torch
+    rng = np.random.default_rng(n + window)
+    P = 16
+    cache = _cache(rng, 2, 1000, P, 1, D)
+    q = torch.from_numpy(rng.standard_normal((2 * n, 2, D)).astype(np.float32)).to(S.torch_type(kind)).cuda()
+    start, lens = torch.tensor([0, n, 2 * n], dtype=torch.int32).cuda(), [1000, 901]
+    ln = torch.tensor(lens, dtype=torch.int32).cuda()
+    ref = cache.attention(q, ln, start, n, window=window)
+    freed = 0
+    for s, m in enumerate(lens):
+        first = max(0, m - n - window + 1)
+        cache.tensors[4][s, :first // P] = torch.tensor([-1, 10 ** 6], dtype=torch.int32).cuda().repeat(100)[:first // P]
+        freed += first // P
+    assert freed > 0
+    err = torch.zeros(1, dtype=torch.int32).cuda()
+    o = cache.attention(q, ln, start, n, window=window, err=err)
+    assert int(err) == 0 and torch.equal(o, ref)
+    cache.tensors[4][0, (1000 - n - window + 1) // P] = -1  # the first page that the first row sees
+    cache.attention(q, ln, start, n, window=window, err=err)
+    assert int(err) == 16
