@@ -714,6 +714,8 @@ extern "C" acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int t
     if (n_tok == 0) {
         return ACB_OK;
     }
+    // A window of all keys is none. What is left is far from where a position less a window leaves 32 bits.
+    window             = window >= max_kv_len ? 0 : window;
     Plan          p    = make_plan(kv, n_heads, max_q_len, max_kv_len, window);
     const int64_t rows = part_rows(kv, n_tok, max_q_len);
     if (p.n_split > 1 && (!work || work_bytes < plan_bytes(p.n_split, kv, rows, n_heads))) {

@@ -547,3 +547,17 @@ def test_pages_behind_the_window_may_be_gone(cuda, kind, D, n, window):
     cache.tensors[4][0, (1000 - n - window + 1) // P] = -1  # the first page that the first row sees
     cache.attention(q, ln, start, n, window=window, err=err)
     assert int(err) == 16
+
+
+@pytest.mark.parametrize("kind,n,L", [("f32", 8, 3), ("bf16", 8, 3), ("bf16", 130, 100), ("f16", 300, 290), ("f32", 130, 100)])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30, 1000])
+def test_windows_of_more_than_all_keys(cuda, kind, n, L, window):
+    """The largest windows, over fewer keys than rows: the bits of no window."""
+    import torch
+    rng = np.random.default_rng(n)
+    cache = _cache(rng, 2, 400, 16, 1, 128)
+    q = torch.from_numpy(rng.standard_normal((2 * n, 2, 128)).astype(np.float32)).to(S.torch_type(kind)).cuda()
+    start, ln = torch.tensor([0, n, 2 * n], dtype=torch.int32).cuda(), torch.tensor([L, L // 2], dtype=torch.int32).cuda()
+    ref = cache.attention(q, ln, start, n)
+    assert torch.equal(cache.attention(q, ln, start, n, window=window), ref)
+    _check(cache, q, ref, [n, n], [L, L // 2], 0, 128 ** -0.5, kind)
