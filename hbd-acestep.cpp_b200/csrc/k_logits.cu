@@ -376,7 +376,8 @@ template <int TI, int TO> acb_status rules_launch(RulesArgs a, int rows, cudaStr
     const auto   kern = vec ? (hash ? logits_rules_kernel<TI, TO, true, true> : logits_rules_kernel<TI, TO, true, false>)
                             : (hash ? logits_rules_kernel<TI, TO, false, true> : logits_rules_kernel<TI, TO, false, false>);
     if (smem) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem);
+        // the kernel's limit, not this launch's size: it holds for the launches of every host thread
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) (kWords * sizeof(uint32_t)));
         if (e != cudaSuccess) {
             set_last_cuda_error(e);
             return ACB_ERR_CUDA;

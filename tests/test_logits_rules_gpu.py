@@ -209,3 +209,38 @@ def test_long_slices_of_many_rows(cuda, V, L, B, pad):
     some = [0, 1, 50, R - 1]
     _check(out[some, :V].cpu().numpy().astype(np.float64), x[some].float().numpy(), len(some), "f32", hist[some], lens[some], prompt[some],
            rep[some], freq[some], pres[some], [b[some] for b in bias] if B else None, bits, mrow[some])
+
+
+def test_host_threads_of_long_and_short_histories(cuda):
+    """Calls from several threads at once, each on a stream of its own and straight into the library, so that they meet
+    there: no call's size limits another's launch."""
+    import ctypes as C
+    import threading
+    import torch
+    rng = np.random.default_rng(8)
+    V, calls, fn = 4096, 5000, acb.lib().acb_logits_rules
+    x = torch.randn(2, V).cuda()
+    rep = torch.full((2,), 1.5).cuda()
+    jobs = []
+    for L in (6000, 3, 5000, 40):
+        hist = torch.from_numpy(rng.integers(0, V, (2, L)).astype(np.int32)).cuda()
+        out = torch.empty_like(x)
+        r = acb._LogitRules(hist=hist.data_ptr(), hist_stride=L, rep=rep.data_ptr())
+        st = torch.cuda.Stream()
+        args = (x.data_ptr(), acb.F32, V, out.data_ptr(), acb.F32, V, 2, V, C.addressof(r), None, st.cuda_stream)
+        jobs.append((args, acb.logits_rules(x, hist, rep=rep), out, st, set(), (hist, r)))
+    torch.cuda.synchronize()
+    go = threading.Barrier(len(jobs))
+
+    def run(args, ref, out, st, seen, keep):
+        go.wait()
+        for _ in range(calls):
+            seen.add(fn(*args))
+    threads = [threading.Thread(target=run, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for args, ref, out, st, seen, keep in jobs:
+        assert seen == {0} and torch.equal(out, ref)
