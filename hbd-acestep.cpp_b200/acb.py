@@ -423,6 +423,16 @@ def _run_on(name, dev, stream, *args):
         raise AcbError(name, st)
 
 
+def _empty(shape, dtype, device, stream):
+    """A tensor for a call on `stream` (None: the current one). It belongs to that stream: what is freed of it may be handed to
+    later work of the same stream only."""
+    import torch
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _device(name, t):
     """Number of the GPU that holds t."""
     dev = t.get_device()
@@ -468,7 +478,7 @@ def rope(x, pos, table, layout="half", inverse=False, out=None, err=None, stream
     T, H, D = x.shape
     dev = _device("rope", x)
     if out is None:
-        out = torch.empty((T, H, D), dtype=x.dtype, device=x.device)
+        out = _empty((T, H, D), x.dtype, x.device, stream)
     sx, so = x.stride(), out.stride()
     if out.dtype is not x.dtype or out.shape != x.shape or out.get_device() != dev or sx[2] != 1 or so[2] != 1:
         raise ValueError("rope: x and out have one type, shape and device, their last dimension contiguous")
@@ -537,7 +547,7 @@ class KVCacheQ4:
         at_qn = _want("KVCacheQ4.append: q_norm", q_norm, f32, dev, D)
         at_kn = _want("KVCacheQ4.append: k_norm", k_norm, f32, dev, D)
         if n_heads > 0 and q_out is None:
-            q_out = torch.empty((T, n_heads, D), dtype=q_dtype or qkv.dtype, device=self.device)
+            q_out = _empty((T, n_heads, D), q_dtype or qkv.dtype, self.device, stream)
         if n_heads > 0 and (q_out.shape != (T, n_heads, D) or q_out.stride()[1:] != (D, 1) or q_out.get_device() != dev):
             raise ValueError("KVCacheQ4.append: q_out [T, n_heads, head_dim] with contiguous rows is wanted")
         if T == 0:
@@ -556,8 +566,7 @@ class KVCacheQ4:
         at_seq = _want("KVCacheQ4.read: seq", seq, torch.int32, self.dev)
         at_pos = _want("KVCacheQ4.read: pos", pos, torch.int32, self.dev, T)
         if k_out is None and v_out is None:
-            k_out = torch.empty(shape, dtype=dtype or torch.float16, device=self.device)
-            v_out = torch.empty_like(k_out)
+            k_out, v_out = (_empty(shape, dtype or torch.float16, self.device, stream) for _ in "kv")
         first = k_out if k_out is not None else v_out
         for t in (k_out, v_out):
             if t is not None and (t.shape != shape or t.dtype is not first.dtype or t.stride() != first.stride()
@@ -569,11 +578,12 @@ class KVCacheQ4:
                 dtype_id(first), _row_stride("KVCacheQ4.read", first, shape[1] * shape[2]), _ptr(err))
         return k_out, v_out
 
-    def attn_workspace(self, n_tok, n_heads, max_q_len, max_kv_len):
-        """A workspace for attention() calls of at most these sizes (None where they need none)."""
+    def attn_workspace(self, n_tok, n_heads, max_q_len, max_kv_len, stream=None):
+        """A workspace for attention() calls of n_heads heads and at most these other sizes (None where they need none); stream:
+        the one they run on, where it is not the current one."""
         import torch
         n = lib().acb_attn_kv_q4_work_bytes(self.ref, n_tok, n_heads, max_q_len, max_kv_len)
-        return torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+        return _empty((n,), torch.uint8, self.device, stream) if n else None
 
     def attention(self, q, kv_len, q_start=None, max_q_len=1, max_kv_len=None, window=0, scale=None, out=None, work=None,
                   err=None, stream=None):
@@ -590,13 +600,13 @@ class KVCacheQ4:
         at_len = _want("KVCacheQ4.attention: kv_len", kv_len, torch.int32, dev, self.n_seq)
         at_start = _want("KVCacheQ4.attention: q_start", q_start, torch.int32, dev, self.n_seq + 1)
         if out is None:
-            out = torch.empty((T, H, D), dtype=q.dtype, device=self.device)
+            out = _empty((T, H, D), q.dtype, self.device, stream)
         if out.dtype is not q.dtype or out.shape != q.shape or out.stride()[1:] != (D, 1) or out.get_device() != dev:
             raise ValueError("KVCacheQ4.attention: out of q's type and shape with contiguous rows is wanted")
         if T == 0:
             return out
         if work is None:
-            work = self.attn_workspace(T, H, max_q_len, max_kv_len)
+            work = self.attn_workspace(T, H, max_q_len, max_kv_len, stream)
         elif work.get_device() != dev or not work.is_contiguous():
             raise ValueError("KVCacheQ4.attention: the workspace is a contiguous tensor on the cache's device")
         _run_on("acb_attn_kv_q4", dev, stream, self.ref, q.data_ptr(), dtype_id(q), _row_stride("KVCacheQ4.attention: q", q, H * D),
@@ -621,7 +631,7 @@ def logits_rules(logits, hist=None, hist_len=None, prompt_len=None, rep=None, fr
     R, V = logits.shape
     dev, i32, f32 = _device("logits_rules", logits), torch.int32, torch.float32
     if out is None:
-        out = torch.empty((R, V), dtype=out_dtype or logits.dtype, device=logits.device)
+        out = _empty((R, V), out_dtype or logits.dtype, logits.device, stream)
     if out.shape != logits.shape or out.get_device() != dev or logits.stride(1) != 1 or out.stride(1) != 1:
         raise ValueError("logits_rules: logits and out [R, V] with contiguous rows are wanted")
     at_len = _want("logits_rules: hist_len", hist_len, i32, dev, R)

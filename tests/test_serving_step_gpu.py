@@ -118,3 +118,65 @@ def test_prompt_then_tokens(cuda, graph):
             fin = np.isfinite(ref)
             assert np.abs(got[fin] - ref[fin]).max() <= tol
             assert picked[step_i, s] == int(np.argmax(got)) and allowed[0, picked[step_i, s]]
+
+
+def _calls(rng):
+    """One call of every operator, to be made on a given stream"""
+    import torch
+    table = torch.arange(64, dtype=torch.int32).view(1, 64).cuda()
+    cache = acb.KVCacheQ4.empty(64, 64, 2, 128, table)
+    cache.tensors[0].random_(0, 256), cache.tensors[2].random_(0, 256)
+    for t in (cache.tensors[1], cache.tensors[3]):
+        t.copy_((0.02 + 0.2 * torch.rand(t.shape)).bfloat16().half())
+    x = torch.from_numpy(rng.standard_normal((2, 8, 128)).astype(np.float32)).cuda()
+    pos, seq = torch.tensor([4094, 4095], dtype=torch.int32).cuda(), torch.zeros(2, dtype=torch.int32).cuda()
+    before = pos - 100  # (a caller's tensors live until the stream is done with them)
+    ln, start = torch.tensor([4090], dtype=torch.int32).cuda(), torch.tensor([0, 2], dtype=torch.int32).cuda()
+    rope = acb.rope_table_scaled(4096, 128, 1e4).cuda()
+    lg = torch.from_numpy(rng.standard_normal((2, 5000)).astype(np.float32)).cuda()
+    hist = torch.from_numpy(rng.integers(0, 5000, (2, 40)).astype(np.int32)).cuda()
+    two = torch.full((2,), 1.5).cuda()
+    return [lambda st: acb.rope(x, pos, rope, stream=st),
+            lambda st: cache.append(x.reshape(2, -1), 4, seq, pos, rope, stream=st),
+            lambda st: cache.read(seq, before, stream=st),
+            lambda st: cache.attention(x, ln, start, 2, stream=st),
+            lambda st: acb.logits_rules(lg, hist, rep=two, stream=st)]
+
+
+@pytest.mark.parametrize("as_number", [False, True])
+def test_what_a_call_makes_belongs_to_its_stream(cuda, monkeypatch, as_number):
+    import torch
+    side, made, empty = torch.cuda.Stream(), [], torch.empty
+
+    def noted(*a, **kw):
+        made.append(torch.cuda.current_stream().cuda_stream)
+        return empty(*a, **kw)
+    for call in _calls(np.random.default_rng(1)):
+        torch.cuda.synchronize()
+        monkeypatch.setattr(torch, "empty", noted)
+        made.clear()
+        call(side.cuda_stream if as_number else side)
+        monkeypatch.undo()
+        assert made and set(made) == {side.cuda_stream}
+        assert torch.cuda.current_stream().cuda_stream != side.cuda_stream
+    torch.cuda.synchronize()
+
+
+def test_a_late_stream_and_new_memory_on_the_current_one(cuda):
+    """The call's stream is busy; what the current stream is given and fills in the meantime is none of the call's memory."""
+    import torch
+    for call in _calls(np.random.default_rng(2)):
+        ref = call(None)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            a = torch.ones(2048, 2048, device="cuda")
+            for _ in range(50):
+                a = (a @ a).clamp_(-1, 1)
+        got = call(side)
+        junk = [torch.full((n,), float("nan"), device="cuda") for n in (64, 512, 4096, 1 << 15, 1 << 18, 1 << 20) for _ in range(20)]
+        torch.cuda.synchronize()
+        # (looked at after the synchronisation only: read gives two tensors)
+        got, ref = (v if isinstance(v, tuple) else (v,) for v in (got, ref))
+        assert all(torch.equal(g, r) for g, r in zip(got, ref)) and len(junk) == 120
