@@ -379,7 +379,7 @@ def argmax(logits, ids, margin=None, pos_advance=None, scratch=None, flags=0, st
     import torch
     rows, V = logits.shape
     if scratch is None:
-        scratch = torch.zeros(lib().acb_argmax_scratch_bytes(rows, V), dtype=torch.uint8, device=logits.device)
+        scratch = _made_on(stream, torch.zeros, lib().acb_argmax_scratch_bytes(rows, V), dtype=torch.uint8, device=logits.device)
     _check("acb_argmax", lib().acb_argmax(_ptr(logits), logits.stride(0), V, rows, _ptr(ids), _ptr(margin),
                                            _ptr(pos_advance), None, None, 0, None, _ptr(scratch), flags,
                                            _stream(stream)))
@@ -423,14 +423,19 @@ def _run_on(name, dev, stream, *args):
         raise AcbError(name, st)
 
 
-def _empty(shape, dtype, device, stream):
-    """A tensor for a call on `stream` (None: the current one). It belongs to that stream: what is freed of it may be handed to
-    later work of the same stream only."""
+def _made_on(stream, make, *args, device, **kw):
+    """make(*args, device=device, ..) for a call on `stream` (None: the current one). What it makes belongs to that stream: freed,
+    it may be handed to later work of the same stream only."""
     import torch
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return make(*args, device=device, **kw)
     with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return make(*args, device=device, **kw)
+
+
+def _empty(shape, dtype, device, stream):
+    import torch
+    return _made_on(stream, torch.empty, shape, dtype=dtype, device=device)
 
 
 def _device(name, t):
@@ -979,8 +984,8 @@ def sample_top_k_p(logits, temperature, top_p, top_k, u=None, uncond=None, cfg_s
     if span_len is None:
         span_len = ld - span_off
     Vc = (1 if col0 >= 0 else 0) + span_len
-    work = torch.empty(max(1, lib().acb_sample_work_bytes(rows, Vc)) // 4, dtype=torch.float32, device=logits.device)
-    idx = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    work = _empty((max(1, lib().acb_sample_work_bytes(rows, Vc)) // 4,), torch.float32, logits.device, stream)
+    idx = _empty((rows,), torch.int32, logits.device, stream)
     _check("acb_sample_top_k_p", lib().acb_sample_top_k_p(
         _ptr(logits), ld, None if uncond is None else _ptr(uncond), 0 if uncond is None else uncond.shape[1],
         float(cfg_scale), int(col0), int(span_off), int(span_len), rows, float(temperature), float(top_p),

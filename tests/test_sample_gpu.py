@@ -146,3 +146,25 @@ def test_lm_forward_batch_sample_matches_host_sampling(cuda, tmp_path):
     assert a.kv_pos(0) == b.kv_pos(0)
     a.close()
     b.close()
+
+
+@pytest.mark.parametrize("as_number", [False, True])
+def test_scratch_belongs_to_the_stream_of_the_call(cuda, monkeypatch, as_number):
+    """What the wrappers make for a call on another stream comes from that stream's memory (and is zeroed on it)."""
+    import torch
+    logits = torch.randn(3, 4000).cuda()
+    ids = torch.zeros(3, dtype=torch.int32).cuda()
+    side, made = torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    stream = side.cuda_stream if as_number else side
+    for name in ("empty", "zeros"):
+        def noted(*a, make=getattr(torch, name), **kw):
+            made.append(torch.cuda.current_stream().cuda_stream)
+            return make(*a, **kw)
+        monkeypatch.setattr(torch, name, noted)
+    picked = acb.sample_top_k_p(logits, 0.0, 1.0, 0, stream=stream)
+    acb.argmax(logits, ids, stream=stream)
+    monkeypatch.undo()
+    torch.cuda.synchronize()
+    assert len(made) == 3 and set(made) == {side.cuda_stream}
+    assert torch.equal(ids.long(), logits.argmax(1)) and torch.equal(picked.long(), logits.argmax(1))
