@@ -457,6 +457,12 @@ def _want(name, t, dtype, dev, numel=0, contiguous=True):
     return t.data_ptr()
 
 
+def _want_err(name, err, dev):
+    """Address of a flag word (a tensor, or an address as it is)."""
+    import torch
+    return err if err is None or isinstance(err, int) else _want(name + ": err", err, torch.int32, dev, 1)
+
+
 def _row_stride(name, t, width):
     """Elements between the rows of t [T, ...], which hold width elements each (a single row may say anything)."""
     if t.shape[0] <= 1:
@@ -493,7 +499,7 @@ def rope(x, pos, table, layout="half", inverse=False, out=None, err=None, stream
     max_pos, width = table.shape
     _run_on("acb_rope", dev, stream, x.data_ptr(), sx[0], sx[1], out.data_ptr(), so[0], so[1],
             dtype_id(x), T, H, D, width,
-            _ROPE_LAYOUT[layout] | (ROPE_INVERSE if inverse else 0), at_pos, at_table, max_pos, _ptr(err))
+            _ROPE_LAYOUT[layout] | (ROPE_INVERSE if inverse else 0), at_pos, at_table, max_pos, _want_err("rope", err, dev))
     return out
 
 
@@ -561,7 +567,7 @@ class KVCacheQ4:
         _run_on("acb_kv_q4_append", dev, stream, self.ref, qkv.data_ptr(), dtype_id(qkv),
                 _row_stride("KVCacheQ4.append: qkv", qkv, qkv.shape[1]), T, n_heads, at_qn, at_kn, eps, at_table, mp, rd,
                 _ROPE_LAYOUT[layout], at_seq, at_pos, _ptr(q_out), dtype_id(q_out if q_out is not None else qkv),
-                _row_stride("KVCacheQ4.append: q_out", q_out, n_heads * D) if q_out is not None else 0, _ptr(err))
+                _row_stride("KVCacheQ4.append: q_out", q_out, n_heads * D) if q_out is not None else 0, _want_err("KVCacheQ4.append", err, dev))
         return q_out
 
     def read(self, seq, pos, k_out=None, v_out=None, dtype=None, err=None, stream=None):
@@ -580,7 +586,7 @@ class KVCacheQ4:
         if T == 0:
             return k_out, v_out
         _run_on("acb_kv_q4_read", self.dev, stream, self.ref, at_seq, at_pos, T, _ptr(k_out), _ptr(v_out),
-                dtype_id(first), _row_stride("KVCacheQ4.read", first, shape[1] * shape[2]), _ptr(err))
+                dtype_id(first), _row_stride("KVCacheQ4.read", first, shape[1] * shape[2]), _want_err("KVCacheQ4.read", err, self.dev))
         return k_out, v_out
 
     def attn_workspace(self, n_tok, n_heads, max_q_len, max_kv_len, stream=None):
@@ -616,7 +622,7 @@ class KVCacheQ4:
             raise ValueError("KVCacheQ4.attention: the workspace is a contiguous tensor on the cache's device")
         _run_on("acb_attn_kv_q4", dev, stream, self.ref, q.data_ptr(), dtype_id(q), _row_stride("KVCacheQ4.attention: q", q, H * D),
                 T, H, at_start, at_len, max_q_len, max_kv_len, window, D ** -0.5 if scale is None else scale, out.data_ptr(),
-                _row_stride("KVCacheQ4.attention: out", out, H * D), _ptr(work), work.numel() * work.element_size() if work is not None else 0, _ptr(err))
+                _row_stride("KVCacheQ4.attention: out", out, H * D), _ptr(work), work.numel() * work.element_size() if work is not None else 0, _want_err("KVCacheQ4.attention", err, dev))
         return out
 
 
@@ -675,7 +681,7 @@ def logits_rules(logits, hist=None, hist_len=None, prompt_len=None, rep=None, fr
     r = _LogitRules(at_hist, n_hist, at_len, at_prompt, at_rep, at_freq, at_pres, at_ids, at_val, bias_stride, n_bias, n_masks,
                     at_mask, words, at_row)
     _run_on("acb_logits_rules", dev, stream, logits.data_ptr(), dtype_id(logits), _row_stride("logits_rules: logits", logits, V),
-            out.data_ptr(), dtype_id(out), _row_stride("logits_rules: out", out, V), R, V, C.addressof(r), _ptr(err))
+            out.data_ptr(), dtype_id(out), _row_stride("logits_rules: out", out, V), R, V, C.addressof(r), _want_err("logits_rules", err, dev))
     return out
 
 

@@ -180,3 +180,21 @@ def test_a_late_stream_and_new_memory_on_the_current_one(cuda):
         # (looked at after the synchronisation only: read gives two tensors)
         got, ref = (v if isinstance(v, tuple) else (v,) for v in (got, ref))
         assert all(torch.equal(g, r) for g, r in zip(got, ref)) and len(junk) == 120
+
+
+def test_flag_words_that_would_be_misread_are_refused(cuda):
+    """A flag on the host, of another type or without an element: refused before anything is launched."""
+    import torch
+    x, pos = torch.randn(1, 4, 64).cuda(), torch.zeros(1, dtype=torch.int32).cuda()
+    table, rope = torch.zeros((1, 1), dtype=torch.int32).cuda(), acb.rope_table_scaled(16, 64, 1e4).cuda()
+    cache = acb.KVCacheQ4.empty(1, 16, 1, 64, table)
+    good = torch.zeros(1, dtype=torch.int32).cuda()
+    for bad in (torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int64).cuda(), torch.zeros(4, dtype=torch.uint8).cuda(),
+                torch.zeros(0, dtype=torch.int32).cuda()):
+        for call in (lambda e: acb.rope(x, pos, rope, err=e), lambda e: cache.append(x.view(1, 256), 2, pos, pos, rope, err=e),
+                     lambda e: cache.read(pos, pos, err=e), lambda e: cache.attention(x, pos + 1, err=e),
+                     lambda e: acb.logits_rules(x.view(1, 256), err=e)):
+            with pytest.raises(ValueError):
+                call(bad)
+            call(good), call(good.data_ptr()), call(None)
+    assert int(good) == 0
