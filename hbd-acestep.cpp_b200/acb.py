@@ -672,6 +672,8 @@ def logits_rules(logits, hist=None, hist_len=None, prompt_len=None, rep=None, fr
         bias_stride = n_bias if bias_ids.dim() == 2 else 0
         if bias_ids.dim() > 2 or (bias_ids.dim() == 2 and bias_ids.shape[0] < R):
             raise ValueError("logits_rules: a bias list for every row, or one for all, is wanted")
+        if bias_val.shape[-1:] != bias_ids.shape[-1:] or (bias_ids.dim() < 2 and bias_val.numel() != n_bias):
+            raise ValueError("logits_rules: bias_val's lists are bias_ids', value by value")
     else:
         at_ids = None
     if mask is not None:

@@ -244,3 +244,16 @@ def test_host_threads_of_long_and_short_histories(cuda):
     torch.cuda.synchronize()
     for args, ref, out, st, seen, keep in jobs:
         assert seen == {0} and torch.equal(out, ref)
+
+
+def test_bias_lists_of_unlike_shapes_are_refused(cuda):
+    import torch
+    x = torch.zeros(2, 50).cuda()
+    i = lambda *s: torch.ones(s, dtype=torch.int32).cuda()  # noqa: E731
+    v = lambda *s: torch.ones(s).cuda()  # noqa: E731
+    for ids, val in ((i(2, 3), v(3, 2)), (i(2, 3), v(6)), (i(3), v(2, 3)), (i(2, 3), v(1, 3)), (i(3), v(2)), (i(1, 3), v(1, 3))):
+        with pytest.raises(ValueError):
+            acb.logits_rules(x, bias_ids=ids, bias_val=val)
+    for ids, val in ((i(2, 3), v(2, 3)), (i(3), v(3)), (i(3, 3), v(2, 3).repeat(2, 1)), (i(3), v(1, 3)), (i(2, 0), v(2, 0))):
+        y = acb.logits_rules(x, bias_ids=ids, bias_val=val)
+        assert bool((y[:, 1] == (1 if ids.numel() else 0)).all()) and int((y != 0).sum()) == (2 if ids.numel() else 0)
