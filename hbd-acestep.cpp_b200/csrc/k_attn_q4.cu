@@ -711,6 +711,9 @@ extern "C" acb_status acb_attn_kv_q4(const acb_kv_q4 * kv, const void * q, int t
         (int64_t) max_q_len * n_heads > (1 << 24)) {
         return ACB_ERR_UNSUPPORTED;
     }
+    if (q == o && n_tok > 1 && q_stride != o_stride) {
+        return ACB_ERR_INVALID_ARG;  // one buffer in two layouts would be written before it is read
+    }
     if (n_tok == 0) {
         return ACB_OK;
     }

@@ -528,6 +528,9 @@ extern "C" acb_status acb_kv_q4_append(const acb_kv_q4 * kv, const void * qkv, i
     if (!is_io_type(type) || (n_heads > 0 && !is_io_type(q_type)) || n_tok > std::min((int64_t) INT32_MAX, (int64_t) INT32_MAX * 8 / nh)) {
         return ACB_ERR_UNSUPPORTED;
     }
+    if (n_heads > 0 && q_out == qkv && (q_type != type || (n_tok > 1 && q_stride != stride))) {
+        return ACB_ERR_INVALID_ARG;  // one buffer in two layouts would be written before it is read
+    }
     if (n_tok == 0) {
         return ACB_OK;
     }

@@ -739,7 +739,8 @@ typedef struct acb_kv_q4 {
 
 /* Token t's row of qkv (type F32, F16 or BF16, stride elements apart) is [q(n_heads) | k(n_kv_heads) | v(n_kv_heads)]
  * heads of head_dim. q and k heads: RMSNorm times q_norm / k_norm (NULL: none), then the rotation of acb_rope by pos[t]
- * (rope_table NULL: none; layout without ACB_ROPE_INVERSE); q goes to q_out (q_type F32, F16 or BF16; n_heads 0: no q), k
+ * (rope_table NULL: none; layout without ACB_ROPE_INVERSE); q goes to q_out (q_type F32, F16 or BF16; n_heads 0: no q; the
+ * q part of qkv itself, with the same pointer, type and stride, or apart from it), k
  * and v into the cache at position pos[t] of sequence seq[t], each block of 32 quantised from its f32 values x as
  *   mx = the x of largest magnitude (positive where both signs have it),
  *   d  = f16(bf16(-mx / 8)) limited to +-2720,  code = min(15, max(0, floor(x / d + 8.5)))  (d 0: code 8).
@@ -770,7 +771,7 @@ ACB_API acb_status acb_kv_q4_read(const acb_kv_q4 * kv, const int32_t * seq, con
  * more rows than max_q_len, rows outside [0, n_tok) or kv_len outside [0, min(max_kv_len, max_pages*page_size)] raises
  * ACB_DEVERR_LEN_RANGE and its rows (the first max_q_len of them inside [0, n_tok)) are zeros; keys on a page outside the pool
  * raise ACB_DEVERR_PAGE_RANGE and take no part. q and o F32, F16 or BF16, the same type, *_stride elements between tokens,
- * heads contiguous. Scores, softmax and sums in f32. The keys of a long sequence are split over blocks and joined by a second
+ * heads contiguous; o is q itself (the same pointer and stride) or apart from it. Scores, softmax and sums in f32. The keys of a long sequence are split over blocks and joined by a second
  * kernel, through `work` (acb_attn_kv_q4_work_bytes, device, 16-byte aligned; smaller or NULL: not split). Calls that share a
  * workspace must not overlap. The result does not depend on what the workspace held. */
 ACB_API size_t     acb_attn_kv_q4_work_bytes(const acb_kv_q4 * kv, int64_t n_tok, int n_heads, int max_q_len,

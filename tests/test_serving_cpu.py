@@ -210,3 +210,12 @@ def test_workspaces_cover_every_count_of_rows(n_seq, n_kv, heads, D, first, last
     assert f(last) > 0
     for q in range(first, last):
         assert f(q) * last >= f(last) * q and f(q) <= f(last)
+
+
+@pytest.mark.parametrize("kw", [dict(q_stride=256), dict(q_type=acb.F16, q_stride=384)])
+def test_append_in_place_wants_one_layout(kw):
+    assert append(cache(), q_out=P, qkv=P, n_tok=2, stride=384, **kw) == 1
+
+
+def test_attention_in_place_wants_one_layout():
+    assert attn(cache(), q_stride=256, o_stride=300) == 1

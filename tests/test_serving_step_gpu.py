@@ -198,3 +198,37 @@ def test_flag_words_that_would_be_misread_are_refused(cuda):
                 call(bad)
             call(good), call(good.data_ptr()), call(None)
     assert int(good) == 0
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("n,D,R,layout", [(1, 128, 128, "half"), (3, 64, 10, "half"), (5, 256, 64, "interleaved"), (400, 128, 128, "half"),
+                                          (1500, 64, 64, "interleaved")])
+def test_queries_in_place(cuda, kind, n, D, R, layout):
+    """q written over the q part of qkv, and the attention's output over q: what separate buffers give."""
+    import torch
+    import serving_ref as S
+    g = torch.Generator().manual_seed(n + D)
+    Nh, Nkv, P, past = 10, 2, 16, 777
+    pages = -(-(n + past) // P)
+    table = torch.arange(pages, dtype=torch.int32).view(1, -1).cuda()
+    cache = acb.KVCacheQ4.empty(pages, P, Nkv, D, table)
+    rope = acb.rope_table_scaled(pages * P, R, 1e4).cuda()
+    w = (1 + 0.1 * torch.randn(D, generator=g)).cuda()
+    x = torch.randn(past + n, (Nh + 2 * Nkv) * D, generator=g).to(S.torch_type(kind)).cuda()
+    pos, seq = torch.arange(past + n, dtype=torch.int32).cuda(), torch.zeros(past + n, dtype=torch.int32).cuda()
+    cache.append(x[:past], Nh, seq[:past], pos[:past], rope, layout, w, w)
+    new, ln, start = x[past:], torch.tensor([past + n], dtype=torch.int32).cuda(), torch.tensor([0, n], dtype=torch.int32).cuda()
+    q = cache.append(new, Nh, seq[past:], pos[past:], rope, layout, w, w)
+    held = [t.clone() for t in cache.tensors[:4]]
+    o = cache.attention(q, ln, start, n)
+    buf = new.clone()
+    view = buf[:, :Nh * D].unflatten(1, (Nh, D))
+    assert cache.append(buf, Nh, seq[past:], pos[past:], rope, layout, w, w, q_out=view) is view
+    assert torch.equal(view, q) and torch.equal(buf[:, Nh * D:], new[:, Nh * D:])
+    assert all(torch.equal(a, b) for a, b in zip(held, cache.tensors))
+    for work in (None, torch.empty(1, dtype=torch.uint8).cuda()):  # the keys cut into chunks, and not
+        ref = cache.attention(q, ln, start, n, work=work)
+        view.copy_(q)
+        cache.attention(view, ln, start, n, out=view, work=work)
+        assert torch.equal(view, ref) and torch.equal(buf[:, Nh * D:], new[:, Nh * D:])
+    assert bool(o.isfinite().all())
