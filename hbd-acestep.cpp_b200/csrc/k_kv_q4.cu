@@ -525,7 +525,8 @@ extern "C" acb_status acb_kv_q4_append(const acb_kv_q4 * kv, const void * qkv, i
                        (layout != ACB_ROPE_HALF && layout != ACB_ROPE_INTERLEAVED))) {
         return ACB_ERR_INVALID_ARG;
     }
-    if (!is_io_type(type) || (n_heads > 0 && !is_io_type(q_type)) || n_tok > std::min((int64_t) INT32_MAX, (int64_t) INT32_MAX * 8 / nh)) {
+    if (!is_io_type(type) || (n_heads > 0 && !is_io_type(q_type)) || n_tok > std::min((int64_t) INT32_MAX, (int64_t) INT32_MAX * 8 / nh) ||
+        nh * D > (int64_t) INT32_MAX) {  // the kernels count within a row in 32 bits
         return ACB_ERR_UNSUPPORTED;
     }
     if (n_heads > 0 && q_out == qkv && (q_type != type || (n_tok > 1 && q_stride != stride))) {

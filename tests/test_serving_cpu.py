@@ -219,3 +219,8 @@ def test_append_in_place_wants_one_layout(kw):
 
 def test_attention_in_place_wants_one_layout():
     assert attn(cache(), q_stride=256, o_stride=300) == 1
+
+
+@pytest.mark.parametrize("heads", [(1 << 25) - 4, (1 << 25) - 3, 1 << 30, 2 ** 31 - 1])
+def test_append_refuses_rows_of_2_to_the_31_elements(heads):
+    assert append(cache(), n_heads=heads, stride=1 << 40, q_stride=1 << 40, q_out=P + 16) == 2
