@@ -4,7 +4,8 @@
 // 128. Every cached value is an f16 number, so nothing is rounded on the way into the tiles. 16 warps, the most that leave a
 // thread 128 registers:
 //   0..3, 4..7  softmax of tile 0 and of tile 1, a thread a row (a TMEM lane): 64 scores of half a block at a time, in registers
-//               once for the maximum and the exponentials; P goes back over them as f16;
+//               once for the maximum and the exponentials; P goes back over them as f16 (half a step of 2^-11 of each
+//               weight, as k_attn_q4.cu says; their sum is of the unrounded ones);
 //   8..11       unpacking V^T: a thread 8 keys by 16 dimensions: the words of two keys are merged by halves, so that unpack4
 //               gives pairs of keys, and four pairs make the 16-byte unit of a dimension;
 //   12, 13      unpacking K: a thread two keys; the 8 dimensions of a word of codes make one 16-byte unit in the order that

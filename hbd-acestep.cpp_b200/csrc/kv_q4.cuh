@@ -6,7 +6,9 @@
 
 namespace acb {
 
-constexpr float kQ4MaxScale = 2720.0f;  // 24 * 2720 is the largest multiple the unpacking forms that f16 holds
+// The format's limit of a scale, so of 8 * 2720 = 21760 for an element. f16 holds (code - 8) d up to d = 8160; the limit is part
+// of the format.
+constexpr float kQ4MaxScale = 2720.0f;
 
 struct KvQ4 {
     uint8_t *       kc;

@@ -771,8 +771,12 @@ ACB_API acb_status acb_kv_q4_read(const acb_kv_q4 * kv, const int32_t * seq, con
  * more rows than max_q_len, rows outside [0, n_tok) or kv_len outside [0, min(max_kv_len, max_pages*page_size)] raises
  * ACB_DEVERR_LEN_RANGE and its rows (the first max_q_len of them inside [0, n_tok)) are zeros; keys on a page outside the pool
  * raise ACB_DEVERR_PAGE_RANGE and take no part. q and o F32, F16 or BF16, the same type, *_stride elements between tokens,
- * heads contiguous; o is q itself (the same pointer and stride) or apart from it. Scores, softmax and sums in f32. The keys of a long sequence are split over blocks and joined by a second
- * kernel, through `work` (acb_attn_kv_q4_work_bytes, device, 16-byte aligned; smaller or NULL: not split). Calls that share a
+ * heads contiguous; o is q itself (the same pointer and stride) or apart from it. Scores, softmax and sums in f32. What the
+ * products take are f16 numbers: q times a power of two per row (F32: the sum of two numbers; what is far below the row's largest
+ * element is off by at most 2^-25 of that) and the weights (F32: the sum of two; F16 and BF16: one, half a step of 2^-11 of each weight).
+ * The keys of a long sequence are split over blocks and joined by a second kernel, through `work` (device, 16-byte aligned; smaller
+ * than needed or NULL: not split). acb_attn_kv_q4_work_bytes is enough for every call with this cache and n_heads and at most
+ * these tokens, rows and keys, whatever its window and its padding. Calls that share a
  * workspace must not overlap. The result does not depend on what the workspace held. */
 ACB_API size_t     acb_attn_kv_q4_work_bytes(const acb_kv_q4 * kv, int64_t n_tok, int n_heads, int max_q_len,
                                              int max_kv_len);

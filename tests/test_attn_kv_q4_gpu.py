@@ -561,3 +561,14 @@ def test_windows_of_more_than_all_keys(cuda, kind, n, L, window):
     ref = cache.attention(q, ln, start, n)
     assert torch.equal(cache.attention(q, ln, start, n, window=window), ref)
     _check(cache, q, ref, [n, n], [L, L // 2], 0, 128 ** -0.5, kind)
+
+
+@pytest.mark.parametrize("kind,D", [("bf16", 128), ("f16", 64), ("f32", 128), ("bf16", 256)])
+def test_repeated_calls_give_the_same_bits(cuda, kind, D):
+    """Prompts and single tokens, in either form, cut and not."""
+    import torch
+    rng = np.random.default_rng(D)
+    for q_lens, kv_lens in (([300, 200, 259], [2000, 300, 1111]), ([1, 1, 1], [4000, 3, 700])):
+        cache, q, ln, start, o = _run(rng, q_lens, kv_lens, 16, 4, 2, D, kind)
+        for _ in range(10):
+            assert torch.equal(cache.attention(q, ln, start, max(q_lens)), o)
