@@ -643,7 +643,8 @@ Plan make_plan(const acb_kv_q4 * kv, int n_heads, int max_q, int max_kv, int win
         p.rows    = INT64_MAX;
         return p;
     }
-    int64_t same = parts / splits;  // the most tasks with as many splits (at 4 or more parts of `slots` the rule above is the same one)
+    // The most tasks that give as many splits. (Where parts is slots these are 4 or more, so it is slots for those tasks too.)
+    int64_t same = parts / splits;
     if (least == 128 && same > num_sms() / 4) {
         same = num_sms() / 4;
     }
@@ -683,9 +684,9 @@ extern "C" size_t acb_attn_kv_q4_work_bytes(const acb_kv_q4 * kv, int64_t n_tok,
     const int64_t G    = n_heads / kv->n_kv_heads;
     size_t        most = 0;
     for (int64_t q = 1; q <= max_q_len; q++) {
-        const Plan p        = make_plan(kv, n_heads, (int) q, max_kv_len, 0);
-        q                   = std::min<int64_t>(max_q_len, p.rows / G);
-        const size_t bytes  = plan_bytes(p.most, kv, part_rows(kv, n_tok, q), n_heads);
+        const Plan p       = make_plan(kv, n_heads, (int) q, max_kv_len, 0);
+        q                  = std::min<int64_t>(max_q_len, p.rows / G);
+        const size_t bytes = plan_bytes(p.most, kv, part_rows(kv, n_tok, q), n_heads);
         most                = bytes > most ? bytes : most;
     }
     return most;
